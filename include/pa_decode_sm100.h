@@ -43,12 +43,15 @@ typedef enum PaDType {
   PA_DT_E4M3FN = 1            /* OCP e4m3fn, max 448 */
 } PaDType;
 
-/* Quantisation mode of a scale argument; the values are the reference's own
+/* Quantisation mode of a scale argument; the first three values are the reference's own
  * (pa_decode_triton_gluon_fp8.py:1752-1790). */
 typedef enum PaQuantMode {
   PA_QUANT_NONE = -1,         /* no scale */
   PA_QUANT_PER_TENSOR = 0,    /* pointer to ONE fp32 in device memory */
-  PA_QUANT_PER_TOKEN = 1      /* [num_blocks, num_kv_heads, block_size] fp32, last dim contiguous */
+  PA_QUANT_PER_TOKEN = 1,     /* [num_blocks, num_kv_heads, block_size] fp32, last dim contiguous */
+  PA_QUANT_PER_BLOCK = 2      /* [num_blocks, num_kv_heads] fp32 by kv_scale_stride_block / _head: one scale for the
+                               * tokens of a page and kv head (e4m3fn KV, partition_size 256).  max_logits then holds
+                               * the maximum of logit + log(value scale) and exp_sums the sum relative to it */
 } PaQuantMode;
 
 /* Value-cache layouts (pa_decode_triton_gluon_fp8.py:1792-1799). */
@@ -86,7 +89,7 @@ typedef struct PaDecodeParams {
   const int32_t* block_tables; /* [S, max_blocks_per_seq] */
   const int32_t* context_lens; /* [S] */
   const float* query_scale;    /* per-tensor [1] / per-token [S, Hkv*eqG]; NULL when PA_QUANT_NONE */
-  const float* key_scale;      /* per-tensor [1] / per-token [NB, Hkv, bs]; NULL when PA_QUANT_NONE */
+  const float* key_scale;      /* per-tensor [1] / per-token [NB, Hkv, bs] / per-block [NB, Hkv]; NULL when PA_QUANT_NONE */
   const float* value_scale;    /* same shape as key_scale */
   const float* alibi_slopes;   /* [Hkv*G] or NULL */
   const float* sink_tokens;    /* [Hkv*G] or NULL: one sink logit per query head; the reduce adds
@@ -139,7 +142,7 @@ typedef struct PaDecodeParams {
   int64_t v_stride_block, v_stride_head;
   int64_t bt_stride_seq;
   int64_t q_scale_stride_seq;              /* per-token query scale only */
-  int64_t kv_scale_stride_block, kv_scale_stride_head;  /* per-token kv scales only */
+  int64_t kv_scale_stride_block, kv_scale_stride_head;  /* per-token and per-block kv scales */
   int64_t ws_stride_seq, ws_stride_head, ws_stride_part;                   /* exp_sums / max_logits */
   int64_t tmp_stride_seq, tmp_stride_head, tmp_stride_part, tmp_stride_row;/* tmp_out */
 
@@ -168,6 +171,16 @@ typedef struct PaDecodeParams {
 /* Partition kernel followed by the reduce kernel on `stream` (a cudaStream_t); one launch that
  * does both when `merge_counters` is given and the shape allows it (see the field). */
 int pa_decode_sm100(const PaDecodeParams* params, void* stream);
+
+/*
+ * pa_decode_sm100 with a block table for each kv head (no counterpart in the reference): head h of
+ * sequence s reads entry i of its table at block_tables[s * bt_stride_seq + h * bt_stride_head + i].
+ * context_lens[s] counts the tokens in the pages of one such table, all heads alike: every page
+ * but the last is full.  bt_stride_head = 0: the heads share a table.  e4m3fn KV, partition_size
+ * 256, scales none, per tensor or per block; no alibi_slopes with bt_stride_head != 0 (a place in
+ * a head's table is no distance).
+ */
+int pa_decode_tables_sm100(const PaDecodeParams* params, int64_t bt_stride_head, void* stream);
 
 /* The partition kernel alone: fills exp_sums / max_logits / tmp_out, leaves `out` untouched. */
 int pa_partition_sm100(const PaDecodeParams* params, void* stream);

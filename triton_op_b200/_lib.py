@@ -8,13 +8,15 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+import torch
+
 from .build import LIB_PATH
 
 PA_ABI_VERSION = 3
 
 PA_OK = 0
 PA_DT_BF16, PA_DT_E4M3FN = 0, 1
-PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN = -1, 0, 1
+PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN, PA_QUANT_PER_BLOCK = -1, 0, 1, 2
 PA_V_NORMAL, PA_V_TRANSPOSED = 0, 1
 PA_DEV_WAIT_TIMEOUT, PA_DEV_BAD_PAGE_ID, PA_DEV_CTX_TOO_LONG = 1, 2, 4
 PA_TRACE_WORDS = 8 * 64 * 4
@@ -22,7 +24,7 @@ PA_NOALLOC_SCRATCH_BYTES = 16 << 20
 PA_IPC_HANDLE_BYTES = 64
 
 EXPORTS = (
-    "pa_decode_sm100", "pa_decode_noalloc_sm100", "pa_partition_sm100", "pa_reduce_sm100", "pa_merge_triples_sm100",
+    "pa_decode_sm100", "pa_decode_tables_sm100", "pa_decode_noalloc_sm100", "pa_partition_sm100", "pa_reduce_sm100", "pa_merge_triples_sm100",
     "pa_merge_packed_triples_sm100", "pa_packed_triple_floats", "pa_exchange_alloc", "pa_exchange_open", "pa_exchange_close", "pa_exchange_free",
     "pa_exchange_bytes", "pa_reduce_push_sm100", "pa_merge_wait_sm100",
     "pa_cache_write_sm100", "pa_stream_probe_sm100", "pa_query_launch_sm100", "pa_strerror", "pa_last_cuda_error", "pa_abi_version",
@@ -95,6 +97,8 @@ def lib() -> C.CDLL:
     P = C.POINTER(PaDecodeParams)
     L.pa_decode_sm100.argtypes = [P, C.c_void_p]
     L.pa_partition_sm100.argtypes = [P, C.c_void_p]
+    L.pa_decode_tables_sm100.argtypes = [P, C.c_int64, C.c_void_p]
+    L.pa_decode_tables_sm100.restype = C.c_int
     L.pa_decode_noalloc_sm100.argtypes = [P, C.c_void_p]
     L.pa_reduce_sm100.argtypes = [P, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     L.pa_merge_triples_sm100.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
@@ -132,6 +136,16 @@ def lib() -> C.CDLL:
         raise ImportError("libpa_decode_sm100.so was built from a different ABI version; rebuild it")
     _LIB = L
     return L
+
+
+def launch(device: torch.device, fn, where: str, *args) -> None:
+    """Calls a launching entry point with ``device`` current, on torch's current stream of it."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), where)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream), where)
 
 
 def check(status: int, where: str) -> None:

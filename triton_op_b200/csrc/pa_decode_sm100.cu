@@ -106,6 +106,7 @@ struct LaunchPlan {
   bool fused = false;        // tcgen05 kernel in its single-launch form: it also merges the partitions
   bool pair = false;         // tcgen05 kernel on 512-token partitions (two work items per partition)
   bool staged = false;       // tcgen05 kernel: per-token scales are staged in the query slots
+  bool blk = false;          // tcgen05 kernel: scales per (page, kv head) and / or block tables per kv head
   bool bf16_kv = false;      // bf16 KV cache (mma.sync bf16 kernel)
   int rows = 0;              // query rows per work item (tcgen05 kernel)
   int grid = 0;
@@ -144,7 +145,8 @@ int validate(const PaDecodeParams* p, bool need_partition_inputs, bool need_out)
 
 // allow_fuse: the caller wants the whole decode (partitions and their merge) and would take it as
 // one launch where the kernel has that form.
-int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false) {
+// bt_stride_head: elements from one kv head's block table to the next; 0: the heads share one.
+int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false, int64_t bt_stride_head = 0) {
   int rc = validate(p, true, false);
   if (rc != PA_OK) return rc;
   DeviceInfo* dev = nullptr;
@@ -158,6 +160,15 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   const bool bf16_kv = p->kv_dtype == PA_DT_BF16;
   const int kv_item = bf16_kv ? 2 : 1;  // bytes per cache element
   if (bf16_kv && p->kv_quant_mode == PA_QUANT_PER_TOKEN) return PA_ERR_UNSUPPORTED;
+  if (p->kv_quant_mode < PA_QUANT_NONE || p->kv_quant_mode > PA_QUANT_PER_BLOCK) return PA_ERR_UNSUPPORTED;
+  // Scales per (page, kv head), or tables per kv head: the tcgen05 kernel's BLK form, 256-token partitions.
+  const bool blk = p->kv_quant_mode == PA_QUANT_PER_BLOCK || bt_stride_head != 0;
+  if (blk) {
+    if (bf16_kv || p->partition_size != pa::tc::kItemTokens || p->tune_warps != 0) return PA_ERR_UNSUPPORTED;
+    if (p->kv_quant_mode == PA_QUANT_PER_TOKEN) return PA_ERR_UNSUPPORTED;
+    // a key position inside a head's own table is not the token's distance from the end
+    if (bt_stride_head != 0 && p->alibi_slopes != nullptr) return PA_ERR_UNSUPPORTED;
+  }
   if (p->block_size != 16 && p->block_size != 64 && p->block_size != 1024) return PA_ERR_UNSUPPORTED;
   // Transposed values [NB, Hkv, bs/16, D, 16] (e4m3): a 16-token page is the same bytes as the
   // normal layout; longer pages are served by the tcgen05 kernel as 2 KB runs.
@@ -169,7 +180,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   // kernel, which also covers other partition sizes for 16-token pages and up to 16 query rows.
   // 512-token partitions run on it too (as pairs of 256-token items merged in the epilogue) with
   // up to 16 query rows and no ALiBi.
-  const bool pair = !bf16_kv && p->partition_size == 2 * pa::tc::kItemTokens && p->tune_warps == 0 && eqG <= 16 &&
+  const bool pair = !bf16_kv && !blk && p->partition_size == 2 * pa::tc::kItemTokens && p->tune_warps == 0 && eqG <= 16 &&
                     p->alibi_slopes == nullptr && p->trace == nullptr;
   const bool tensor_path = !bf16_kv && (p->partition_size == pa::tc::kItemTokens || pair) && p->tune_warps == 0;
   if (!tensor_path) {
@@ -229,6 +240,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   k.v_stride_block = p->v_stride_block * kv_item;
   k.v_stride_head = p->v_stride_head * kv_item;
   k.bt_stride_seq = p->bt_stride_seq;
+  k.bt_stride_head = bt_stride_head;
   k.q_scale_stride_seq = p->q_scale_stride_seq;
   k.kvs_stride_block = p->kv_scale_stride_block;
   k.kvs_stride_head = p->kv_scale_stride_head;
@@ -241,6 +253,13 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   k.tmp_stride_row = p->tmp_stride_row;
   k.q_quant_mode = p->q_quant_mode;
   k.kv_quant_mode = p->kv_quant_mode;
+  plan->blk = blk;
+  if (blk) {
+    // the BLK form applies every scale itself: a per-tensor one is a block scale with strides of zero
+    if (p->kv_quant_mode == PA_QUANT_NONE) k.k_scale = k.v_scale = nullptr;
+    if (p->kv_quant_mode != PA_QUANT_PER_BLOCK) k.kvs_stride_block = k.kvs_stride_head = 0;
+    k.kv_quant_mode = PA_QUANT_PER_BLOCK;
+  }
   k.softmax_scale = p->softmax_scale;
 
   plan->per_token = per_token;
@@ -269,7 +288,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
     // Single launch: one row block per (partition, head), every row's partitions within one chunk
     // of the merge (32), and a counter array for the row sets that are cut by the end of a team's range.
     plan->pair = pair;
-    plan->fused = allow_fuse && !pair && p->merge_counters != nullptr && p->out != nullptr && nrb == 1 && qr <= 8 &&
+    plan->fused = allow_fuse && !pair && !blk && p->merge_counters != nullptr && p->out != nullptr && nrb == 1 && qr <= 8 &&
                   p->max_partitions <= 32 && p->alibi_slopes == nullptr && p->trace == nullptr && p->tune_fuse > 0;
     if (plan->fused) {
       k.out = static_cast<uint8_t*>(p->out);
@@ -299,7 +318,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
     for (int attempt = 0; attempt < 2 && !placed; ++attempt) {
     const bool staged = want_staged && attempt == 0;
     if (attempt == 1 && (!want_staged || pair)) break;     // nothing else to try
-    const int qslot = pa::tc::q_slot_bytes(qr, staged);
+    const int qslot = pa::tc::q_slot_bytes(qr, staged) + (blk ? pa::tc::kQBlockScales : 0);
     for (const auto& d : kDepths) {
       if (p->tune_stages > 0 && d[0] > p->tune_stages) continue;
       if (p->tune_vstages > 0 && d[1] != p->tune_vstages) continue;
@@ -397,9 +416,10 @@ int launch_partition_t(const LaunchPlan& plan, cudaStream_t stream) {
   return PA_OK;
 }
 
-template <int BS, int QR, bool PT, bool TRACE, bool ALIBI = false, bool FUSE = false, bool PAIR = false, bool STAGE = true>
+template <int BS, int QR, bool PT, bool TRACE, bool ALIBI = false, bool FUSE = false, bool PAIR = false, bool STAGE = true,
+          bool BLK = false>
 int launch_tensor_t(const LaunchPlan& plan, cudaStream_t stream) {
-  auto kern = pa::tc::pa_partition_fp8_tc_kernel<BS, QR, PT, TRACE, ALIBI, FUSE, PAIR, STAGE>;
+  auto kern = pa::tc::pa_partition_fp8_tc_kernel<BS, QR, PT, TRACE, ALIBI, FUSE, PAIR, STAGE, BLK>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
   if (e != cudaSuccess) return cuda_fail(e);
   // Programmatic dependent launch: in a decode loop the CTAs may become resident and set up their
@@ -425,6 +445,21 @@ int launch_tensor_t(const LaunchPlan& plan, cudaStream_t stream) {
 template <int BS, bool TRACE>
 int launch_tensor_bs(const LaunchPlan& plan, cudaStream_t stream) {
   const bool pt = plan.per_token;
+  if constexpr (!TRACE) {
+    if (plan.blk) {                           // block scales, tables per kv head
+      const bool al = plan.kp.alibi != nullptr;
+#define PA_BLK(QR) \
+  return al ? launch_tensor_t<BS, QR, false, false, true, false, false, true, true>(plan, stream) \
+            : launch_tensor_t<BS, QR, false, false, false, false, false, true, true>(plan, stream)
+      switch (plan.rows) {
+        case 4: PA_BLK(4);
+        case 8: PA_BLK(8);
+        case 16: PA_BLK(16);
+        default: return PA_ERR_UNSUPPORTED;
+      }
+#undef PA_BLK
+    }
+  }
   if (!TRACE && plan.fused) {                 // the single-launch instantiations (4 or 8 rows per item)
     if (plan.rows == 4)
       return pt ? launch_tensor_t<BS, 4, true, false, false, true>(plan, stream) : launch_tensor_t<BS, 4, false, false, false, true>(plan, stream);
@@ -473,13 +508,13 @@ int launch_partition(const LaunchPlan& plan, cudaStream_t stream) {
     switch (plan.kp.block_size) {
       case 16:
 #ifdef PA_TRACE_BUILD   // tuning builds (-DPA_TRACE_BUILD): clock stamps compiled in (pages of 16 and of 1024 tokens)
-        if (plan.kp.trace != nullptr) return launch_tensor_bs<16, true>(plan, stream);
+        if (plan.kp.trace != nullptr && !plan.blk) return launch_tensor_bs<16, true>(plan, stream);
 #endif
         return launch_tensor_bs<16, false>(plan, stream);
       case 64: return launch_tensor_bs<64, false>(plan, stream);
       case 1024:
 #ifdef PA_TRACE_BUILD
-        if (plan.kp.trace != nullptr) return launch_tensor_bs<1024, true>(plan, stream);
+        if (plan.kp.trace != nullptr && !plan.blk) return launch_tensor_bs<1024, true>(plan, stream);
 #endif
         return launch_tensor_bs<1024, false>(plan, stream);
       default: return PA_ERR_UNSUPPORTED;
@@ -616,6 +651,18 @@ int pa_decode_sm100(const PaDecodeParams* params, void* stream) {
   if (rc != PA_OK) return rc;
   rc = launch_partition(plan, static_cast<cudaStream_t>(stream));
   if (rc != PA_OK || plan.fused) return rc;   // the single-launch kernel has merged the partitions itself
+  return launch_reduce(params, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int pa_decode_tables_sm100(const PaDecodeParams* params, int64_t bt_stride_head, void* stream) {
+  if (bt_stride_head < 0) return PA_ERR_BAD_SHAPE;
+  LaunchPlan plan;
+  int rc = make_plan(params, &plan, false, bt_stride_head);
+  if (rc != PA_OK) return rc;
+  rc = validate(params, true, true);
+  if (rc != PA_OK) return rc;
+  rc = launch_partition(plan, static_cast<cudaStream_t>(stream));
+  if (rc != PA_OK) return rc;
   return launch_reduce(params, nullptr, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
 

@@ -43,6 +43,7 @@ struct KernelParams {
   int64_t k_stride_block, k_stride_head;
   int64_t v_stride_block, v_stride_head;
   int64_t bt_stride_seq;
+  int64_t bt_stride_head;      // 0: one table row for all kv heads of a sequence (read by the BLK form of the tcgen05 kernel only)
   int64_t q_scale_stride_seq;
   int64_t kvs_stride_block, kvs_stride_head;
   int64_t ws_stride_seq, ws_stride_head, ws_stride_part;

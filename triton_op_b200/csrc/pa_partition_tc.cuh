@@ -115,6 +115,8 @@ __host__ __device__ constexpr bool staged_token_scales(int block_size, bool per_
 __host__ __device__ constexpr int q_slot_bytes(int qr, bool staged_scales) {
   return q_tile_bytes(qr) + kQTokScales + (staged_scales ? 2 * kItemTokens * 4 : 0);
 }
+// Block scales: the item's 16 key scales and 16 value scales (one each for every page it touches).
+constexpr int kQBlockScales = 2 * 16 * 4;
 // P^T tile of one item, an MN-major operand: the 16 tile rows (N) of one token are 16 consecutive bytes, the
 // tokens (K) of an 8-token core matrix are 16 bytes apart and core matrices follow one another,
 // so token t of the item sits at t * 16 and a softmax thread stores its token's bytes of a
@@ -541,17 +543,29 @@ struct Geo {
 // second half's epilogue merges the two and stores the partition (see the epilogue).
 // STAGE: per-token scales of pages of 64 tokens or more travel in the query slots (see q_slot_bytes);
 // false where the host found no room for that.
-template <int BS, int QR, bool PER_TOKEN, bool TRACE, bool ALIBI = false, bool FUSE = false, bool PAIR = false, bool STAGE = true>
+// BLK: one K and one V scale for each (page, kv head), and block tables that may differ between kv
+// heads (p.bt_stride_head).  The query producer brings the item's scales into its slot with 4-byte
+// asynchronous copies (at most 16 + 16 of them; they complete the slot's barrier).  The key scale
+// multiplies the product; the value scale goes into the EXPONENT, as log2(scale) added to the base-2
+// logit, so the probabilities that meet e4m3 are exp2(s_j + log2 vs_j - max_j(s_j + log2 vs_j)): their
+// largest is at the top of the type's range whichever page holds it, and a page whose values are
+// thousands of times smaller than its neighbour's keeps its digits when it holds the weight.
+// The row sum divides the scale out again in fp32.  The partition's "maximum" is then that of the
+// shifted logits; (max, sum) stay consistent, which is all that the reduce needs.
+template <int BS, int QR, bool PER_TOKEN, bool TRACE, bool ALIBI = false, bool FUSE = false, bool PAIR = false, bool STAGE = true,
+          bool BLK = false>
 __global__ void __launch_bounds__(kThreads, 1)
 pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<BS>;
   static_assert(!FUSE || (QR <= 8 && !ALIBI && !TRACE), "the single-launch form exists for 4- and 8-row items");
   static_assert(!PAIR || (!FUSE && !ALIBI && !TRACE), "the PAIR form is plain");
+  static_assert(!BLK || (!PER_TOKEN && !FUSE && !PAIR && !TRACE), "block scales exist in the two-launch form");
+  constexpr bool kFinished = ALIBI || BLK;   // the logits that the maxima are taken of are complete (factor and per-token term applied)
   constexpr int NG = kNG;
   constexpr bool kSum = sums_in_tensor_core(QR);   // hi and lo products summed by the tensor core
   constexpr int N = acc_n(QR);                 // MMA N and TMEM columns per tile
   constexpr bool kStaged = STAGE && staged_token_scales(BS, PER_TOKEN) && !(PAIR && QR == 16);
-  constexpr int kQSlotBytes = q_slot_bytes(QR, kStaged);
+  constexpr int kQSlotBytes = q_slot_bytes(QR, kStaged) + (BLK ? kQBlockScales : 0);
   constexpr bool kItemFromSlot = PA_ITEM_FROM_SLOT && (!PER_TOKEN || kStaged);
   constexpr bool kKeepInTmem = sums_in_tensor_core(QR);   // two chunks of rows, one accumulator column per row
   constexpr int kQTile = q_tile_bytes(QR);
@@ -586,7 +600,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
   if (tid == 0) {
     for (int s = 0; s < kMaxSlots; ++s) {
       mbar_init(bar(kBarKFull, s), 1);
-      mbar_init(bar(kBarQFull, s), 1);
+      mbar_init(bar(kBarQFull, s), BLK ? 33 : 1);   // block scales: every lane's copies arrive too
       mbar_init(bar(kBarVFull, s), 1);
       mbar_init(bar(kBarQEmpty, s), 4);
     }
@@ -698,7 +712,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
   // after the load would make them wait for it there), so clamping is a separate step.
   auto page_id_raw = [&](const TcItem& it, int pg) -> int {
     const int64_t col = BS >= kItemTokens ? (int64_t)(it.tok0 / BS) : (int64_t)(it.tok0 / BS + pg);
-    return __ldg(p.block_tables + (int64_t)it.seq * p.bt_stride_seq + col);
+    return __ldg(p.block_tables + (int64_t)it.seq * p.bt_stride_seq + (BLK ? (int64_t)it.head * p.bt_stride_head : 0) + col);
   };
   auto clamp_page = [&](int id, bool report) -> int {
     if ((unsigned)id >= (unsigned)p.num_blocks) {
@@ -858,6 +872,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
     // tokens, or four of 64); its block-table entry is fetched an item ahead
     constexpr int kScalePages = BS >= kItemTokens ? 1 : kItemTokens / (BS >= 64 ? BS : 64);
     auto scale_page_id = [&](const TcItem& it) -> int {
+      if (BLK) return (lane & 15) < pages_of(it) ? page_id_raw(it, lane & 15) : 0;   // lanes 0-15 key scales, 16-31 value scales
       return (kStaged && lane < kScalePages && lane < pages_of(it)) ? page_id_raw(it, lane) : 0;
     };
     int spid_next = 0;
@@ -941,6 +956,15 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
           bulk_g2s(dst, p.k_scale + idx, kRun, bar(kBarQFull, slot), pol);
           bulk_g2s(dst + kItemTokens * 4, p.v_scale + idx, kRun, bar(kBarQFull, slot), pol);
         }
+      }
+      if (BLK) {
+        const uint32_t dst = item_aux + kQTokScales + lane * 4;
+        const float* src = lane < 16 ? p.k_scale : p.v_scale;
+        if (src != nullptr && (lane & 15) < pages_of(it))
+          cp_async4(dst, src + (int64_t)clamp_page(spid, false) * p.kvs_stride_block + (int64_t)it.head * p.kvs_stride_head);
+        else
+          sts32(dst, __float_as_uint(1.0f));   // a page without tokens of the context, or a cache without scales
+        cp_async_arrive(bar(kBarQFull, slot));
       }
       // (rolled: the code of every role's loop should stay resident in the instruction cache)
 #pragma unroll 1
@@ -1216,6 +1240,23 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         ks_tok[0] = tok_scales[0], ks_tok[1] = tok_scales[1];
         vs_tok[0] = tok_scales[2], vs_tok[1] = tok_scales[3];
       }
+      // Block scales: key scale, log2 of the value scale and its reciprocal for this lane's two tokens.
+      // (Value scales below 2^-100 are read as that; a page of zeros needs none smaller.)
+      float ks_blk[2] = {1.f, 1.f}, lv_blk[2] = {0.f, 0.f}, iv_blk[2] = {1.f, 1.f};
+      if (BLK) {
+#pragma unroll
+        for (int tg = 0; tg < 2; ++tg) {
+          if (tg == 1 && BS != 64) {   // tokens of one lane share a page unless pages hold 64 tokens
+            ks_blk[1] = ks_blk[0], lv_blk[1] = lv_blk[0], iv_blk[1] = iv_blk[0];
+          } else {
+            const int pg = BS == 16 ? (tok[tg] >> 4) : (BS == 64 ? (tok[tg] >> 6) : 0);
+            ks_blk[tg] = __uint_as_float(lds32(item_aux + kQTokScales + pg * 4));
+            const float vs = fmaxf(__uint_as_float(lds32(item_aux + kQTokScales + (16 + pg) * 4)), 0x1p-100f);
+            lv_blk[tg] = __log2f(vs);
+            iv_blk[tg] = __fdividef(1.0f, vs);
+          }
+        }
+      }
       fence_after_sync();
       if (wq == 0) stamp(6, i, 0);
 
@@ -1243,7 +1284,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
           for (int q = 0; q < RC; ++q) {
             float v = row_value(h[tg], l[tg], q);
             if (PER_TOKEN) v *= ks_tok[tg];
-            if (ALIBI) v = fmaf(v, row_scale[q], slope[q] * rel_pos[tg]);
+            if (BLK) v = fmaf(v * ks_blk[tg], row_scale[q], ALIBI ? fmaf(slope[q], rel_pos[tg], lv_blk[tg]) : lv_blk[tg]);
+            else if (ALIBI) v = fmaf(v, row_scale[q], slope[q] * rel_pos[tg]);
             s[tg][q] = room[tg] > lim[q] ? v : -INFINITY;
           }
         }
@@ -1284,8 +1326,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         const float4 m4 = *reinterpret_cast<const float4*>(rm + r * 4);
         const float m = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
         const float sc = __uint_as_float(lds32(aux + r * 4));
-        row_off[grp * 16 + r] = (m == -INFINITY) ? 8.0f : (ALIBI ? 8.0f - m : fmaf(-m, sc, 8.0f));
-        m_fin[par * 16 + r] = (m == -INFINITY || ALIBI) ? m : m * sc;
+        row_off[grp * 16 + r] = (m == -INFINITY) ? 8.0f : (kFinished ? 8.0f - m : fmaf(-m, sc, 8.0f));
+        m_fin[par * 16 + r] = (m == -INFINITY || kFinished) ? m : m * sc;
       }
       named_barrier_sync(bar_a, 128);
       float vinv = 1.0f, vnorm = 1.0f;
@@ -1341,14 +1383,14 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         for (int q = 0; q < RC; ++q) {
           // exponent argument raw * factor - m * factor + 8 as one multiply-add per element
           float p0, p1;
-          if (ALIBI) {   // s_keep holds finished logits
+          if (kFinished) {   // s_keep holds finished logits
             p0 = ex2(s_keep[0][q] + offs[q]);
             p1 = ex2(s_keep[1][q] + offs[q]);
           } else {
             p0 = ex2(fmaf(s_keep[0][q], row_scale[q], offs[q]));
             p1 = ex2(fmaf(s_keep[1][q], row_scale[q], offs[q]));
           }
-          psum[q] = p0 + p1;
+          psum[q] = BLK ? fmaf(p0, iv_blk[0], p1 * iv_blk[1]) : p0 + p1;   // (block scales: the value scale divided out again)
           split_parts<kSum>(PER_TOKEN ? p0 * vs_tok[0] : p0, hi[0][q], lo[0][q]);
           split_parts<kSum>(PER_TOKEN ? p1 * vs_tok[1] : p1, hi[1][q], lo[1][q]);
         }

@@ -15,6 +15,7 @@ ABI (``include/pa_decode_sm100.h``) on torch's current stream.  No synchronisati
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -140,7 +141,17 @@ def _kv_scale(scale, other, name: str, device) -> Tuple[Optional[torch.Tensor], 
         _fail(f"Expected 4D {name} tensor, but got shape {tuple(scale.shape)}")
     if not (scale.shape[-1] == 1):
         _fail(f"Expected {name}.shape[-1] == 1, but got {name}.shape[-1]={scale.shape[-1]}")
+    if scale.shape[2] == 1:   # (pages hold 16 tokens or more, so this is no per-token scale)
+        return scale, _lib.PA_QUANT_PER_BLOCK
     return scale, _lib.PA_QUANT_PER_TOKEN
+
+
+def _by_block(key_scale, value_scale, block_tables) -> bool:
+    """Scales per (page, kv head), or block tables per kv head: the forms whose calls keep nothing
+    for the next one (no cached parameters, workspaces of the call's own)."""
+    if isinstance(block_tables, torch.Tensor) and block_tables.dim() == 3:
+        return True
+    return any(isinstance(s, torch.Tensor) and s.dim() == 4 and s.shape[2] == 1 for s in (key_scale, value_scale))
 
 
 _PARAM_CACHE: Dict[tuple, PaDecodeParams] = {}
@@ -177,7 +188,7 @@ def build_params(output, query, key_cache, value_cache, sequence_lengths, block_
     """Validated C parameter block for the arguments, from a small cache when the same tensors
     (addresses, shapes, strides, dtypes) and scalars were validated before."""
     key = None
-    if tune is None:
+    if tune is None and not _by_block(key_scale, value_scale, block_tables):
         key = _params_key(output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
                           query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale,
                           value_scale, alibi_slopes, partition_size, exp_sums, max_logits, tmp_output, status,
@@ -310,6 +321,8 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
         v_scale_t, v_mode = _kv_scale(value_scale, key_scale, "value_scale", dev)
         if not (kv_mode == v_mode and tuple(k_scale_t.shape) == tuple(v_scale_t.shape)):
             _fail(f"Key and value scales must have same shape, but got key: {tuple(k_scale_t.shape)}, value: {tuple(v_scale_t.shape)}")
+        if kv_mode == _lib.PA_QUANT_PER_BLOCK:
+            _check_block_scales(k_scale_t, v_scale_t, key_cache, dev)
         if kv_mode == _lib.PA_QUANT_PER_TOKEN:
             if not (tuple(k_scale_t.shape[:3]) == (num_blocks, num_kv_heads, kv_block_size)):
                 _fail("per-token kv scales must be [num_blocks, num_kv_heads, block_size, 1]")
@@ -325,6 +338,8 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     if (own_workspaces and partition_size > SEQUENCE_PARTITION_SIZE and partition_size % SEQUENCE_PARTITION_SIZE == 0
             and kv_dtype == _lib.PA_DT_E4M3FN and not (tune and tune.get("warps"))):
         partition_size = SEQUENCE_PARTITION_SIZE
+    if kv_mode == _lib.PA_QUANT_PER_BLOCK and (partition_size != SEQUENCE_PARTITION_SIZE or (tune and tune.get("warps"))):
+        _fail(f"block kv scales run in partitions of {SEQUENCE_PARTITION_SIZE} tokens, but got partition_size {partition_size}")
     max_partitions = max(1, (int(max_sequence_length) + partition_size - 1) // partition_size)
     if exp_sums is None or max_logits is None or tmp_output is None:
         ws = get_workspaces(num_seqs, num_kv_heads, max_partitions, eq_group, head_size, output.dtype, dev)
@@ -376,7 +391,7 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     p.v_stride_block, p.v_stride_head = value_cache.stride(0), value_cache.stride(1)
     p.bt_stride_seq = block_tables.stride(0)
     p.q_scale_stride_seq = q_scale_stride
-    if kv_mode == _lib.PA_QUANT_PER_TOKEN:
+    if kv_mode in (_lib.PA_QUANT_PER_TOKEN, _lib.PA_QUANT_PER_BLOCK):
         p.kv_scale_stride_block, p.kv_scale_stride_head = k_scale_t.stride(0), k_scale_t.stride(1)
     p.ws_stride_seq, p.ws_stride_head, p.ws_stride_part = exp_sums.stride(0), exp_sums.stride(1), exp_sums.stride(2)
     p.tmp_stride_seq, p.tmp_stride_head = tmp_output.stride(0), tmp_output.stride(1)
@@ -398,6 +413,152 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     cacheable = all(u is g or (isinstance(u, torch.Tensor) and isinstance(g, torch.Tensor)
                                and u.data_ptr() == g.data_ptr()) for u, g in zip(used, given))
     return p, keep, cacheable
+
+
+def _check_block_scales(k_scale, v_scale, key_cache, dev) -> None:
+    want = (key_cache.shape[0], key_cache.shape[1], 1, 1)
+    if not (k_scale.shape == want and v_scale.shape == want):
+        _fail(f"block kv scales must be [num_blocks, num_kv_heads, 1, 1] = {want}")
+    if not (k_scale.stride()[:2] == v_scale.stride()[:2]):
+        _fail("block kv scales must share strides")
+    if not (k_scale.device == dev and v_scale.device == dev):
+        _fail(f"block kv scales must live on {dev}, the output's device")
+    if not (key_cache.dtype == FP8_DTYPE):
+        _fail(f"block kv scales need a {FP8_DTYPE} cache, but got key_cache.dtype == {key_cache.dtype}")
+
+
+# PaDecodeParams as one packed record: filling the block field by field costs more host time than a
+# small call takes on the GPU.
+_PACK = struct.Struct("=2I17Q10i19q6if6i4x")
+assert _PACK.size == C.sizeof(PaDecodeParams)
+
+
+def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
+                    query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,
+                    alibi_slopes, sink_tokens, status):
+    """(parameter block, elements between the kv heads' tables, tensors to keep alive, workspaces) of
+    a call with scales per (page, kv head) and / or a block table per kv head."""
+    if not isinstance(output, torch.Tensor):
+        _fail("output must be a torch.Tensor")
+    dev = output.device
+    if not (output.dim() == 3 and output.dtype == torch.bfloat16):
+        _fail(f"Expected a 3D bfloat16 output tensor, but got {output.dtype} of shape {tuple(output.shape)}")
+    if query.shape != output.shape:
+        _fail("output and query must have the same shape")
+    if key_cache.dim() != 5:
+        _fail(f"Expected 5D key_cache tensor, but got shape {tuple(key_cache.shape)}")
+    if not (key_cache.dtype == FP8_DTYPE and value_cache.dtype == FP8_DTYPE):
+        _fail(f"block kv scales and block tables per kv head need {FP8_DTYPE} caches, but got {key_cache.dtype} and {value_cache.dtype}")
+    if not _compute_type_matches(compute_type, torch.bfloat16):
+        _fail(f"compute_type {compute_type} disagrees with output.dtype {output.dtype}")
+    q_dtype = _dtype_code(query.dtype, "query")
+    if not (sequence_lengths.dtype == torch.int32 and block_tables.dtype == torch.int32):
+        _fail("sequence_lengths and block_tables must be int32")
+    for name, t in (("query", query), ("key_cache", key_cache), ("value_cache", value_cache),
+                    ("sequence_lengths", sequence_lengths), ("block_tables", block_tables)):
+        if t.device != dev:
+            _fail(f"{name} must live on {dev}, the output's device")
+    ql = int(query_sequence_length)
+    if not 1 <= ql <= 4:
+        _fail(f"QUERY_SEQ_LEN={ql}, only 1 to 4 are supported")
+    num_seqs, q_heads, head_size = query.shape
+    num_blocks, num_kv_heads, dx, bs, x = key_cache.shape
+    if not (x == 16 and dx * x == head_size):
+        _fail("key_cache must be [num_blocks, num_kv_heads, head_size/16, block_size, 16]")
+    if bs not in SUPPORTED_BLOCK_SIZES:
+        _fail(f"kv_block_size == {bs} not in {list(SUPPORTED_BLOCK_SIZES)}")
+    if head_size != 128:
+        _fail(f"head_size must be 128, but got {head_size}")
+    group = q_heads // (ql * num_kv_heads)
+    if group * ql * num_kv_heads != q_heads or group < 1:
+        _fail("query heads must be num_kv_heads * query_sequence_length * group_size")
+    if group * ql > 64:
+        _fail(f"equivalent query group size {group * ql} exceeds maximum of 64")
+    if value_cache.dim() == 4:
+        v_layout, want_v = _lib.PA_V_NORMAL, (num_blocks, num_kv_heads, head_size, bs)
+    else:
+        v_layout, want_v = _lib.PA_V_TRANSPOSED, (num_blocks, num_kv_heads, bs // 16, head_size, 16)
+    if value_cache.shape != want_v:
+        _fail(f"value_cache must be {want_v}")
+    per_head = block_tables.dim() == 3
+    if not (block_tables.dim() in (2, 3) and block_tables.shape[0] == num_seqs and sequence_lengths.numel() == num_seqs):
+        _fail("block_tables must be [num_seqs, max_blocks] or [num_seqs, num_kv_heads, max_blocks] and sequence_lengths [num_seqs]")
+    if per_head and block_tables.shape[1] != num_kv_heads:
+        _fail("block_tables with a table per kv head must be [num_seqs, num_kv_heads, max_blocks]")
+    if per_head and alibi_slopes is not None:
+        _fail("alibi_slopes with a block table per kv head: a place in a head's table is no distance")
+    if output.stride(2) != 1:
+        _fail("output's last dim must be contiguous")
+    if query.stride(2) != 1 or query.stride(1) != head_size:
+        query = query.contiguous()
+    if not (_inner_contiguous(key_cache, 2) and _inner_contiguous(value_cache, 2)):
+        _fail("the per-(block, head) slabs of the KV caches must be contiguous")
+    if sequence_lengths.dim() != 1 or sequence_lengths.stride(0) != 1:
+        sequence_lengths = sequence_lengths.reshape(-1).contiguous()
+    if block_tables.stride(-1) != 1 or (per_head and num_kv_heads > 1 and block_tables.stride(1) <= 0):
+        block_tables = block_tables.contiguous()
+
+    q_ptr = 0
+    q_mode, q_scale_stride = _lib.PA_QUANT_NONE, 0
+    if query_scale is not None:
+        if isinstance(query_scale, (int, float)):
+            query_scale = _scalar_on_device(float(query_scale), dev)
+        if not (query_scale.dtype == torch.float32 and query_scale.device == dev):
+            _fail(f"query_scale must be a float32 tensor on {dev}")
+        if query_scale.dim() == 0:
+            q_mode = _lib.PA_QUANT_PER_TENSOR
+        else:
+            if query_scale.shape != (num_seqs, q_heads, 1):
+                _fail(f"Expected query_scale [num_seqs, heads, 1], but got shape {tuple(query_scale.shape)}")
+            if query_scale.stride(1) != 1:
+                query_scale = query_scale.contiguous()
+            q_mode, q_scale_stride = _lib.PA_QUANT_PER_TOKEN, query_scale.stride(0)
+        q_ptr = query_scale.data_ptr()
+    if (key_scale is None) != (value_scale is None):
+        _fail("key_scale and value_scale go together")
+    kv_mode, ks_ptr, vs_ptr, s_block, s_head = _lib.PA_QUANT_NONE, 0, 0, 0, 0
+    if key_scale is not None:
+        key_scale, kv_mode = _kv_scale(key_scale, value_scale, "key_scale", dev)
+        value_scale, v_mode = _kv_scale(value_scale, key_scale, "value_scale", dev)
+        if kv_mode != v_mode:
+            _fail(f"Key and value scales must have same shape, but got key: {tuple(key_scale.shape)}, value: {tuple(value_scale.shape)}")
+        if kv_mode == _lib.PA_QUANT_PER_TOKEN:
+            _fail("a block table per kv head goes with no scales, per-tensor scales or block scales")
+        if kv_mode == _lib.PA_QUANT_PER_BLOCK:
+            _check_block_scales(key_scale, value_scale, key_cache, dev)
+            s_block, s_head = key_scale.stride(0), key_scale.stride(1)
+        elif not (key_scale.device == dev and value_scale.device == dev):
+            _fail(f"key_scale and value_scale must live on {dev}, the output's device")
+        ks_ptr, vs_ptr = key_scale.data_ptr(), value_scale.data_ptr()
+    for name, t in (("alibi_slopes", alibi_slopes), ("sink_tokens", sink_tokens)):
+        if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == dev
+                                  and t.numel() == num_kv_heads * group and t.is_contiguous()):
+            _fail(f"{name} must be a contiguous fp32 tensor with one value per query head on the output's device")
+    if status is not None and not (status.dtype == torch.int32 and status.device == dev):
+        _fail(f"status must be an int32 tensor on {dev}")
+
+    rows = group * ql
+    parts = max(1, -(-int(max_sequence_length) // SEQUENCE_PARTITION_SIZE))
+    sums = torch.empty((2, num_seqs, num_kv_heads, parts, rows), dtype=torch.float32, device=dev)
+    exp_sums, max_logits = sums[0], sums[1]
+    tmp = torch.empty((num_seqs, num_kv_heads, parts, rows, head_size), dtype=torch.bfloat16, device=dev)
+    w_head, w_part = parts * rows, rows
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    p = PaDecodeParams.from_buffer_copy(_PACK.pack(
+        _PACK.size, _lib.PA_ABI_VERSION,
+        output.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+        sequence_lengths.data_ptr(), q_ptr, ks_ptr, vs_ptr, ptr(alibi_slopes), ptr(sink_tokens),
+        exp_sums.data_ptr(), max_logits.data_ptr(), tmp.data_ptr(), ptr(status), 0, 0,
+        num_seqs, num_kv_heads, group, ql, head_size, bs, num_blocks, block_tables.shape[-1], SEQUENCE_PARTITION_SIZE, parts,
+        output.stride(0), output.stride(1), query.stride(0), query.stride(1), key_cache.stride(0), key_cache.stride(1),
+        value_cache.stride(0), value_cache.stride(1), block_tables.stride(0), q_scale_stride, s_block, s_head,
+        num_kv_heads * w_head, w_head, w_part, num_kv_heads * w_head * head_size, w_head * head_size,
+        w_part * head_size, head_size,
+        q_dtype, _lib.PA_DT_E4M3FN, _lib.PA_DT_BF16, q_mode, kv_mode, v_layout, float(softmax_scale),
+        0, 0, 0, 0, 0, 0))
+    keep = (query, sequence_lengths, block_tables, query_scale, key_scale, value_scale)
+    head_stride = block_tables.stride(1) if per_head and num_kv_heads > 1 else 0
+    return p, head_stride, keep, (exp_sums, max_logits, tmp)
 
 
 def paged_attention_decode(
@@ -431,8 +592,20 @@ def paged_attention_decode(
     Arguments up to ``alibi_slopes`` are the reference's (pa_decode_triton_gluon_fp8.py:1659-1675).
     ``max_sequence_length`` only sizes the partition axis of the workspaces, as there.
     ``num_sequence_partitions`` is accepted and unused, as there.  Scales: ``None``, a 0-dim fp32
-    CUDA tensor (per tensor) or ``[num_blocks, num_kv_heads, block_size, 1]`` fp32 (per token and
-    head); a Python float is accepted for per-tensor scales like the bf16 reference entry does.
+    CUDA tensor (per tensor), ``[num_blocks, num_kv_heads, block_size, 1]`` fp32 (per token and
+    head) or ``[num_blocks, num_kv_heads, 1, 1]`` fp32 (per page and head; positive); a Python float
+    is accepted for per-tensor scales like the bf16 reference entry does.
+
+    ``block_tables`` may be ``[num_seqs, num_kv_heads, max_blocks]``: each kv head then reads the pages
+    of its own table (a selection of the sequence's pages, :func:`triton_op_b200.select_blocks`).
+    ``sequence_lengths[s]`` counts the tokens in one such table -- every page but the last full, the
+    last one the sequence's last -- and ``max_sequence_length`` bounds that.  With ``L`` query tokens
+    the last ``L - 1`` tokens of the sequence have to be the last of every table.  e4m3fn caches
+    with no, per-tensor or per-page scales; no ``alibi_slopes``.
+
+    With per-page scales or tables per kv head the call allocates its workspaces from torch's
+    allocator (its own stream's, or the graph's under capture) and keeps nothing for the next call.
+    ``maximum_logits`` / ``exponential_sums`` then refer to logit + log(value scale) of the token.
 
     Keyword-only additions: ``partition_size`` (reference constant 256); ``exp_sums`` /
     ``max_logits`` ``[num_seqs, num_kv_heads, P, eq_group]`` fp32 and ``tmp_output``
@@ -459,6 +632,23 @@ def paged_attention_decode(
     to the default two-launch form, and measured slower than it (that numbering reads the cache
     slower than the round-robin one, by more than the second launch costs), so it is opt-in.
     """
+    if _by_block(key_scale, value_scale, block_tables):
+        special = exp_sums is not None or max_logits is not None or tmp_output is not None or time_kernels or tune is not None
+        if special and block_tables.dim() == 3:
+            _fail("a block table per kv head takes no workspaces, time_kernels or tune")
+        if partition_size <= 0 or partition_size % SEQUENCE_PARTITION_SIZE:
+            _fail(f"block kv scales and block tables per kv head run in partitions of {SEQUENCE_PARTITION_SIZE} tokens, but got partition_size {partition_size}")
+        if not special:
+            p, head_stride, keep, ws = _build_by_block(
+                output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
+                query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,
+                alibi_slopes, sink_tokens, status)
+            if not output.is_cuda:
+                raise RuntimeError("paged_attention_decode runs on CUDA tensors only; there is no CPU fallback")
+            _lib.launch(output.device, _lib.lib().pa_decode_tables_sm100, "pa_decode_tables_sm100", C.byref(p), head_stride)
+            return {"triton_decode_time": 0.0, "triton_reduce_time": 0.0, "temporary_output": ws[2],
+                    "final_output": output, "exponential_sums": ws[0], "maximum_logits": ws[1],
+                    "total_triton_time": 0.0, "partition_size": SEQUENCE_PARTITION_SIZE}
     p, keep = build_params(output, query, key_cache, value_cache, sequence_lengths, block_tables,
                            softmax_scale, query_sequence_length, max_sequence_length, compute_type,
                            query_scale, key_scale, value_scale, alibi_slopes, partition_size,
