@@ -64,6 +64,7 @@ typedef enum PaVLayout {
 #define PA_DEV_WAIT_TIMEOUT   1  /* a bounded wait on a bulk copy ran out; results are undefined */
 #define PA_DEV_BAD_PAGE_ID    2  /* a block-table entry was outside [0, num_blocks); it was clamped */
 #define PA_DEV_CTX_TOO_LONG   4  /* a context length exceeded max_blocks_per_seq*block_size; it was clamped */
+#define PA_DEV_BAD_RANGE      8  /* an append's rows leave the given ones, or outnumber the sequence's tokens; cut */
 
 /* Size, in uint64 words, of the optional trace buffer: [8 roles][item < 64][4 points]. */
 #define PA_TRACE_WORDS (8 * 64 * 4)
@@ -304,6 +305,111 @@ typedef struct PaCacheWriteParams {
 } PaCacheWriteParams;
 
 int pa_cache_write_sm100(const PaCacheWriteParams* params, void* stream);
+
+/*
+ * Append to a cache with one scale per (page, kv head) (no counterpart in the reference): the rows
+ * row_start[s] .. row_start[s+1] - 1 of key / value become the last tokens of sequence s, whose
+ * length with them is context_lens[s].  A page and kv head that receives rows gets, for its keys and
+ * its values separately,
+ *   want  = the smallest power of two >= max|x| / 448 over the finite elements, at least 2^-40
+ *   scale = want where a row goes to the page's first slot, else max(old scale, want)
+ *   old codes = e4m3fn(code * (old scale / scale)) for every slot without a new row, where the scale grew
+ *   new codes = e4m3fn(x / scale), saturating
+ * and key_bounds (optional) the smallest and the largest key code of every head dim over the page's
+ * tokens.  Scales of pages that hold tokens must be positive.  Pages that receive no row, and, where
+ * no scale grows, slots that receive no row, are left as they are.  No page may receive rows of two sequences.
+ *   kv_quant_mode PA_QUANT_PER_BLOCK   key_scale / value_scale [NB, Hkv] are read and written
+ *                 PA_QUANT_PER_TENSOR  key_scale / value_scale point to one value, read only
+ * Rows without a place (a table too narrow, a page id outside the pool, more rows than tokens) are
+ * skipped and reported in *status.
+ */
+typedef struct PaCacheAppendParams {
+  uint32_t struct_size;        /* = sizeof(PaCacheAppendParams) */
+  uint32_t abi_version;        /* = PA_ABI_VERSION */
+  const void* key;             /* [T, Hkv, D] bf16, last dim contiguous, 16-byte aligned rows */
+  const void* value;           /* [T, Hkv, D] bf16 */
+  void* key_cache;             /* [NB, Hkv, D/16, bs, 16] e4m3fn */
+  void* value_cache;           /* [NB, Hkv, D, bs] or transposed [NB, Hkv, bs/16, D, 16] */
+  float* key_scale;
+  float* value_scale;
+  void* key_bounds;            /* [NB, Hkv, 2, D] e4m3fn (smallest, largest) or NULL */
+  const int32_t* block_tables; /* [S, max_blocks_per_seq] */
+  const int32_t* context_lens; /* [S] */
+  const int32_t* row_start;    /* [S + 1] */
+  int32_t* status;             /* optional */
+  int32_t num_tokens;          /* T: rows of key / value */
+  int32_t num_seqs;            /* S, at most 8192 */
+  int32_t num_kv_heads, head_size, block_size, num_blocks, max_blocks_per_seq;
+  int32_t kv_quant_mode;       /* PaQuantMode */
+  int32_t v_layout;            /* PaVLayout */
+  int32_t reserved;            /* 0 */
+  int64_t key_stride_token, key_stride_head;       /* elements */
+  int64_t value_stride_token, value_stride_head;
+  int64_t k_stride_block, k_stride_head;           /* caches, elements */
+  int64_t v_stride_block, v_stride_head;
+  int64_t kv_scale_stride_block, kv_scale_stride_head;
+  int64_t bounds_stride_block, bounds_stride_head;
+  int64_t bt_stride_seq;
+} PaCacheAppendParams;
+
+int pa_cache_append_sm100(const PaCacheAppendParams* params, void* stream);
+
+/*
+ * Page scores (no counterpart in the reference): for every page i of a sequence's table that holds a
+ * token of its context
+ *   scores[s, h, i] = key_scale[page, h] * max_r softmax_scale * qs_r * sum_d max(q_rd lo_d, q_rd hi_d)
+ * over the query rows r of kv head h, where (lo, hi) = key_bounds[page, h]: no logit of the group
+ * with a key of the page is larger.  Entries past the last such page become -inf.
+ */
+typedef struct PaBlockScoreParams {
+  uint32_t struct_size, abi_version;
+  const void* query;           /* [S, Hkv*rows, D] bf16 or e4m3fn, rows contiguous */
+  const void* key_bounds;      /* [NB, Hkv, 2, D] e4m3fn */
+  const int32_t* block_tables; /* [S, max_blocks_per_seq] */
+  const int32_t* context_lens; /* [S] */
+  const float* query_scale;    /* see q_quant_mode */
+  const float* key_scale;      /* see kv_quant_mode: none, per tensor or per block */
+  float* scores;               /* [S, Hkv, max_blocks_per_seq] */
+  int32_t* status;             /* optional */
+  int32_t num_seqs, num_kv_heads;
+  int32_t rows;                /* query rows per kv head, 1..64 */
+  int32_t head_size, block_size, num_blocks, max_blocks_per_seq;
+  int32_t q_dtype, q_quant_mode, kv_quant_mode;
+  int64_t q_stride_seq;                            /* elements */
+  int64_t bounds_stride_block, bounds_stride_head;
+  int64_t bt_stride_seq, q_scale_stride_seq;
+  int64_t kv_scale_stride_block, kv_scale_stride_head;
+  int64_t scores_stride_seq, scores_stride_head;
+  float softmax_scale;         /* > 0 */
+  int32_t reserved;            /* 0 */
+} PaBlockScoreParams;
+
+int pa_block_scores_sm100(const PaBlockScoreParams* params, void* stream);
+
+/*
+ * Page selection (no counterpart in the reference): per (sequence, kv head) the first keep_first and
+ * the last keep_last pages of the context and those with the highest scores of the others (NaN
+ * lowest, ties to the lower place), top_k in all, as a block table in the order of the context.
+ * A sequence of at most top_k pages keeps them all.  Unused entries become 0.
+ *   lengths[s] = tokens in the pages of one such table (the same for every kv head)
+ */
+typedef struct PaBlockSelectParams {
+  uint32_t struct_size, abi_version;
+  const float* scores;         /* [S, Hkv, >= pages] */
+  const int32_t* block_tables; /* [S, max_blocks_per_seq] */
+  const int32_t* context_lens; /* [S] */
+  int32_t* tables;             /* [S, Hkv, top_k] */
+  int32_t* lengths;            /* [S] */
+  int32_t* status;             /* optional */
+  int32_t num_seqs, num_kv_heads, block_size, max_blocks_per_seq;
+  int32_t top_k;               /* >= keep_first + keep_last, > 0 */
+  int32_t keep_first;          /* >= 0 */
+  int32_t keep_last;           /* >= 1: the attention wants the last page of the context last */
+  int32_t reserved;            /* 0 */
+  int64_t scores_stride_seq, scores_stride_head, bt_stride_seq, tables_stride_seq, tables_stride_head;
+} PaBlockSelectParams;
+
+int pa_block_select_sm100(const PaBlockSelectParams* params, void* stream);
 
 /* Bytes of dynamic shared memory and the grid the partition kernel would use for `params`
  * (host-only query, launches nothing).  Any output pointer may be NULL. */

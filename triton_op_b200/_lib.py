@@ -18,7 +18,7 @@ PA_OK = 0
 PA_DT_BF16, PA_DT_E4M3FN = 0, 1
 PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN, PA_QUANT_PER_BLOCK = -1, 0, 1, 2
 PA_V_NORMAL, PA_V_TRANSPOSED = 0, 1
-PA_DEV_WAIT_TIMEOUT, PA_DEV_BAD_PAGE_ID, PA_DEV_CTX_TOO_LONG = 1, 2, 4
+PA_DEV_WAIT_TIMEOUT, PA_DEV_BAD_PAGE_ID, PA_DEV_CTX_TOO_LONG, PA_DEV_BAD_RANGE = 1, 2, 4, 8
 PA_TRACE_WORDS = 8 * 64 * 4
 PA_NOALLOC_SCRATCH_BYTES = 16 << 20
 PA_IPC_HANDLE_BYTES = 64
@@ -27,7 +27,7 @@ EXPORTS = (
     "pa_decode_sm100", "pa_decode_tables_sm100", "pa_decode_noalloc_sm100", "pa_partition_sm100", "pa_reduce_sm100", "pa_merge_triples_sm100",
     "pa_merge_packed_triples_sm100", "pa_packed_triple_floats", "pa_exchange_alloc", "pa_exchange_open", "pa_exchange_close", "pa_exchange_free",
     "pa_exchange_bytes", "pa_reduce_push_sm100", "pa_merge_wait_sm100",
-    "pa_cache_write_sm100", "pa_stream_probe_sm100", "pa_query_launch_sm100", "pa_strerror", "pa_last_cuda_error", "pa_abi_version",
+    "pa_cache_write_sm100", "pa_cache_append_sm100", "pa_block_scores_sm100", "pa_block_select_sm100", "pa_stream_probe_sm100", "pa_query_launch_sm100", "pa_strerror", "pa_last_cuda_error", "pa_abi_version",
 )
 
 
@@ -66,6 +66,48 @@ class PaCacheWriteParams(C.Structure):
         + [(n, C.c_int64) for n in ("key_stride_token", "key_stride_head", "value_stride_token", "value_stride_head",
                                     "k_stride_block", "k_stride_head", "v_stride_block", "v_stride_head",
                                     "kv_scale_stride_block", "kv_scale_stride_head")]
+    )
+
+
+class PaCacheAppendParams(C.Structure):
+    """Field-for-field mirror of ``struct PaCacheAppendParams``."""
+    _fields_ = (
+        [("struct_size", C.c_uint32), ("abi_version", C.c_uint32)]
+        + [(n, C.c_void_p) for n in ("key", "value", "key_cache", "value_cache", "key_scale", "value_scale", "key_bounds",
+                                     "block_tables", "context_lens", "row_start", "status")]
+        + [(n, C.c_int32) for n in ("num_tokens", "num_seqs", "num_kv_heads", "head_size", "block_size", "num_blocks",
+                                    "max_blocks_per_seq", "kv_quant_mode", "v_layout", "reserved")]
+        + [(n, C.c_int64) for n in ("key_stride_token", "key_stride_head", "value_stride_token", "value_stride_head",
+                                    "k_stride_block", "k_stride_head", "v_stride_block", "v_stride_head",
+                                    "kv_scale_stride_block", "kv_scale_stride_head", "bounds_stride_block",
+                                    "bounds_stride_head", "bt_stride_seq")]
+    )
+
+
+class PaBlockScoreParams(C.Structure):
+    """Field-for-field mirror of ``struct PaBlockScoreParams``."""
+    _fields_ = (
+        [("struct_size", C.c_uint32), ("abi_version", C.c_uint32)]
+        + [(n, C.c_void_p) for n in ("query", "key_bounds", "block_tables", "context_lens", "query_scale", "key_scale",
+                                     "scores", "status")]
+        + [(n, C.c_int32) for n in ("num_seqs", "num_kv_heads", "rows", "head_size", "block_size", "num_blocks",
+                                    "max_blocks_per_seq", "q_dtype", "q_quant_mode", "kv_quant_mode")]
+        + [(n, C.c_int64) for n in ("q_stride_seq", "bounds_stride_block", "bounds_stride_head", "bt_stride_seq",
+                                    "q_scale_stride_seq", "kv_scale_stride_block", "kv_scale_stride_head",
+                                    "scores_stride_seq", "scores_stride_head")]
+        + [("softmax_scale", C.c_float), ("reserved", C.c_int32)]
+    )
+
+
+class PaBlockSelectParams(C.Structure):
+    """Field-for-field mirror of ``struct PaBlockSelectParams``."""
+    _fields_ = (
+        [("struct_size", C.c_uint32), ("abi_version", C.c_uint32)]
+        + [(n, C.c_void_p) for n in ("scores", "block_tables", "context_lens", "tables", "lengths", "status")]
+        + [(n, C.c_int32) for n in ("num_seqs", "num_kv_heads", "block_size", "max_blocks_per_seq", "top_k",
+                                    "keep_first", "keep_last", "reserved")]
+        + [(n, C.c_int64) for n in ("scores_stride_seq", "scores_stride_head", "bt_stride_seq", "tables_stride_seq",
+                                    "tables_stride_head")]
     )
 
 
@@ -124,6 +166,10 @@ def lib() -> C.CDLL:
         getattr(L, name).restype = C.c_int
     L.pa_cache_write_sm100.argtypes = [C.POINTER(PaCacheWriteParams), C.c_void_p]
     L.pa_cache_write_sm100.restype = C.c_int
+    for name, struct in (("pa_cache_append_sm100", PaCacheAppendParams), ("pa_block_scores_sm100", PaBlockScoreParams),
+                         ("pa_block_select_sm100", PaBlockSelectParams)):
+        getattr(L, name).argtypes = [C.POINTER(struct), C.c_void_p]
+        getattr(L, name).restype = C.c_int
     L.pa_stream_probe_sm100.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
     L.pa_stream_probe_sm100.restype = C.c_int
     for name in ("pa_decode_sm100", "pa_decode_noalloc_sm100", "pa_partition_sm100", "pa_reduce_sm100",

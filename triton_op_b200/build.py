@@ -1,7 +1,8 @@
 """In-tree build of the CUDA library (``python -m triton_op_b200.build``).
 
-One nvcc invocation turns ``csrc/pa_decode_sm100.cu`` into ``lib/libpa_decode_sm100.so`` for
-sm_100a.  nvcc cross-compiles, so this also runs on a machine without a GPU.
+nvcc turns the sources in ``csrc/`` into ``lib/libpa_decode_sm100.so`` for sm_100a, one object each
+(side by side, and only what is older than its sources).  nvcc cross-compiles, so this also runs on
+a machine without a GPU.
 """
 from __future__ import annotations
 
@@ -14,15 +15,19 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpa_decode_sm100.so")
-SOURCES = ["pa_decode_sm100.cu"]
-HEADERS = ["pa_common.cuh", "pa_params.cuh", "pa_partition_fp8.cuh", "pa_partition_bf16.cuh", "pa_partition_tc.cuh", "pa_tcgen05.cuh",
-           "pa_reduce.cuh", "pa_cache_write.cuh", "pa_exchange.cuh", "pa_stream_probe.cuh",
-           os.path.join("..", "..", "include", "pa_decode_sm100.h")]
+_COMMON = ["pa_common.cuh", "pa_params.cuh", "pa_host.h", os.path.join("..", "..", "include", "pa_decode_sm100.h")]
+# source -> headers it includes
+SOURCES = {
+    "pa_decode_sm100.cu": _COMMON + [
+        "pa_partition_fp8.cuh", "pa_partition_bf16.cuh", "pa_partition_tc.cuh", "pa_tcgen05.cuh", "pa_reduce.cuh",
+        "pa_cache_write.cuh", "pa_exchange.cuh", "pa_stream_probe.cuh"],
+    "pa_blocks_sm100.cu": _COMMON + ["pa_block_score.cuh", "pa_block_select.cuh", "pa_cache_append.cuh"],
+}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -33,12 +38,19 @@ def _nvcc() -> str:
     return exe
 
 
-def needs_build() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _object(source: str) -> str:
+    return os.path.join(LIB_DIR, os.path.splitext(source)[0] + ".o")
+
+
+def _stale(target: str, source: str) -> bool:
+    if not os.path.exists(target):
         return True
-    built = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, s) for s in SOURCES] + [os.path.join(CSRC, h) for h in HEADERS]
-    return any(os.path.getmtime(d) > built for d in deps)
+    built = os.path.getmtime(target)
+    return any(os.path.getmtime(os.path.join(CSRC, d)) > built for d in [source] + SOURCES[source])
+
+
+def needs_build() -> bool:
+    return any(_stale(LIB_PATH, s) for s in SOURCES)
 
 
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
@@ -47,13 +59,22 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
     if not force and not needs_build():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + (["-DPA_TRACE_BUILD"] if trace else [])
-    cmd += ["-o", LIB_PATH] + [os.path.join(CSRC, s) for s in SOURCES]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    flags = NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + (["-DPA_TRACE_BUILD"] if trace else [])
+    jobs = {s: subprocess.Popen([_nvcc()] + flags + ["-c", "-o", _object(s), os.path.join(CSRC, s)],
+                                stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+            for s in SOURCES if force or _stale(_object(s), s)}
+    logs = {s: (job.communicate()[0], job.returncode) for s, job in jobs.items()}
+    for s, (text, code) in logs.items():
+        if code != 0:
+            if os.path.exists(_object(s)):
+                os.remove(_object(s))
+            raise RuntimeError(f"nvcc failed on {s}:\n{text}")
+        if verbose:
+            sys.stderr.write(text)
+    proc = subprocess.run([_nvcc()] + NVCC_FLAGS + ["-shared", "-o", LIB_PATH] + [_object(s) for s in SOURCES],
+                          capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
-    if verbose:
-        sys.stderr.write(proc.stderr)
     return LIB_PATH
 
 

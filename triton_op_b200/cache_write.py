@@ -3,19 +3,21 @@
 The reference prepares its caches offline (layouts: test_pa_mtp.py:109-172; per-token e4m3
 quantisation ``quantize_kv_cache_symmetric``: :294-369).  A serving loop does the same for the
 tokens of every step; :func:`write_kv_cache` is that step as one CUDA kernel
-(``pa_cache_write_sm100``): quantise and scatter, no intermediate tensors.
+(``pa_cache_write_sm100``): quantise and scatter, no intermediate tensors.  :func:`append_kv_cache` is
+the same step for caches with one scale per (page, kv head) (``pa_cache_append_sm100``).
 """
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .pa_decode import FP8_DTYPE, PaArgumentError
+from .pa_decode import FP8_DTYPE, SUPPORTED_BLOCK_SIZES, PaArgumentError, _check_block_scales, _inner_contiguous
 
-__all__ = ["write_kv_cache", "slots_for"]
+__all__ = ["write_kv_cache", "append_kv_cache", "slots_for"]
 
 
 def slots_for(block_tables: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor, block_size: int) -> torch.Tensor:
@@ -102,3 +104,100 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tens
     with torch.cuda.device(key.device):
         _lib.check(_lib.lib().pa_cache_write_sm100(C.byref(p), torch.cuda.current_stream().cuda_stream),
                    "pa_cache_write_sm100")
+
+
+_APPEND = struct.Struct("=2I11Q10i13q")
+assert _APPEND.size == C.sizeof(_lib.PaCacheAppendParams)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [T, Hkv, D] bf16 with 16-byte aligned rows (a copy where it has none)."""
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                    key_scale: torch.Tensor, value_scale: torch.Tensor, block_tables: torch.Tensor,
+                    sequence_lengths: torch.Tensor, query_start_loc: torch.Tensor, *,
+                    key_bounds: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """Appends every sequence's new tokens to an e4m3fn cache with one scale per (page, kv head).
+
+    Rows ``query_start_loc[s] .. query_start_loc[s + 1] - 1`` of ``key`` / ``value`` (bf16
+    ``[T, num_kv_heads, head_size]``) become the last tokens of sequence ``s``, whose length with them
+    is ``sequence_lengths[s]`` -- the tensors the decode call after it takes.  ``key_scale`` /
+    ``value_scale`` fp32 ``[num_blocks, num_kv_heads, 1, 1]`` are read and written: a page that begins with
+    this call gets the smallest power of two that brings its largest value to 448 at most (2**-40 at
+    least); in a page with tokens the scale grows if it has to, and the page's codes are brought to the
+    new scale.  Nothing else of the cache changes.  0-dim scales (per tensor) are read only.
+
+    ``key_bounds``: e4m3fn ``[num_blocks, num_kv_heads, 2, head_size]``, the smallest and largest key
+    code of every head dim over the page's tokens, kept up to date for
+    :func:`triton_op_b200.score_blocks`.  ``status`` (int32 scalar) receives ``PA_DEV_*`` bits for rows
+    that have no place; they are skipped.  No page may get rows of two sequences in a call.  Runs on
+    the current stream; there is no CPU fallback.
+    """
+    dev = key.device
+    if not (key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16 and key.shape == value.shape and key.dim() == 3):
+        raise PaArgumentError("key and value must be bf16 [num_tokens, num_kv_heads, head_size] of one shape")
+    if not (key_cache.dim() == 5 and key_cache.dtype == FP8_DTYPE and value_cache.dtype == FP8_DTYPE):
+        raise PaArgumentError(f"append_kv_cache needs {FP8_DTYPE} caches, a 5-D key_cache and a 4-D or 5-D value_cache")
+    num_tokens, num_kv_heads, head_size = key.shape
+    num_blocks, bs = key_cache.shape[0], key_cache.shape[3]
+    if head_size != 128 or bs not in SUPPORTED_BLOCK_SIZES:
+        raise PaArgumentError(f"head_size must be 128 and block_size in {list(SUPPORTED_BLOCK_SIZES)}, but got {head_size} and {bs}")
+    if key_cache.shape != (num_blocks, num_kv_heads, head_size // 16, bs, 16):
+        raise PaArgumentError(f"key_cache must be [num_blocks, {num_kv_heads}, {head_size // 16}, block_size, 16]")
+    trans = value_cache.dim() == 5
+    want_v = (num_blocks, num_kv_heads, bs // 16, head_size, 16) if trans else (num_blocks, num_kv_heads, head_size, bs)
+    if value_cache.shape != want_v:
+        raise PaArgumentError(f"value_cache must be {want_v}")
+    if not (_inner_contiguous(key_cache, 2) and _inner_contiguous(value_cache, 2)):
+        raise PaArgumentError("the per-(block, head) slabs of the KV caches must be contiguous")
+    for name, s in (("key_scale", key_scale), ("value_scale", value_scale)):
+        if not (isinstance(s, torch.Tensor) and s.dtype == torch.float32 and s.device == dev):
+            raise PaArgumentError(f"{name} must be a float32 tensor on {dev}")
+    if key_scale.dim() == 0 and value_scale.dim() == 0:
+        mode, s_block, s_head = _lib.PA_QUANT_PER_TENSOR, 0, 0
+    else:
+        _check_block_scales(key_scale, value_scale, key_cache, dev)
+        if (num_blocks > 1 and key_scale.stride(0) == 0) or (num_kv_heads > 1 and key_scale.stride(1) == 0):
+            raise PaArgumentError("block kv scales are written: every page and kv head needs a place of its own")
+        mode, s_block, s_head = _lib.PA_QUANT_PER_BLOCK, key_scale.stride(0), key_scale.stride(1)
+    b_block = b_head = 0
+    if key_bounds is not None:
+        if not (key_bounds.dtype == FP8_DTYPE and key_bounds.shape == (num_blocks, num_kv_heads, 2, head_size)
+                and _inner_contiguous(key_bounds, 2) and key_bounds.device == dev):
+            raise PaArgumentError(f"key_bounds must be {FP8_DTYPE} {(num_blocks, num_kv_heads, 2, head_size)} on {dev}, its last two dims contiguous")
+        b_block, b_head = key_bounds.stride(0), key_bounds.stride(1)
+    num_seqs = block_tables.shape[0]
+    for name, t in (("block_tables", block_tables), ("sequence_lengths", sequence_lengths), ("query_start_loc", query_start_loc)):
+        if not (t.dtype == torch.int32 and t.device == dev):
+            raise PaArgumentError(f"{name} must be int32 on {dev}")
+    if not (block_tables.dim() == 2 and block_tables.shape[1] >= 1 and sequence_lengths.numel() == num_seqs
+            and query_start_loc.numel() == num_seqs + 1):
+        raise PaArgumentError("block_tables must be [num_seqs, max_blocks], sequence_lengths [num_seqs] and query_start_loc [num_seqs + 1]")
+    for name, t in (("value", value), ("key_cache", key_cache), ("value_cache", value_cache)):
+        if t.device != dev:
+            raise PaArgumentError(f"{name} must live on {dev}, the key's device")
+    if status is not None and not (status.dtype == torch.int32 and status.device == dev):
+        raise PaArgumentError(f"status must be an int32 tensor on {dev}")
+    if not key.is_cuda:
+        raise RuntimeError("append_kv_cache runs on CUDA tensors only; there is no CPU fallback")
+    key, value = _rows(key), _rows(value)
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    if not sequence_lengths.is_contiguous():
+        sequence_lengths = sequence_lengths.contiguous()
+    if not query_start_loc.is_contiguous():
+        query_start_loc = query_start_loc.contiguous()
+    p = _lib.PaCacheAppendParams.from_buffer_copy(_APPEND.pack(
+        _APPEND.size, _lib.PA_ABI_VERSION,
+        key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
+        value_scale.data_ptr(), 0 if key_bounds is None else key_bounds.data_ptr(), block_tables.data_ptr(),
+        sequence_lengths.data_ptr(), query_start_loc.data_ptr(), 0 if status is None else status.data_ptr(),
+        num_tokens, num_seqs, num_kv_heads, head_size, bs, num_blocks, block_tables.shape[1], mode,
+        _lib.PA_V_TRANSPOSED if trans else _lib.PA_V_NORMAL, 0,
+        key.stride(0), key.stride(1), value.stride(0), value.stride(1), key_cache.stride(0), key_cache.stride(1),
+        value_cache.stride(0), value_cache.stride(1), s_block, s_head, b_block, b_head, block_tables.stride(0)))
+    _lib.launch(dev, _lib.lib().pa_cache_append_sm100, "pa_cache_append_sm100", C.byref(p))

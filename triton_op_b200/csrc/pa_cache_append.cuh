@@ -1,0 +1,405 @@
+// Append to a cache with one scale for each (page, kv head): the new tokens of every sequence are
+// quantised to e4m3 and stored behind the tokens that its pages hold already.
+//
+// For a page and kv head that receives the rows x_i (keys and values separately):
+//   want  = the smallest power of two >= max|x| / 448 (finite elements; at least 2^-40)
+//   scale = want                        where the rows begin the page
+//         = max(old scale, want)        where the page holds tokens already
+//   codes of the page := e4m3(code * (old scale / scale))   where the scale grew
+//   code_i = e4m3(x_i / scale), saturating
+// A scale that is a power of two costs no precision (e4m3 keeps its four significant bits wherever
+// the value lies), and it makes growing a page a shift of exponents: only codes that become
+// subnormal are rounded again, however often a page grows.  With a per-tensor scale (read, never
+// written) only the last line applies.  Optionally the smallest and largest key code of each head
+// dim are kept per (page, kv head), as the page scores need them; rounding is monotone, so they
+// are found on the bf16 inputs and rounded once.
+//
+// A unit of work is (page, kv head, key or value), and all of it belongs to one group of warps: the
+// scale is a maximum over every row the page gets, and two writers of one page would race on it.
+// Each warp takes 16 consecutive slots of the page, whose rows stay in registers between the
+// maximum and the store (pages of 1024 tokens: four such runs per warp, read twice).  Keys are
+// stored as 16-byte chunks [d/16][token][16], values as 16 tokens of a head dim, 16 bytes too;
+// values of a run that is not whole are merged with the bytes that are there.
+// What bounds it: 512 bytes read and 256 written per (token, kv head) -- HBM for a prompt; a decode
+// step of a few hundred rows is launch latency and one chain of loads.
+#pragma once
+
+#include "../../include/pa_decode_sm100.h"
+#include "pa_common.cuh"
+#include "pa_params.cuh"
+
+namespace pa {
+
+constexpr float kAppendMinScale = 0x1p-40f;
+constexpr int kAppendMaxSeqs = 8192;     // sequences whose index a CTA holds (one int each)
+
+struct CacheAppendParams {
+  const uint8_t* key;          // [T, Hkv, 128] bf16
+  const uint8_t* value;
+  uint8_t* key_cache;
+  uint8_t* value_cache;
+  float* k_scale;              // [NB, Hkv] by strides (written), or one value (read)
+  float* v_scale;
+  uint8_t* bounds;             // [NB, Hkv, 2, 128] e4m3, or null
+  const int32_t* block_tables; // [S, width]
+  const int32_t* context_lens; // [S]: lengths with the new tokens
+  const int32_t* row_start;    // [S + 1]: the sequence's first row in key / value
+  int32_t* status;
+  int32_t T, S, Hkv, num_blocks, width, v_trans, per_block;
+  int64_t key_stride_tok, key_stride_head;       // elements
+  int64_t value_stride_tok, value_stride_head;
+  int64_t kc_stride_block, kc_stride_head;       // bytes
+  int64_t vc_stride_block, vc_stride_head;
+  int64_t ks_stride_block, ks_stride_head;       // elements
+  int64_t b_stride_block, b_stride_head;         // bytes
+  int64_t bt_stride_seq;
+};
+
+// Four e4m3 codes times a factor, rounded to e4m3 again.
+__device__ __forceinline__ uint32_t rescale_e4m3x4(uint32_t w, float f) {
+  uint32_t lo, hi;
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
+  float x0, x1, x2, x3;
+  asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(x0), "=f"(x1) : "r"(lo));
+  asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(x2), "=f"(x3) : "r"(hi));
+  return pack_e4m3x4(x0 * f, x1 * f, x2 * f, x3 * f);
+}
+__device__ __forceinline__ uint4 rescale_e4m3x16(uint4 v, float f) {
+  return make_uint4(rescale_e4m3x4(v.x, f), rescale_e4m3x4(v.y, f), rescale_e4m3x4(v.z, f), rescale_e4m3x4(v.w, f));
+}
+__device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
+  uint32_t h;
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, a;}" : "=r"(h) : "r"(byte & 0xffu));
+  float x;
+  asm("{.reg .f16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, a;}" : "=f"(x) : "r"(h));
+  return x;
+}
+// Largest |x| of two packed bf16 as a bf16 bit pattern per half; NaN and infinity count as zero.
+__device__ __forceinline__ uint32_t finite_abs2(uint32_t w) {
+  const uint32_t a = w & 0x7fff7fffu;
+  uint32_t lo = a & 0xffffu, hi = a >> 16;
+  lo = lo >= 0x7f80u ? 0u : lo;
+  hi = hi >= 0x7f80u ? 0u : hi;
+  return lo | (hi << 16);
+}
+// The smallest power of two s with amax <= 448 s, at least 2^-40.  amax is a finite bf16 value.
+__device__ __forceinline__ float page_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) + ((u & 0x7fffffu) > 0x600000u ? 1 : 0) - 8;   // 448 = 1.75 * 2^8
+  return __uint_as_float((uint32_t)max(e, 127 - 40) << 23);
+}
+__device__ __forceinline__ uint32_t bf16x2_min(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t bf16x2_max(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// x / scale for a whole unit: an exact product where the scale is a power of two.
+struct Quantiser {
+  float scale, inv;
+  bool exact;
+  __device__ explicit Quantiser(float s) : scale(s), inv(1.0f / s) {
+    const uint32_t u = __float_as_uint(s);
+    exact = (u & 0x7fffffu) == 0u && u >= (2u << 23) && u <= (252u << 23);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return exact ? x * inv : __fdiv_rn(x, scale); }
+  __device__ __forceinline__ uint32_t four(uint32_t w0, uint32_t w1) const {   // bf16 pairs -> e4m3 codes
+    const Quantiser& q = *this;
+    return pack_e4m3x4(q(bf16_lo_to_f32(w0)), q(bf16_hi_to_f32(w0)), q(bf16_lo_to_f32(w1)), q(bf16_hi_to_f32(w1)));
+  }
+};
+
+// BS: tokens per page.  WPU: warps per unit.
+template <int BS, int WPU>
+__global__ void __launch_bounds__(WPU > 4 ? WPU * 32 : 128)
+pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
+  constexpr int kThreads = WPU > 4 ? WPU * 32 : 128;
+  constexpr int kUnits = kThreads / 32 / WPU;                       // units a CTA works on at a time
+  constexpr int kRuns = BS / 16;                                    // 16-slot runs of a page
+  constexpr int kPerWarp = (kRuns + WPU - 1) / WPU;                 // ... that a warp takes
+  extern __shared__ int index_smem[];
+  int* unit_off = index_smem;          // [S + 1] pages touched before each sequence
+  __shared__ int scan[32];
+  __shared__ uint32_t red_max[kThreads / 32];
+  __shared__ uint32_t red_lo[WPU > 1 ? WPU : 1][64], red_hi[WPU > 1 ? WPU : 1][64];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int sub = warp % WPU;          // warp inside its unit
+
+  grid_dependency_wait();
+  // rows of a sequence: [first row, count), and its first new token's position
+  auto rows_of = [&](int s, int& row, int& count, int& pos, bool report) {
+    const int a = p.row_start[s], b = p.row_start[s + 1], len = p.context_lens[s];
+    row = min(max(a, 0), p.T);
+    const int end = min(max(b, row), p.T);
+    count = end - row;
+    bool bad = a < 0 || b > p.T || b < a;
+    if (count > len) {       // more rows than tokens: the first ones have no place
+      bad = bad || count > 0;
+      row += count - max(len, 0);
+      count = max(len, 0);
+    }
+    pos = max(len, 0) - count;
+    const int64_t cap = (int64_t)p.width * BS;
+    if (pos + (int64_t)count > cap) {   // tokens past the table have no page
+      count = (int)max((int64_t)0, cap - pos);
+      if (report && p.status) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
+    }
+    if (bad && report && p.status) atomicOr(p.status, PA_DEV_BAD_RANGE);
+  };
+  // ---- pages touched, summed over the sequences (every CTA for itself: S is small)
+  {
+    const int chunk = (p.S + kThreads - 1) / kThreads;
+    const int beg = min(tid * chunk, p.S), end = min(beg + chunk, p.S);
+    int sum = 0;
+    for (int s = beg; s < end; ++s) {
+      int row, count, pos;
+      rows_of(s, row, count, pos, blockIdx.x == 0);
+      const int n = count > 0 ? (pos + count - 1) / BS - pos / BS + 1 : 0;
+      unit_off[s + 1] = n;
+      sum += n;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFullMask, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    if (tid == 0) unit_off[0] = 0;
+    __syncthreads();
+    int run = incl - sum;
+    for (int w = 0; w < warp; ++w) run += scan[w];
+    for (int s = beg; s < end; ++s) {
+      run += unit_off[s + 1];
+      unit_off[s + 1] = run;
+    }
+    __syncthreads();
+  }
+  const int64_t units = (int64_t)unit_off[p.S] * p.Hkv * 2;
+
+  for (int64_t u0 = (int64_t)blockIdx.x * kUnits; u0 < units; u0 += (int64_t)gridDim.x * kUnits) {
+    const int64_t u = u0 + warp / WPU;
+    bool live = u < units;
+    // unit = ((page of the sequence, sequence), head, key or value), the last fastest
+    const bool is_v = live && (u & 1);
+    const int64_t ph = u >> 1;
+    const int touched = live ? (int)(ph / p.Hkv) : 0, head = live ? (int)(ph - (int64_t)touched * p.Hkv) : 0;
+    int seq = 0;
+    {
+      int lo = 0, hi = p.S;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (unit_off[mid] <= touched) lo = mid; else hi = mid;
+      }
+      seq = lo;
+    }
+    int row = 0, count = 0, pos = 0;
+    if (live) rows_of(seq, row, count, pos, false);
+    const int page = pos / BS + (touched - unit_off[seq]);
+    // slots [o0, o1) of the page receive rows row0 ..
+    const int o0 = max(pos - page * BS, 0), o1 = live ? min(BS, pos + count - page * BS) : o0;
+    const int row0 = row + (page * BS + o0 - pos);
+    int blk = live ? p.block_tables[(int64_t)seq * p.bt_stride_seq + page] : 0;
+    if ((unsigned)blk >= (unsigned)p.num_blocks) {
+      if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_BAD_PAGE_ID);
+      live = false;
+      blk = 0;
+    }
+    const uint8_t* src = (is_v ? p.value : p.key) +
+                         2 * ((int64_t)row0 * (is_v ? p.value_stride_tok : p.key_stride_tok) +
+                              (int64_t)head * (is_v ? p.value_stride_head : p.key_stride_head));
+    const int64_t tok_bytes = 2 * (is_v ? p.value_stride_tok : p.key_stride_tok);
+    uint8_t* cache = is_v ? p.value_cache + (int64_t)blk * p.vc_stride_block + (int64_t)head * p.vc_stride_head
+                          : p.key_cache + (int64_t)blk * p.kc_stride_block + (int64_t)head * p.kc_stride_head;
+    float* scale_at = (is_v ? p.v_scale : p.k_scale) + (p.per_block ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
+    const float old_scale = live ? *scale_at : 1.0f;
+    // keys: lane = (chunk c of 16 dims, phase f), slots f, f + 4, f + 8, f + 12 of a run, 32 bytes each
+    // values: lane = head dims 4 lane .. 4 lane + 3 of every slot of a run, 8 bytes each
+    const int c = lane >> 2, f = lane & 3;
+    uint4 ka[4], kb[4];   // keys of the warp's (last) run
+    uint2 va[16];         // values
+    auto load_run = [&](int run) {
+      if (is_v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int o = run * 16 + i;
+          va[i] = (o >= o0 && o < o1) ? __ldg(reinterpret_cast<const uint2*>(src + (int64_t)(o - o0) * tok_bytes) + lane) : make_uint2(0u, 0u);
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int o = run * 16 + 4 * m + f;
+          const bool in = o >= o0 && o < o1;
+          const uint4* at = reinterpret_cast<const uint4*>(src + (int64_t)(o - o0) * tok_bytes + c * 32);
+          ka[m] = in ? __ldg(at) : make_uint4(0u, 0u, 0u, 0u);
+          kb[m] = in ? __ldg(at + 1) : make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    };
+    // runs of the page that receive rows: [run0, run1); this warp takes sub, sub + WPU, ... of all runs
+    const int run0 = o0 >> 4, run1 = live && o1 > o0 ? ((o1 - 1) >> 4) + 1 : run0;
+    auto mine = [&](int k) -> int { return sub + k * WPU; };
+
+    // ---- the largest finite |x|, and the smallest and largest key of every head dim
+    uint32_t top = 0;
+    uint32_t lo8[8], hi8[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo8[e] = 0x7f807f80u, hi8[e] = 0xff80ff80u;   // +inf, -inf
+    const bool want_bounds = p.bounds != nullptr && !is_v;
+    int loaded = -1;
+#pragma unroll 1
+    for (int k = 0; k < kPerWarp; ++k) {
+      const int run = mine(k);
+      if (run < run0 || run >= run1) continue;
+      load_run(run);
+      loaded = run;
+      if (is_v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = __vmaxu2(top, __vmaxu2(finite_abs2(va[i].x), finite_abs2(va[i].y)));
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t w[8] = {ka[m].x, ka[m].y, ka[m].z, ka[m].w, kb[m].x, kb[m].y, kb[m].z, kb[m].w};
+          const int o = run * 16 + 4 * m + f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            top = __vmaxu2(top, finite_abs2(w[e]));
+            if (o >= o0 && o < o1) lo8[e] = bf16x2_min(lo8[e], w[e]), hi8[e] = bf16x2_max(hi8[e], w[e]);
+          }
+        }
+      }
+    }
+    uint32_t top1 = __reduce_max_sync(kFullMask, max(top & 0xffffu, top >> 16));
+    if (want_bounds) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1) {
+          lo8[e] = bf16x2_min(lo8[e], __shfl_xor_sync(kFullMask, lo8[e], o));
+          hi8[e] = bf16x2_max(hi8[e], __shfl_xor_sync(kFullMask, hi8[e], o));
+        }
+      }
+    }
+    if (WPU > 1) {   // over the warps of the unit (a CTA then has one unit)
+      if (lane == 0) red_max[warp] = top1;
+      if (want_bounds && f == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) red_lo[sub][c * 8 + e] = lo8[e], red_hi[sub][c * 8 + e] = hi8[e];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WPU; ++w) top1 = max(top1, red_max[w]);
+      if (want_bounds && sub == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll 1
+          for (int w = 0; w < WPU; ++w) lo8[e] = bf16x2_min(lo8[e], red_lo[w][c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], red_hi[w][c * 8 + e]);
+        }
+      }
+    }
+    const bool fresh = o0 == 0;
+    float scale = old_scale, ratio = 1.0f;
+    bool grew = false;
+    if (p.per_block) {
+      const float want = page_scale(__uint_as_float(top1 << 16));
+      scale = fresh ? want : fmaxf(old_scale, want);
+      grew = !fresh && scale != old_scale;
+      if (grew) ratio = __fdiv_rn(old_scale, scale);
+    }
+    if (live && o1 > o0) {
+      const Quantiser q(scale);
+#pragma unroll 1
+      for (int k = 0; k < kPerWarp; ++k) {
+        const int run = mine(k);
+        const bool has = run >= run0 && run < run1;
+        if (run >= kRuns || !(has || grew)) continue;
+        if (has && run != loaded) {
+          load_run(run);
+          loaded = run;
+        }
+        if (!is_v) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const int o = run * 16 + 4 * m + f;
+            uint4* dst = reinterpret_cast<uint4*>(cache + ((int64_t)c * BS + o) * 16);
+            if (o >= o0 && o < o1) {
+              *dst = make_uint4(q.four(ka[m].x, ka[m].y), q.four(ka[m].z, ka[m].w), q.four(kb[m].x, kb[m].y), q.four(kb[m].z, kb[m].w));
+            } else if (grew) {
+              *dst = rescale_e4m3x16(*dst, ratio);
+            }
+          }
+        } else {
+          const int a = max(o0 - run * 16, 0), b = has ? min(o1 - run * 16, 16) : 0;   // slots [a, b) of the run are new
+          const bool merge = !has || a > 0 || b < 16;
+          uint32_t qv[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) qv[i] = q.four(va[i].x, va[i].y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 4 * lane + e;
+            uint4* dst = reinterpret_cast<uint4*>(p.v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t lo = __byte_perm(qv[4 * j], qv[4 * j + 1], 0x0040 + 0x0011 * e);
+              const uint32_t hi = __byte_perm(qv[4 * j + 2], qv[4 * j + 3], 0x0040 + 0x0011 * e);
+              w[j] = __byte_perm(lo, hi, 0x5410);
+            }
+            if (merge) {
+              uint4 was = *dst;
+              if (grew) was = rescale_e4m3x16(was, ratio);
+              const uint32_t o4[4] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // bytes of word j that are new: slots 4 j .. 4 j + 3 inside [a, b)
+                const int from = min(max(a - 4 * j, 0), 4), to = min(max(b - 4 * j, 0), 4);
+                const uint32_t below_to = to >= 4 ? 0xffffffffu : (1u << (8 * to)) - 1u;
+                const uint32_t below_from = from >= 4 ? 0xffffffffu : (1u << (8 * from)) - 1u;
+                const uint32_t fresh_bytes = below_to & ~below_from;
+                w[j] = (w[j] & fresh_bytes) | (o4[j] & ~fresh_bytes);
+              }
+            }
+            *dst = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (want_bounds && sub == 0 && f == 0) {
+        uint4* at_lo = reinterpret_cast<uint4*>(p.bounds + (int64_t)blk * p.b_stride_block + (int64_t)head * p.b_stride_head + c * 16);
+        uint4* at_hi = at_lo + kD / 16;
+        uint32_t l4[4], h4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l4[j] = q.four(lo8[2 * j], lo8[2 * j + 1]), h4[j] = q.four(hi8[2 * j], hi8[2 * j + 1]);
+        if (!fresh) {
+          uint4 ol = *at_lo, oh = *at_hi;
+          if (grew) ol = rescale_e4m3x16(ol, ratio), oh = rescale_e4m3x16(oh, ratio);
+          const uint32_t wl[4] = {ol.x, ol.y, ol.z, ol.w}, wh[4] = {oh.x, oh.y, oh.z, oh.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a[4], b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              a[e] = fminf(e4m3_to_f32(l4[j] >> (8 * e)), e4m3_to_f32(wl[j] >> (8 * e)));
+              b[e] = fmaxf(e4m3_to_f32(h4[j] >> (8 * e)), e4m3_to_f32(wh[j] >> (8 * e)));
+            }
+            l4[j] = pack_e4m3x4(a[0], a[1], a[2], a[3]);
+            h4[j] = pack_e4m3x4(b[0], b[1], b[2], b[3]);
+          }
+        }
+        *at_lo = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+        *at_hi = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+      }
+    }
+    // every warp of the unit has read the old scale (before the barrier of the maximum, or, with one
+    // warp, by the lanes above): the new one may go there
+    __syncwarp();
+    if (p.per_block && live && o1 > o0 && sub == 0 && lane == 0) *scale_at = scale;
+    if (WPU > 1) __syncthreads();   // the reduction buffers are free for the next unit
+  }
+}
+
+}  // namespace pa

@@ -96,7 +96,7 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint32_t bar, uint32_t parity
 // code, and the kernels' hot loops should stay inside the instruction cache.  (A tighter loop,
 // four instructions a poll in one asm block, measured slower: the waiting roles then poll more
 // often and take more issue slots from the warps that compute.)
-__device__ __noinline__ bool mbar_wait_poll(uint32_t bar, uint32_t parity) {
+static __device__ __noinline__ bool mbar_wait_poll(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
   for (uint32_t it = 0; it < kWaitPollLimit; ++it) {
     if (mbar_try_wait_hint(bar, parity, kPollSuspendNs)) return true;

@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "../../include/pa_decode_sm100.h"
+#include "pa_host.h"
 #include "pa_partition_bf16.cuh"
 #include "pa_partition_fp8.cuh"
 #include "pa_partition_tc.cuh"
@@ -18,16 +19,12 @@
 #include "pa_stream_probe.cuh"
 
 namespace {
-
 thread_local int g_last_cuda_error = 0;
-
-struct DeviceInfo {
-  int sm_count = 0;
-  int max_smem_optin = 0;
-  bool ready = false;
-};
 constexpr int kMaxDevices = 64;
-DeviceInfo g_dev[kMaxDevices];
+pa_host::DeviceInfo g_dev[kMaxDevices];
+}  // namespace
+
+namespace pa_host {
 
 int cuda_fail(cudaError_t e) {
   g_last_cuda_error = (int)e;
@@ -54,6 +51,14 @@ int device_info(DeviceInfo** out) {
   *out = &d;
   return PA_OK;
 }
+
+}  // namespace pa_host
+
+namespace {
+
+using pa_host::cuda_fail;
+using pa_host::device_info;
+using pa_host::DeviceInfo;
 
 // cuTensorMapEncodeTiled, looked up through the runtime so that the library does not link libcuda.
 typedef CUresult (*TensorMapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
