@@ -312,7 +312,8 @@ int pa_cache_write_sm100(const PaCacheWriteParams* params, void* stream);
  * length with them is context_lens[s].  A page and kv head that receives rows gets, for its keys and
  * its values separately,
  *   want  = the smallest power of two >= max|x| / 448 over the finite elements, at least 2^-40
- *   scale = want where a row goes to the page's first slot, else max(old scale, want)
+ *   scale = want where a row goes to the page's first slot, else max(old scale, want), where an old scale
+ *           that is no power of two counts as the next one
  *   old codes = e4m3fn(code * (old scale / scale)) for every slot without a new row, where the scale grew
  *   new codes = e4m3fn(x / scale), saturating
  * and key_bounds (optional) the smallest and the largest key code of every head dim over the page's

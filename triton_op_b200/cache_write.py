@@ -128,8 +128,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     is ``sequence_lengths[s]`` -- the tensors the decode call after it takes.  ``key_scale`` /
     ``value_scale`` fp32 ``[num_blocks, num_kv_heads, 1, 1]`` are read and written: a page that begins with
     this call gets the smallest power of two that brings its largest value to 448 at most (2**-40 at
-    least); in a page with tokens the scale grows if it has to, and the page's codes are brought to the
-    new scale.  Nothing else of the cache changes.  0-dim scales (per tensor) are read only.
+    least); in a page with tokens the scale grows if it has to (or to the next power of two if it is none),
+    and the page's codes are brought to the new scale.  Nothing else of the cache changes.  0-dim scales (per tensor) are read only.
 
     ``key_bounds``: e4m3fn ``[num_blocks, num_kv_heads, 2, head_size]``, the smallest and largest key
     code of every head dim over the page's tokens, kept up to date for

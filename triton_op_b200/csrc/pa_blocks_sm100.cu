@@ -85,7 +85,7 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   k.num_blocks = p->num_blocks;
   k.width = p->max_blocks_per_seq;
   k.v_trans = p->v_layout == PA_V_TRANSPOSED;
-  k.per_block = p->kv_quant_mode == PA_QUANT_PER_BLOCK;
+  const bool blk = p->kv_quant_mode == PA_QUANT_PER_BLOCK;
   k.key_stride_tok = p->key_stride_token;
   k.key_stride_head = p->key_stride_head;
   k.value_stride_tok = p->value_stride_token;
@@ -111,9 +111,9 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   const size_t smem = (size_t)(p->num_seqs + 1) * 4;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (p->block_size) {
-    case 16: return launch(pa::pa_cache_append_kernel<16, 1>, dim3((unsigned)grid), threads, smem, st, k);
-    case 64: return launch(pa::pa_cache_append_kernel<64, 4>, dim3((unsigned)grid), threads, smem, st, k);
-    default: return launch(pa::pa_cache_append_kernel<1024, 16>, dim3((unsigned)grid), threads, smem, st, k);
+    case 16: return launch(blk ? pa::pa_cache_append_kernel<16, 1, true> : pa::pa_cache_append_kernel<16, 1, false>, dim3((unsigned)grid), threads, smem, st, k);
+    case 64: return launch(blk ? pa::pa_cache_append_kernel<64, 4, true> : pa::pa_cache_append_kernel<64, 4, false>, dim3((unsigned)grid), threads, smem, st, k);
+    default: return launch(blk ? pa::pa_cache_append_kernel<1024, 16, true> : pa::pa_cache_append_kernel<1024, 16, false>, dim3((unsigned)grid), threads, smem, st, k);
   }
 }
 

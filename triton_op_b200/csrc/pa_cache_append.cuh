@@ -4,7 +4,8 @@
 // For a page and kv head that receives the rows x_i (keys and values separately):
 //   want  = the smallest power of two >= max|x| / 448 (finite elements; at least 2^-40)
 //   scale = want                        where the rows begin the page
-//         = max(old scale, want)        where the page holds tokens already
+//         = max(old scale, want)        where the page holds tokens already (an old scale that is no
+//                                       power of two counts as the next one)
 //   codes of the page := e4m3(code * (old scale / scale))   where the scale grew
 //   code_i = e4m3(x_i / scale), saturating
 // A scale that is a power of two costs no precision (e4m3 keeps its four significant bits wherever
@@ -45,7 +46,7 @@ struct CacheAppendParams {
   const int32_t* context_lens; // [S]: lengths with the new tokens
   const int32_t* row_start;    // [S + 1]: the sequence's first row in key / value
   int32_t* status;
-  int32_t T, S, Hkv, num_blocks, width, v_trans, per_block;
+  int32_t T, S, Hkv, num_blocks, width, v_trans;
   int64_t key_stride_tok, key_stride_head;       // elements
   int64_t value_stride_tok, value_stride_head;
   int64_t kc_stride_block, kc_stride_head;       // bytes
@@ -99,24 +100,42 @@ __device__ __forceinline__ uint32_t bf16x2_max(uint32_t a, uint32_t b) {
   return r;
 }
 
-// x / scale for a whole unit: an exact product where the scale is a power of two.
-struct Quantiser {
-  float scale, inv;
-  bool exact;
-  __device__ explicit Quantiser(float s) : scale(s), inv(1.0f / s) {
-    const uint32_t u = __float_as_uint(s);
-    exact = (u & 0x7fffffu) == 0u && u >= (2u << 23) && u <= (252u << 23);
-  }
-  __device__ __forceinline__ float operator()(float x) const { return exact ? x * inv : __fdiv_rn(x, scale); }
-  __device__ __forceinline__ uint32_t four(uint32_t w0, uint32_t w1) const {   // bf16 pairs -> e4m3 codes
-    const Quantiser& q = *this;
-    return pack_e4m3x4(q(bf16_lo_to_f32(w0)), q(bf16_hi_to_f32(w0)), q(bf16_lo_to_f32(w1)), q(bf16_hi_to_f32(w1)));
-  }
-};
+// Two words of bf16 pairs -> four e4m3 codes of x / scale.  A page's scale is a power of two, so its
+// reciprocal and the product are exact; a per-tensor scale may be anything and is divided by.
+template <bool DIVIDE>
+__device__ __forceinline__ uint32_t quantise_four(uint32_t w0, uint32_t w1, float scale, float inv) {
+  if (DIVIDE)
+    return pack_e4m3x4(__fdiv_rn(bf16_lo_to_f32(w0), scale), __fdiv_rn(bf16_hi_to_f32(w0), scale),
+                       __fdiv_rn(bf16_lo_to_f32(w1), scale), __fdiv_rn(bf16_hi_to_f32(w1), scale));
+  return pack_e4m3x4(bf16_lo_to_f32(w0) * inv, bf16_hi_to_f32(w0) * inv, bf16_lo_to_f32(w1) * inv, bf16_hi_to_f32(w1) * inv);
+}
+// The smallest power of two >= s, for a positive s (what a page's scale becomes if it came as none).
+__device__ __forceinline__ float up_to_power(float s) {
+  const uint32_t u = __float_as_uint(s);
+  return (u & 0x7fffffu) == 0u ? s : __uint_as_float(min((u >> 23) + 1u, 254u) << 23);
+}
 
-// BS: tokens per page.  WPU: warps per unit.
-template <int BS, int WPU>
-__global__ void __launch_bounds__(WPU > 4 ? WPU * 32 : 128)
+// Brings a page's codes to a larger scale: runs first, first + step, ... of 16 slots.  A rare path, out
+// of line so that the common one keeps its registers.  Each thread touches the 16-byte pieces that
+// it writes in the kernel below, so nothing has to be waited for in between.
+template <int BS>
+static __device__ __noinline__ void rescale_runs(uint8_t* cache, bool is_v, bool v_trans, int first, int step, float ratio, int lane) {
+#pragma unroll 1
+  for (int run = first; run < BS / 16; run += step) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 4 * lane + e;
+      uint4* at = reinterpret_cast<uint4*>(
+          is_v ? (v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16)
+               : cache + ((int64_t)(lane >> 2) * BS + run * 16 + 4 * e + (lane & 3)) * 16);
+      *at = rescale_e4m3x16(*at, ratio);
+    }
+  }
+}
+
+// BS: tokens per page.  WPU: warps per unit.  PER_BLOCK: scales per (page, kv head), else per tensor.
+template <int BS, int WPU, bool PER_BLOCK>
+__global__ void __launch_bounds__(WPU > 4 ? WPU * 32 : 128, WPU > 4 ? 1 : 5)
 pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
   constexpr int kThreads = WPU > 4 ? WPU * 32 : 128;
   constexpr int kUnits = kThreads / 32 / WPU;                       // units a CTA works on at a time
@@ -216,19 +235,19 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     const int64_t tok_bytes = 2 * (is_v ? p.value_stride_tok : p.key_stride_tok);
     uint8_t* cache = is_v ? p.value_cache + (int64_t)blk * p.vc_stride_block + (int64_t)head * p.vc_stride_head
                           : p.key_cache + (int64_t)blk * p.kc_stride_block + (int64_t)head * p.kc_stride_head;
-    float* scale_at = (is_v ? p.v_scale : p.k_scale) + (p.per_block ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
+    float* scale_at = (is_v ? p.v_scale : p.k_scale) + (PER_BLOCK ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
     const float old_scale = live ? *scale_at : 1.0f;
     // keys: lane = (chunk c of 16 dims, phase f), slots f, f + 4, f + 8, f + 12 of a run, 32 bytes each
     // values: lane = head dims 4 lane .. 4 lane + 3 of every slot of a run, 8 bytes each
     const int c = lane >> 2, f = lane & 3;
-    uint4 ka[4], kb[4];   // keys of the warp's (last) run
-    uint2 va[16];         // values
+    uint32_t raw[32];     // the warp's (last) run: keys [slot f + 4 m][8 words], values [slot][2 words]
     auto load_run = [&](int run) {
       if (is_v) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int o = run * 16 + i;
-          va[i] = (o >= o0 && o < o1) ? __ldg(reinterpret_cast<const uint2*>(src + (int64_t)(o - o0) * tok_bytes) + lane) : make_uint2(0u, 0u);
+          const uint2 v = (o >= o0 && o < o1) ? __ldg(reinterpret_cast<const uint2*>(src + (int64_t)(o - o0) * tok_bytes) + lane) : make_uint2(0u, 0u);
+          raw[2 * i] = v.x, raw[2 * i + 1] = v.y;
         }
       } else {
 #pragma unroll
@@ -236,8 +255,9 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
           const int o = run * 16 + 4 * m + f;
           const bool in = o >= o0 && o < o1;
           const uint4* at = reinterpret_cast<const uint4*>(src + (int64_t)(o - o0) * tok_bytes + c * 32);
-          ka[m] = in ? __ldg(at) : make_uint4(0u, 0u, 0u, 0u);
-          kb[m] = in ? __ldg(at + 1) : make_uint4(0u, 0u, 0u, 0u);
+          const uint4 a = in ? __ldg(at) : make_uint4(0u, 0u, 0u, 0u), b = in ? __ldg(at + 1) : make_uint4(0u, 0u, 0u, 0u);
+          raw[8 * m] = a.x, raw[8 * m + 1] = a.y, raw[8 * m + 2] = a.z, raw[8 * m + 3] = a.w;
+          raw[8 * m + 4] = b.x, raw[8 * m + 5] = b.y, raw[8 * m + 6] = b.z, raw[8 * m + 7] = b.w;
         }
       }
     };
@@ -258,18 +278,23 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
       if (run < run0 || run >= run1) continue;
       load_run(run);
       loaded = run;
-      if (is_v) {
+      // non-negative bf16 bit patterns order like integers; infinity and NaN lie above all others
+      uint32_t any = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = __vmaxu2(top, __vmaxu2(finite_abs2(va[i].x), finite_abs2(va[i].y)));
-      } else {
+      for (int e = 0; e < 32; ++e) any = __vmaxu2(any, raw[e] & 0x7fff7fffu);
+      if ((any & 0xffffu) >= 0x7f80u || (any >> 16) >= 0x7f80u) {
+        any = 0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) any = __vmaxu2(any, finite_abs2(raw[e]));
+      }
+      top = __vmaxu2(top, any);
+      if (want_bounds) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const uint32_t w[8] = {ka[m].x, ka[m].y, ka[m].z, ka[m].w, kb[m].x, kb[m].y, kb[m].z, kb[m].w};
           const int o = run * 16 + 4 * m + f;
+          if (o >= o0 && o < o1) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            top = __vmaxu2(top, finite_abs2(w[e]));
-            if (o >= o0 && o < o1) lo8[e] = bf16x2_min(lo8[e], w[e]), hi8[e] = bf16x2_max(hi8[e], w[e]);
+            for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], raw[8 * m + e]), hi8[e] = bf16x2_max(hi8[e], raw[8 * m + e]);
           }
         }
       }
@@ -305,20 +330,21 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     const bool fresh = o0 == 0;
     float scale = old_scale, ratio = 1.0f;
     bool grew = false;
-    if (p.per_block) {
+    if (PER_BLOCK) {
       const float want = page_scale(__uint_as_float(top1 << 16));
-      scale = fresh ? want : fmaxf(old_scale, want);
+      scale = fresh ? want : fmaxf(up_to_power(old_scale), want);
       grew = !fresh && scale != old_scale;
       if (grew) ratio = __fdiv_rn(old_scale, scale);
     }
     if (live && o1 > o0) {
-      const Quantiser q(scale);
+      const float inv = 1.0f / scale;
+      if (PER_BLOCK && grew) rescale_runs<BS>(cache, is_v, p.v_trans != 0, sub, WPU, ratio, lane);
+      auto four = [&](uint32_t w0, uint32_t w1) -> uint32_t { return quantise_four<!PER_BLOCK>(w0, w1, scale, inv); };
 #pragma unroll 1
       for (int k = 0; k < kPerWarp; ++k) {
         const int run = mine(k);
-        const bool has = run >= run0 && run < run1;
-        if (run >= kRuns || !(has || grew)) continue;
-        if (has && run != loaded) {
+        if (run < run0 || run >= run1) continue;
+        if (run != loaded) {
           load_run(run);
           loaded = run;
         }
@@ -328,17 +354,16 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
             const int o = run * 16 + 4 * m + f;
             uint4* dst = reinterpret_cast<uint4*>(cache + ((int64_t)c * BS + o) * 16);
             if (o >= o0 && o < o1) {
-              *dst = make_uint4(q.four(ka[m].x, ka[m].y), q.four(ka[m].z, ka[m].w), q.four(kb[m].x, kb[m].y), q.four(kb[m].z, kb[m].w));
-            } else if (grew) {
-              *dst = rescale_e4m3x16(*dst, ratio);
+              *dst = make_uint4(four(raw[8 * m], raw[8 * m + 1]), four(raw[8 * m + 2], raw[8 * m + 3]),
+                                four(raw[8 * m + 4], raw[8 * m + 5]), four(raw[8 * m + 6], raw[8 * m + 7]));
             }
           }
         } else {
-          const int a = max(o0 - run * 16, 0), b = has ? min(o1 - run * 16, 16) : 0;   // slots [a, b) of the run are new
-          const bool merge = !has || a > 0 || b < 16;
+          const int a = max(o0 - run * 16, 0), b = min(o1 - run * 16, 16);   // slots [a, b) of the run are new
+          const bool merge = a > 0 || b < 16;
           uint32_t qv[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) qv[i] = q.four(va[i].x, va[i].y);
+          for (int i = 0; i < 16; ++i) qv[i] = four(raw[2 * i], raw[2 * i + 1]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int d = 4 * lane + e;
@@ -351,8 +376,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
               w[j] = __byte_perm(lo, hi, 0x5410);
             }
             if (merge) {
-              uint4 was = *dst;
-              if (grew) was = rescale_e4m3x16(was, ratio);
+              const uint4 was = *dst;
               const uint32_t o4[4] = {was.x, was.y, was.z, was.w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -373,7 +397,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
         uint4* at_hi = at_lo + kD / 16;
         uint32_t l4[4], h4[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) l4[j] = q.four(lo8[2 * j], lo8[2 * j + 1]), h4[j] = q.four(hi8[2 * j], hi8[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) l4[j] = four(lo8[2 * j], lo8[2 * j + 1]), h4[j] = four(hi8[2 * j], hi8[2 * j + 1]);
         if (!fresh) {
           uint4 ol = *at_lo, oh = *at_hi;
           if (grew) ol = rescale_e4m3x16(ol, ratio), oh = rescale_e4m3x16(oh, ratio);
@@ -397,7 +421,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     // every warp of the unit has read the old scale (before the barrier of the maximum, or, with one
     // warp, by the lanes above): the new one may go there
     __syncwarp();
-    if (p.per_block && live && o1 > o0 && sub == 0 && lane == 0) *scale_at = scale;
+    if (PER_BLOCK && live && o1 > o0 && sub == 0 && lane == 0) *scale_at = scale;
     if (WPU > 1) __syncthreads();   // the reduction buffers are free for the next unit
   }
 }
