@@ -184,14 +184,13 @@ def lib() -> C.CDLL:
     return L
 
 
-def launch(device: torch.device, fn, where: str, *args) -> None:
-    """Calls a launching entry point with ``device`` current, on torch's current stream of it."""
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), where)
+def launch(index: int, fn, where: str, *args) -> None:
+    """Calls a launching entry point with device ``index`` current, on torch's current stream of it."""
+    if index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(index).cuda_stream), where)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream), where)
+        with torch.cuda.device(index):
+            check(fn(*args, torch.cuda.current_stream(index).cuda_stream), where)
 
 
 def check(status: int, where: str) -> None:

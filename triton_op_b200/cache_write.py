@@ -160,10 +160,10 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     if key_scale.dim() == 0 and value_scale.dim() == 0:
         mode, s_block, s_head = _lib.PA_QUANT_PER_TENSOR, 0, 0
     else:
-        _check_block_scales(key_scale, value_scale, key_cache, dev)
-        if (num_blocks > 1 and key_scale.stride(0) == 0) or (num_kv_heads > 1 and key_scale.stride(1) == 0):
+        s_block, s_head = _check_block_scales(key_scale, value_scale, key_cache)
+        if (num_blocks > 1 and s_block == 0) or (num_kv_heads > 1 and s_head == 0):
             raise PaArgumentError("block kv scales are written: every page and kv head needs a place of its own")
-        mode, s_block, s_head = _lib.PA_QUANT_PER_BLOCK, key_scale.stride(0), key_scale.stride(1)
+        mode = _lib.PA_QUANT_PER_BLOCK
     b_block = b_head = 0
     if key_bounds is not None:
         if not (key_bounds.dtype == FP8_DTYPE and key_bounds.shape == (num_blocks, num_kv_heads, 2, head_size)
@@ -200,4 +200,4 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
         _lib.PA_V_TRANSPOSED if trans else _lib.PA_V_NORMAL, 0,
         key.stride(0), key.stride(1), value.stride(0), value.stride(1), key_cache.stride(0), key_cache.stride(1),
         value_cache.stride(0), value_cache.stride(1), s_block, s_head, b_block, b_head, block_tables.stride(0)))
-    _lib.launch(dev, _lib.lib().pa_cache_append_sm100, "pa_cache_append_sm100", C.byref(p))
+    _lib.launch(key.get_device(), _lib.lib().pa_cache_append_sm100, "pa_cache_append_sm100", C.byref(p))

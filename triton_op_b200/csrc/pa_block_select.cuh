@@ -4,14 +4,19 @@
 // in the order of the context, with the number of tokens those pages hold.
 //
 // One CTA per (sequence, kv head).  Scores become unsigned keys of the same order (NaN below
-// everything).  The key of rank top_k is found by narrowing a key range: a histogram of 2048 equal
-// bins over [smallest, largest] key, the bin in which the rank falls becomes the next range.  Bins
-// over the ACTUAL range spread the shared-memory counters, where a fixed digit would count most
-// pages of a head in two or three of them (their scores share sign and exponent); a 32-bit range is down
-// to single keys after three rounds at most, and as a rule the search ends after two, as soon as the
-// bin is taken whole.  Then one ordered pass writes the pages above the threshold and the first of those on it.
-// Nothing here is a sum of floating-point numbers and counters are only added to: the same
-// scores give the same table whatever the order of the threads.
+// everything).  The key of rank top_k is found by narrowing a key range: a histogram of equal bins over
+// [smallest, largest] key, then the bin in which the rank falls.  Bins over the ACTUAL range spread the
+// shared-memory counters, where a fixed digit would count most pages of a head in two or three of
+// them (their scores share sign and exponent), and leave few keys in the rank's bin: up to 32 of them
+// are ranked outright by a warp, more make the next range.  Then one ordered pass writes the pages above
+// the threshold and the first of those on it.  Nothing here is a sum of floating-point numbers and
+// counters are only added to: the same scores give the same table whatever the order of the threads.
+//
+// What bounds it: 4 bytes per page and kv head, a few MB at most; it is the latency of one CTA's chain
+// (lengths and scores, range, histogram, rank, ordered pass: six block barriers).  So keys stay in
+// registers, a warp's pages are rows of 32 (coalesced loads, ballots give a page's place among
+// the warp's), every warp combines the block's partial results for itself instead of waiting for
+// one that does, and the CTA is as large as the table is wide.
 #pragma once
 
 #include "../../include/pa_decode_sm100.h"
@@ -20,10 +25,9 @@
 
 namespace pa {
 
-constexpr int kSelectThreads = 512;
-constexpr int kSelectItems = 16;     // pages per thread and sweep
-constexpr int kSelectSweep = kSelectThreads * kSelectItems;
-constexpr int kSelectBins = 2048;
+// Threads and pages per thread by the width of the table: a CTA holds THREADS * ITEMS pages at a time and
+// sweeps over more than that.
+constexpr int kSelectSmall = 128 * 4, kSelectMedium = 256 * 8, kSelectLarge = 512 * 16;
 
 struct BlockSelectParams {
   const float* scores;         // [S, Hkv, >= pages]
@@ -38,178 +42,211 @@ struct BlockSelectParams {
   int64_t out_stride_seq, out_stride_head;
 };
 
-// Unsigned key with the order of the floats; NaN is below -inf.
+// Unsigned key with the order of the floats, NaN below -inf.  Two keys no score has mark the pages that do
+// not compete: kKeyNone for places past the context, kKeyKept for the kept pages.
+constexpr uint32_t kKeyNone = 0u, kKeyNan = 1u, kKeyKept = 0xffffffffu;
 __device__ __forceinline__ uint32_t score_key(float x) {
   const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
+  if ((u & 0x7fffffffu) > 0x7f800000u) return kKeyNan;
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kSelectThreads)
+template <int THREADS, int ITEMS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1)
 pa_block_select_kernel(const __grid_constant__ BlockSelectParams p) {
-  __shared__ int bins[kSelectBins];
-  __shared__ int warp_sums[kSelectThreads / 32], warp_sums2[kSelectThreads / 32];
-  __shared__ uint32_t warp_lo[kSelectThreads / 32], warp_hi[kSelectThreads / 32];
-  __shared__ int found_bin, found_above, found_count;
+  constexpr int kWarps = THREADS / 32, kSweep = THREADS * ITEMS, kPer = 4, kBins = kPer * THREADS;
+  __shared__ __align__(16) int bins[kBins];
+  __shared__ uint32_t part_lo[32], part_hi[32];
+  __shared__ int part_sum[32];
+  __shared__ uint32_t part_pair[32];
+  __shared__ uint32_t cand[32];
+  __shared__ int found[4];   // bin, keys above it, keys in it; candidates stored
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seq = (int)blockIdx.x / p.Hkv, head = (int)blockIdx.x - seq * p.Hkv;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) bins[i * THREADS + tid] = 0;
   grid_dependency_wait();
   grid_launch_dependents();
+
+  const float* scores = p.scores + (int64_t)seq * p.sc_stride_seq + (int64_t)head * p.sc_stride_head;
+  uint32_t keys[ITEMS];
+  // a warp's pages are ITEMS rows of 32: page of item j
+  auto page_of = [&](int sweep, int j) -> int { return sweep + (warp * ITEMS + j) * 32 + lane; };
+  // (the scores of a narrow table are requested before the length is known: the buffer has its full width)
+  constexpr bool kEarly = ITEMS <= 8;
+  const bool one_sweep = p.width <= kSweep;
+  float early[kEarly ? ITEMS : 1];
+  if (kEarly) {
+#pragma unroll
+    for (int j = 0; j < (kEarly ? ITEMS : 1); ++j) {
+      const int i = page_of(0, j);
+      early[j] = i < p.width ? scores[i] : 0.f;
+    }
+  }
+
   const int ctx = p.context_lens[seq];
   const int64_t cap = (int64_t)p.width * p.block_size;
-  const int tokens = ctx <= 0 ? 0 : (int)min(cap, (int64_t)ctx);
+  const int64_t tokens = ctx <= 0 ? 0 : min(cap, (int64_t)ctx);
   if (ctx > cap && p.status && tid == 0) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
-  const int pages = (int)(((int64_t)tokens + p.block_size - 1) / p.block_size);
+  const int pages = (int)((tokens + p.block_size - 1) / p.block_size);
   const int held = min(pages, p.top_k);
   if (head == 0 && tid == 0)   // every page but the last is full
     p.lengths[seq] = held == 0 ? 0 : (int)min((int64_t)0x7fffffff, (int64_t)held * p.block_size - ((int64_t)pages * p.block_size - tokens));
   const int32_t* table = p.block_tables + (int64_t)seq * p.bt_stride_seq;
   int32_t* out = p.tables + (int64_t)seq * p.out_stride_seq + (int64_t)head * p.out_stride_head;
-  for (int i = held + tid; i < p.top_k; i += kSelectThreads) out[i] = 0;
+  for (int i = held + tid; i < p.top_k; i += THREADS) out[i] = 0;
   if (pages <= p.top_k) {
-    for (int i = tid; i < pages; i += kSelectThreads) out[i] = __ldg(table + i);
+    for (int i = tid; i < pages; i += THREADS) out[i] = __ldg(table + i);
     return;
   }
 
   // keep_first + keep_last <= top_k < pages, so the two ends do not meet
-  const float* scores = p.scores + (int64_t)seq * p.sc_stride_seq + (int64_t)head * p.sc_stride_head;
   const int first = p.keep_first, last = pages - p.keep_last;   // pages [first, last) compete
-  int need = p.top_k - p.keep_first - p.keep_last;              // for this many places
-  const bool one_sweep = pages <= kSelectSweep;
-  uint32_t keys[kSelectItems];
-  // thread tid holds pages sweep + tid * kSelectItems + [0, kSelectItems)
+  int need = p.top_k - p.keep_first - p.keep_last;              // for these places
+  uint32_t lo = 0xffffffffu, hi = 0u;                           // range of the competing keys
   auto load = [&](int sweep) {
-    const int at = sweep + tid * kSelectItems;
 #pragma unroll
-    for (int j = 0; j < kSelectItems; ++j) keys[j] = (at + j >= first && at + j < last) ? score_key(scores[at + j]) : 0u;
+    for (int j = 0; j < ITEMS; ++j) {
+      const int i = page_of(sweep, j);
+      if (i >= first && i < last) {
+        keys[j] = score_key(kEarly && one_sweep ? early[kEarly ? j : 0] : scores[i]);
+        lo = min(lo, keys[j]), hi = max(hi, keys[j]);
+      } else {
+        keys[j] = i < pages ? kKeyKept : kKeyNone;
+      }
+    }
   };
-  if (one_sweep) load(0);
+  for (int sweep = 0; sweep < pages; sweep += kSweep) load(sweep);
+  auto reload = [&](int sweep) {     // the same keys, the range as it has become
+    const uint32_t keep_lo = lo, keep_hi = hi;
+    load(sweep);
+    lo = keep_lo, hi = keep_hi;
+  };
 
-  uint32_t lo = 0xffffffffu, hi = 0u;   // range of the competing keys
-  for (int sweep = 0; sweep < pages; sweep += kSelectSweep) {
-    if (!one_sweep) load(sweep);
-    const int at = sweep + tid * kSelectItems;
-#pragma unroll
-    for (int j = 0; j < kSelectItems; ++j) {
-      if (at + j >= first && at + j < last) lo = min(lo, keys[j]), hi = max(hi, keys[j]);
-    }
-  }
-  lo = __reduce_min_sync(kFullMask, lo);
-  hi = __reduce_max_sync(kFullMask, hi);
-  if (lane == 0) warp_lo[warp] = lo, warp_hi[warp] = hi;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelectThreads / 32; ++w) lo = min(lo, warp_lo[w]), hi = max(hi, warp_hi[w]);
-
-  // The `need` best of the keys in [lo, hi]; all keys above hi are taken already.  Ends with
-  // threshold: keys > threshold are taken, and `ties` of those equal to it.
-  uint32_t threshold = hi;
+  // keys above the threshold are taken, and the first `ties` of those equal to it (kept pages are above
+  // any; with no place to compete for, they alone)
+  uint32_t threshold = kKeyKept - 1u;
   int ties = 0;
-  while (need > 0) {
-    if (lo == hi) {        // what is left is one key
-      threshold = lo;
-      ties = need;
-      break;
-    }
-    int shift = 0;
-    while (((hi - lo) >> shift) >= (uint32_t)kSelectBins) ++shift;
-    for (int i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+  if (need > 0) {
+    lo = __reduce_min_sync(kFullMask, lo);
+    hi = __reduce_max_sync(kFullMask, hi);
+    if (lane == 0) part_lo[warp] = lo, part_hi[warp] = hi;
+    if (tid == 0) found[3] = 0;
     __syncthreads();
-    for (int sweep = 0; sweep < pages; sweep += kSelectSweep) {
-      if (!one_sweep) load(sweep);
-      const int at = sweep + tid * kSelectItems;
-#pragma unroll
-      for (int j = 0; j < kSelectItems; ++j) {
-        if (at + j >= first && at + j < last && keys[j] >= lo && keys[j] <= hi) atomicAdd(&bins[(keys[j] - lo) >> shift], 1);
-      }
-    }
-    __syncthreads();
-    // the bin that holds rank `need`, counted from the top: thread tid has the bins top - 4 tid - {0..3}
-    constexpr int kPer = kSelectBins / kSelectThreads;
-    int own[kPer], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) own[j] = bins[kSelectBins - 1 - tid * kPer - j], sum += own[j];
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFullMask, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) warp_sums[warp] = incl;
-    __syncthreads();
-    int before = incl - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-    if (before < need && before + sum >= need) {
-      int above = before;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        if (above < need && above + own[j] >= need) {
-          found_bin = kSelectBins - 1 - tid * kPer - j;
-          found_above = above;
-          found_count = own[j];
-        }
-        above += own[j];
-      }
-    }
-    __syncthreads();
-    const uint32_t bin_lo = lo + ((uint32_t)found_bin << shift);
-    const uint32_t bin_hi = min(hi, bin_lo + ((1u << shift) - 1u));
-    need -= found_above;
-    if (need == found_count) {   // the whole bin is taken: everything from bin_lo up
-      threshold = bin_lo;
-      ties = 0x7fffffff;
-      break;
-    }
-    lo = bin_lo;
-    hi = bin_hi;
-  }
+    lo = __reduce_min_sync(kFullMask, lane < kWarps ? part_lo[lane] : 0xffffffffu);
+    hi = __reduce_max_sync(kFullMask, lane < kWarps ? part_hi[lane] : 0u);
 
-  // ---- ordered pass: page i goes to place (taken pages before it)
-  int placed = 0, tied = 0;     // over the sweeps so far
-  for (int sweep = 0; sweep < pages; sweep += kSelectSweep) {
-    if (!one_sweep) load(sweep);
-    const int at = sweep + tid * kSelectItems;
-    int above = 0, equal = 0;
-    const bool any = p.top_k > p.keep_first + p.keep_last;
+    while (true) {
+      if (lo == hi) {        // what is left is one key
+        threshold = lo;
+        ties = need;
+        break;
+      }
+      // the smallest shift that maps the range into the bins
+      const int width_bits = 32 - __clz((int)(hi - lo));
+      constexpr int kBinBits = 31 - __builtin_clz(kBins);
+      const int shift = max(width_bits - kBinBits, 0);
+      for (int sweep = 0; sweep < pages; sweep += kSweep) {
+        if (!one_sweep) reload(sweep);
 #pragma unroll
-    for (int j = 0; j < kSelectItems; ++j) {
-      const int i = at + j;
-      if (i < pages && (i < first || i >= last)) ++above;
-      else if (i < pages && any) above += keys[j] > threshold, equal += keys[j] == threshold;
-    }
-    int sum = above, sum2 = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(kFullMask, sum, o), v2 = __shfl_up_sync(kFullMask, sum2, o);
-      if (lane >= o) sum += v, sum2 += v2;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = sum, warp_sums2[warp] = sum2;
-    __syncthreads();
-    int before = placed + sum - above, ties_before = tied + sum2 - equal;
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
-      if (w < warp) before += warp_sums[w], ties_before += warp_sums2[w];
-      placed += warp_sums[w], tied += warp_sums2[w];
-    }
-#pragma unroll
-    for (int j = 0; j < kSelectItems; ++j) {
-      const int i = at + j;
-      bool take = false;
-      if (i < pages && (i < first || i >= last)) take = true;
-      else if (i < pages && any && keys[j] > threshold) take = true;
-      else if (i < pages && any && keys[j] == threshold) {
-        if (ties_before < ties) {
-          const int place = before + min(ties_before, ties);
-          if (place < p.top_k) out[place] = __ldg(table + i);
+        for (int j = 0; j < ITEMS; ++j) {
+          if (keys[j] >= lo && keys[j] <= hi) atomicAdd(&bins[(keys[j] - lo) >> shift], 1);
         }
-        ++ties_before;
-        continue;
       }
-      if (take) {
-        const int place = before + min(ties_before, ties);
-        if (place < p.top_k) out[place] = __ldg(table + i);
-        ++before;
+      __syncthreads();
+      // the bin that holds rank `need`, counted from the top: thread tid has four bins from kBins - 1 - 4 tid down
+      const int4 own = *reinterpret_cast<const int4*>(&bins[kBins - 4 - tid * kPer]);
+      const int sum = own.x + own.y + own.z + own.w;
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFullMask, incl, o);
+        if (lane >= o) incl += v;
       }
+      if (lane == 31) part_sum[warp] = incl;
+      __syncthreads();
+      const int before = incl - sum + (int)__reduce_add_sync(kFullMask, lane < warp ? (unsigned)part_sum[lane] : 0u);
+      *reinterpret_cast<int4*>(&bins[kBins - 4 - tid * kPer]) = make_int4(0, 0, 0, 0);   // for the next round
+      if (before < need && before + sum >= need) {
+        const int top[4] = {own.w, own.z, own.y, own.x};
+        int above = before;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (above < need && above + top[j] >= need) {
+            found[0] = kBins - 1 - tid * kPer - j;
+            found[1] = above;
+            found[2] = top[j];
+          }
+          above += top[j];
+        }
+      }
+      __syncthreads();
+      const uint32_t bin_lo = lo + ((uint32_t)found[0] << shift);
+      const uint32_t bin_hi = min(hi, bin_lo + ((1u << shift) - 1u));
+      const int inside = found[2];
+      need -= found[1];
+      if (need == inside) {   // the whole bin is taken: everything from bin_lo up
+        threshold = bin_lo;
+        ties = 0x7fffffff;
+        break;
+      }
+      lo = bin_lo;
+      hi = bin_hi;
+      if (inside > 32 || lo == hi) continue;
+      // few are left: gather them, and every warp finds the need-th for itself (ties share a key, so
+      // the order in which they were gathered does not matter)
+      for (int sweep = 0; sweep < pages; sweep += kSweep) {
+        if (!one_sweep) reload(sweep);
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+          if (keys[j] >= lo && keys[j] <= hi) cand[atomicAdd(&found[3], 1) & 31] = keys[j];
+        }
+      }
+      __syncthreads();
+      const uint32_t mine = lane < inside ? cand[lane] : 0u;
+      int above = 0, equal = 0;
+      for (int l = 0; l < inside; ++l) {
+        const uint32_t other = __shfl_sync(kFullMask, mine, l);
+        above += other > mine;
+        equal += other == mine;
+      }
+      const unsigned hit = __ballot_sync(kFullMask, lane < inside && above < need && above + equal >= need);
+      const int src = __ffs((int)hit) - 1;
+      threshold = __shfl_sync(kFullMask, mine, src);
+      ties = need - __shfl_sync(kFullMask, above, src);
+      break;
+    }
+  }
+  // ---- ordered pass: a taken page goes to the place that the taken pages before it leave
+  const unsigned below = (1u << lane) - 1u;
+  int placed = 0, tied = 0;     // over the sweeps so far: pages above the threshold (or kept), pages on it
+  for (int sweep = 0; sweep < pages; sweep += kSweep) {
+    if (!one_sweep) reload(sweep);
+    int n_above = 0, n_equal = 0;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) n_above += keys[j] > threshold, n_equal += keys[j] == threshold;
+    const uint32_t sums = __reduce_add_sync(kFullMask, (uint32_t)n_above | ((uint32_t)n_equal << 16));   // at most kSweep <= 8192 each
+    if (sweep > 0) __syncthreads();
+    if (lane == 0) part_pair[warp] = sums;
+    __syncthreads();
+    const uint32_t pair = lane < kWarps ? part_pair[lane] : 0u;
+    const uint32_t mine = __reduce_add_sync(kFullMask, lane < warp ? pair : 0u), all = __reduce_add_sync(kFullMask, pair);
+    int before = placed + (int)(mine & 0xffffu), ties_before = tied + (int)(mine >> 16);
+    placed += (int)(all & 0xffffu);
+    tied += (int)(all >> 16);
+    if (sums == 0) continue;   // nothing of this warp's
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const unsigned any = __ballot_sync(kFullMask, keys[j] >= threshold);
+      if (any == 0) continue;
+      const unsigned is_above = __ballot_sync(kFullMask, keys[j] > threshold), is_equal = any & ~is_above;
+      const int rank_equal = ties_before + __popc(is_equal & below);
+      if (((is_above >> lane) & 1u) || (((is_equal >> lane) & 1u) && rank_equal < ties)) {
+        const int place = before + __popc(is_above & below) + min(rank_equal, ties);
+        if (place < p.top_k) out[place] = __ldg(table + page_of(sweep, j));
+      }
+      before += __popc(is_above);
+      ties_before += __popc(is_equal);
     }
   }
 }

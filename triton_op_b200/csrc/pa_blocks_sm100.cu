@@ -205,7 +205,7 @@ int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
   if (p->num_seqs == 0) return PA_OK;
   if (!p->scores || !p->block_tables || !p->context_lens || !p->tables || !p->lengths) return PA_ERR_NULL_POINTER;
   const int64_t grid = (int64_t)p->num_seqs * p->num_kv_heads;
-  if (grid > 0x7fffffff || (int64_t)p->max_blocks_per_seq > 0x7fffffff - pa::kSelectSweep) return PA_ERR_TOO_LARGE;
+  if (grid > 0x7fffffff || (int64_t)p->max_blocks_per_seq > 0x7fffffff - pa::kSelectLarge) return PA_ERR_TOO_LARGE;
   pa::BlockSelectParams k;
   memset(&k, 0, sizeof(k));
   k.scores = p->scores;
@@ -226,7 +226,11 @@ int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
   k.bt_stride_seq = p->bt_stride_seq;
   k.out_stride_seq = p->tables_stride_seq;
   k.out_stride_head = p->tables_stride_head;
-  return launch(pa::pa_block_select_kernel, dim3((unsigned)grid), pa::kSelectThreads, 0, static_cast<cudaStream_t>(stream), k);
+  const dim3 ctas((unsigned)grid);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->max_blocks_per_seq <= pa::kSelectSmall) return launch(pa::pa_block_select_kernel<128, 4>, ctas, 128, 0, st, k);
+  if (p->max_blocks_per_seq <= pa::kSelectMedium) return launch(pa::pa_block_select_kernel<256, 8>, ctas, 256, 0, st, k);
+  return launch(pa::pa_block_select_kernel<512, 16>, ctas, 512, 0, st, k);
 }
 
 }  // extern "C"

@@ -322,7 +322,9 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
         if not (kv_mode == v_mode and tuple(k_scale_t.shape) == tuple(v_scale_t.shape)):
             _fail(f"Key and value scales must have same shape, but got key: {tuple(k_scale_t.shape)}, value: {tuple(v_scale_t.shape)}")
         if kv_mode == _lib.PA_QUANT_PER_BLOCK:
-            _check_block_scales(k_scale_t, v_scale_t, key_cache, dev)
+            _check_block_scales(k_scale_t, v_scale_t, key_cache)
+            if not (k_scale_t.device == dev and v_scale_t.device == dev):
+                _fail(f"block kv scales must live on {dev}, the output's device")
         if kv_mode == _lib.PA_QUANT_PER_TOKEN:
             if not (tuple(k_scale_t.shape[:3]) == (num_blocks, num_kv_heads, kv_block_size)):
                 _fail("per-token kv scales must be [num_blocks, num_kv_heads, block_size, 1]")
@@ -415,16 +417,17 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     return p, keep, cacheable
 
 
-def _check_block_scales(k_scale, v_scale, key_cache, dev) -> None:
+def _check_block_scales(k_scale, v_scale, key_cache) -> Tuple[int, int]:
+    """Strides (page, kv head) of scales per (page, kv head)."""
     want = (key_cache.shape[0], key_cache.shape[1], 1, 1)
     if not (k_scale.shape == want and v_scale.shape == want):
         _fail(f"block kv scales must be [num_blocks, num_kv_heads, 1, 1] = {want}")
-    if not (k_scale.stride()[:2] == v_scale.stride()[:2]):
+    stride, other = k_scale.stride(), v_scale.stride()
+    if not (stride[0] == other[0] and stride[1] == other[1]):
         _fail("block kv scales must share strides")
-    if not (k_scale.device == dev and v_scale.device == dev):
-        _fail(f"block kv scales must live on {dev}, the output's device")
     if not (key_cache.dtype == FP8_DTYPE):
         _fail(f"block kv scales need a {FP8_DTYPE} cache, but got key_cache.dtype == {key_cache.dtype}")
+    return stride[0], stride[1]
 
 
 # PaDecodeParams as one packed record: filling the block field by field costs more host time than a
@@ -433,76 +436,98 @@ _PACK = struct.Struct("=2I17Q10i19q6if6i4x")
 assert _PACK.size == C.sizeof(PaDecodeParams)
 
 
+def _slabs_dense(t: torch.Tensor, stride: tuple, bs: int) -> bool:
+    """_inner_contiguous(t, 2) for a key or value cache, the common layouts first."""
+    if len(stride) == 5 and stride[4] == 1 and stride[3] == 16 and stride[2] == 16 * t.shape[3]:
+        return True
+    if len(stride) == 4 and stride[3] == 1 and stride[2] == bs:
+        return True
+    return _inner_contiguous(t, 2)
+
+
 def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
                     query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,
                     alibi_slopes, sink_tokens, status):
     """(parameter block, elements between the kv heads' tables, tensors to keep alive, workspaces) of
-    a call with scales per (page, kv head) and / or a block table per kv head."""
+    a call with scales per (page, kv head) and / or a block table per kv head.
+
+    Every call validates its arguments, so each shape and stride tuple is fetched once: the host
+    time of a small call is mostly such accesses."""
     if not isinstance(output, torch.Tensor):
         _fail("output must be a torch.Tensor")
-    dev = output.device
-    if not (output.dim() == 3 and output.dtype == torch.bfloat16):
-        _fail(f"Expected a 3D bfloat16 output tensor, but got {output.dtype} of shape {tuple(output.shape)}")
-    if query.shape != output.shape:
+    on = output.get_device()
+    q_shape = output.shape
+    if not (len(q_shape) == 3 and output.dtype == torch.bfloat16):
+        _fail(f"Expected a 3D bfloat16 output tensor, but got {output.dtype} of shape {tuple(q_shape)}")
+    if query.shape != q_shape:
         _fail("output and query must have the same shape")
-    if key_cache.dim() != 5:
-        _fail(f"Expected 5D key_cache tensor, but got shape {tuple(key_cache.shape)}")
+    num_seqs, q_heads, head_size = q_shape
+    k_shape = key_cache.shape
+    if len(k_shape) != 5:
+        _fail(f"Expected 5D key_cache tensor, but got shape {tuple(k_shape)}")
+    num_blocks, num_kv_heads, dx, bs, x = k_shape
     if not (key_cache.dtype == FP8_DTYPE and value_cache.dtype == FP8_DTYPE):
         _fail(f"block kv scales and block tables per kv head need {FP8_DTYPE} caches, but got {key_cache.dtype} and {value_cache.dtype}")
-    if not _compute_type_matches(compute_type, torch.bfloat16):
+    if compute_type is not torch.bfloat16 and not _compute_type_matches(compute_type, torch.bfloat16):
         _fail(f"compute_type {compute_type} disagrees with output.dtype {output.dtype}")
     q_dtype = _dtype_code(query.dtype, "query")
     if not (sequence_lengths.dtype == torch.int32 and block_tables.dtype == torch.int32):
         _fail("sequence_lengths and block_tables must be int32")
-    for name, t in (("query", query), ("key_cache", key_cache), ("value_cache", value_cache),
-                    ("sequence_lengths", sequence_lengths), ("block_tables", block_tables)):
-        if t.device != dev:
-            _fail(f"{name} must live on {dev}, the output's device")
+    if not (query.get_device() == on and key_cache.get_device() == on and value_cache.get_device() == on
+            and sequence_lengths.get_device() == on and block_tables.get_device() == on):
+        _fail(f"query, key_cache, value_cache, sequence_lengths and block_tables must live on {output.device}, the output's device")
     ql = int(query_sequence_length)
     if not 1 <= ql <= 4:
         _fail(f"QUERY_SEQ_LEN={ql}, only 1 to 4 are supported")
-    num_seqs, q_heads, head_size = query.shape
-    num_blocks, num_kv_heads, dx, bs, x = key_cache.shape
     if not (x == 16 and dx * x == head_size):
         _fail("key_cache must be [num_blocks, num_kv_heads, head_size/16, block_size, 16]")
     if bs not in SUPPORTED_BLOCK_SIZES:
         _fail(f"kv_block_size == {bs} not in {list(SUPPORTED_BLOCK_SIZES)}")
     if head_size != 128:
         _fail(f"head_size must be 128, but got {head_size}")
-    group = q_heads // (ql * num_kv_heads)
-    if group * ql * num_kv_heads != q_heads or group < 1:
+    group = q_heads // (ql * num_kv_heads) if num_kv_heads else 0
+    rows = group * ql
+    if group < 1 or rows * num_kv_heads != q_heads:
         _fail("query heads must be num_kv_heads * query_sequence_length * group_size")
-    if group * ql > 64:
-        _fail(f"equivalent query group size {group * ql} exceeds maximum of 64")
-    if value_cache.dim() == 4:
+    if rows > 64:
+        _fail(f"equivalent query group size {rows} exceeds maximum of 64")
+    v_shape = value_cache.shape
+    if len(v_shape) == 4:
         v_layout, want_v = _lib.PA_V_NORMAL, (num_blocks, num_kv_heads, head_size, bs)
     else:
         v_layout, want_v = _lib.PA_V_TRANSPOSED, (num_blocks, num_kv_heads, bs // 16, head_size, 16)
-    if value_cache.shape != want_v:
+    if v_shape != want_v:
         _fail(f"value_cache must be {want_v}")
-    per_head = block_tables.dim() == 3
-    if not (block_tables.dim() in (2, 3) and block_tables.shape[0] == num_seqs and sequence_lengths.numel() == num_seqs):
+    t_shape, t_stride = block_tables.shape, block_tables.stride()
+    per_head = len(t_shape) == 3
+    if not (len(t_shape) in (2, 3) and t_shape[0] == num_seqs and sequence_lengths.numel() == num_seqs):
         _fail("block_tables must be [num_seqs, max_blocks] or [num_seqs, num_kv_heads, max_blocks] and sequence_lengths [num_seqs]")
-    if per_head and block_tables.shape[1] != num_kv_heads:
-        _fail("block_tables with a table per kv head must be [num_seqs, num_kv_heads, max_blocks]")
-    if per_head and alibi_slopes is not None:
-        _fail("alibi_slopes with a block table per kv head: a place in a head's table is no distance")
-    if output.stride(2) != 1:
+    if per_head:
+        if t_shape[1] != num_kv_heads:
+            _fail("block_tables with a table per kv head must be [num_seqs, num_kv_heads, max_blocks]")
+        if alibi_slopes is not None:
+            _fail("alibi_slopes with a block table per kv head: a place in a head's table is no distance")
+    o_stride, q_stride = output.stride(), query.stride()
+    k_stride, v_stride = key_cache.stride(), value_cache.stride()
+    if o_stride[2] != 1:
         _fail("output's last dim must be contiguous")
-    if query.stride(2) != 1 or query.stride(1) != head_size:
+    if q_stride[2] != 1 or q_stride[1] != head_size:
         query = query.contiguous()
-    if not (_inner_contiguous(key_cache, 2) and _inner_contiguous(value_cache, 2)):
+        q_stride = query.stride()
+    if not (_slabs_dense(key_cache, k_stride, bs) and _slabs_dense(value_cache, v_stride, bs)):
         _fail("the per-(block, head) slabs of the KV caches must be contiguous")
-    if sequence_lengths.dim() != 1 or sequence_lengths.stride(0) != 1:
-        sequence_lengths = sequence_lengths.reshape(-1).contiguous()
-    if block_tables.stride(-1) != 1 or (per_head and num_kv_heads > 1 and block_tables.stride(1) <= 0):
+    if not sequence_lengths.is_contiguous():
+        sequence_lengths = sequence_lengths.contiguous()
+    if t_stride[-1] != 1 or (per_head and num_kv_heads > 1 and t_stride[1] <= 0):
         block_tables = block_tables.contiguous()
+        t_stride = block_tables.stride()
 
+    dev = output.device
     q_ptr = 0
     q_mode, q_scale_stride = _lib.PA_QUANT_NONE, 0
     if query_scale is not None:
         if isinstance(query_scale, (int, float)):
-            query_scale = _scalar_on_device(float(query_scale), dev)
+            query_scale = torch.full((), float(query_scale), dtype=torch.float32, device=dev)
         if not (query_scale.dtype == torch.float32 and query_scale.device == dev):
             _fail(f"query_scale must be a float32 tensor on {dev}")
         if query_scale.dim() == 0:
@@ -518,46 +543,56 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
         _fail("key_scale and value_scale go together")
     kv_mode, ks_ptr, vs_ptr, s_block, s_head = _lib.PA_QUANT_NONE, 0, 0, 0, 0
     if key_scale is not None:
+        if isinstance(key_scale, (int, float)):
+            key_scale = torch.full((), float(key_scale), dtype=torch.float32, device=dev)
+        if isinstance(value_scale, (int, float)):
+            value_scale = torch.full((), float(value_scale), dtype=torch.float32, device=dev)
         key_scale, kv_mode = _kv_scale(key_scale, value_scale, "key_scale", dev)
         value_scale, v_mode = _kv_scale(value_scale, key_scale, "value_scale", dev)
         if kv_mode != v_mode:
             _fail(f"Key and value scales must have same shape, but got key: {tuple(key_scale.shape)}, value: {tuple(value_scale.shape)}")
         if kv_mode == _lib.PA_QUANT_PER_TOKEN:
             _fail("a block table per kv head goes with no scales, per-tensor scales or block scales")
-        if kv_mode == _lib.PA_QUANT_PER_BLOCK:
-            _check_block_scales(key_scale, value_scale, key_cache, dev)
-            s_block, s_head = key_scale.stride(0), key_scale.stride(1)
-        elif not (key_scale.device == dev and value_scale.device == dev):
+        if not (key_scale.get_device() == on and value_scale.get_device() == on):
             _fail(f"key_scale and value_scale must live on {dev}, the output's device")
+        if kv_mode == _lib.PA_QUANT_PER_BLOCK:
+            s_block, s_head = _check_block_scales(key_scale, value_scale, key_cache)
         ks_ptr, vs_ptr = key_scale.data_ptr(), value_scale.data_ptr()
-    for name, t in (("alibi_slopes", alibi_slopes), ("sink_tokens", sink_tokens)):
-        if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == dev
-                                  and t.numel() == num_kv_heads * group and t.is_contiguous()):
-            _fail(f"{name} must be a contiguous fp32 tensor with one value per query head on the output's device")
-    if status is not None and not (status.dtype == torch.int32 and status.device == dev):
-        _fail(f"status must be an int32 tensor on {dev}")
+    a_ptr = s_ptr = st_ptr = 0
+    if alibi_slopes is not None or sink_tokens is not None:
+        for name, t in (("alibi_slopes", alibi_slopes), ("sink_tokens", sink_tokens)):
+            if t is not None and not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == dev
+                                      and t.numel() == num_kv_heads * group and t.is_contiguous()):
+                _fail(f"{name} must be a contiguous fp32 tensor with one value per query head on the output's device")
+        a_ptr = 0 if alibi_slopes is None else alibi_slopes.data_ptr()
+        s_ptr = 0 if sink_tokens is None else sink_tokens.data_ptr()
+    if status is not None:
+        if not (status.dtype == torch.int32 and status.device == dev):
+            _fail(f"status must be an int32 tensor on {dev}")
+        st_ptr = status.data_ptr()
 
-    rows = group * ql
     parts = max(1, -(-int(max_sequence_length) // SEQUENCE_PARTITION_SIZE))
-    sums = torch.empty((2, num_seqs, num_kv_heads, parts, rows), dtype=torch.float32, device=dev)
-    exp_sums, max_logits = sums[0], sums[1]
-    tmp = torch.empty((num_seqs, num_kv_heads, parts, rows, head_size), dtype=torch.bfloat16, device=dev)
-    w_head, w_part = parts * rows, rows
-    ptr = lambda t: 0 if t is None else t.data_ptr()
+    ws_shape, w_head = (num_seqs, num_kv_heads, parts, rows), parts * rows
+    ws_stride = (num_kv_heads * w_head, w_head, rows, 1)
+    # (given its strides, an allocation costs less than half the host time)
+    exp_sums = torch.empty_strided(ws_shape, ws_stride, dtype=torch.float32, device=dev)
+    max_logits = torch.empty_strided(ws_shape, ws_stride, dtype=torch.float32, device=dev)
+    tmp = torch.empty_strided(ws_shape + (head_size,), (num_kv_heads * w_head * head_size, w_head * head_size,
+                                                        rows * head_size, head_size, 1), dtype=torch.bfloat16, device=dev)
     p = PaDecodeParams.from_buffer_copy(_PACK.pack(
         _PACK.size, _lib.PA_ABI_VERSION,
         output.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-        sequence_lengths.data_ptr(), q_ptr, ks_ptr, vs_ptr, ptr(alibi_slopes), ptr(sink_tokens),
-        exp_sums.data_ptr(), max_logits.data_ptr(), tmp.data_ptr(), ptr(status), 0, 0,
-        num_seqs, num_kv_heads, group, ql, head_size, bs, num_blocks, block_tables.shape[-1], SEQUENCE_PARTITION_SIZE, parts,
-        output.stride(0), output.stride(1), query.stride(0), query.stride(1), key_cache.stride(0), key_cache.stride(1),
-        value_cache.stride(0), value_cache.stride(1), block_tables.stride(0), q_scale_stride, s_block, s_head,
-        num_kv_heads * w_head, w_head, w_part, num_kv_heads * w_head * head_size, w_head * head_size,
-        w_part * head_size, head_size,
+        sequence_lengths.data_ptr(), q_ptr, ks_ptr, vs_ptr, a_ptr, s_ptr,
+        exp_sums.data_ptr(), max_logits.data_ptr(), tmp.data_ptr(), st_ptr, 0, 0,
+        num_seqs, num_kv_heads, group, ql, head_size, bs, num_blocks, t_shape[-1], SEQUENCE_PARTITION_SIZE, parts,
+        o_stride[0], o_stride[1], q_stride[0], q_stride[1], k_stride[0], k_stride[1],
+        v_stride[0], v_stride[1], t_stride[0], q_scale_stride, s_block, s_head,
+        num_kv_heads * w_head, w_head, rows, num_kv_heads * w_head * head_size, w_head * head_size,
+        rows * head_size, head_size,
         q_dtype, _lib.PA_DT_E4M3FN, _lib.PA_DT_BF16, q_mode, kv_mode, v_layout, float(softmax_scale),
         0, 0, 0, 0, 0, 0))
     keep = (query, sequence_lengths, block_tables, query_scale, key_scale, value_scale)
-    head_stride = block_tables.stride(1) if per_head and num_kv_heads > 1 else 0
+    head_stride = t_stride[1] if per_head and num_kv_heads > 1 else 0
     return p, head_stride, keep, (exp_sums, max_logits, tmp)
 
 
@@ -645,7 +680,7 @@ def paged_attention_decode(
                 alibi_slopes, sink_tokens, status)
             if not output.is_cuda:
                 raise RuntimeError("paged_attention_decode runs on CUDA tensors only; there is no CPU fallback")
-            _lib.launch(output.device, _lib.lib().pa_decode_tables_sm100, "pa_decode_tables_sm100", C.byref(p), head_stride)
+            _lib.launch(output.get_device(), _lib.lib().pa_decode_tables_sm100, "pa_decode_tables_sm100", C.byref(p), head_stride)
             return {"triton_decode_time": 0.0, "triton_reduce_time": 0.0, "temporary_output": ws[2],
                     "final_output": output, "exponential_sums": ws[0], "maximum_logits": ws[1],
                     "total_triton_time": 0.0, "partition_size": SEQUENCE_PARTITION_SIZE}

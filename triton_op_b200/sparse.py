@@ -23,8 +23,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import _lib
-from .pa_decode import (FP8_DTYPE, SUPPORTED_BLOCK_SIZES, PaArgumentError, _dtype_code, _kv_scale, _scalar_on_device,
-                        paged_attention_decode)
+from .pa_decode import (FP8_DTYPE, SUPPORTED_BLOCK_SIZES, PaArgumentError, _dtype_code, _kv_scale, paged_attention_decode)
 
 __all__ = ["score_blocks", "select_blocks", "sparse_attention_decode"]
 
@@ -105,7 +104,7 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
     q_mode, q_ptr, q_stride = _lib.PA_QUANT_NONE, 0, 0
     if query_scale is not None:
         if isinstance(query_scale, (int, float)):
-            query_scale = _scalar_on_device(float(query_scale), dev)
+            query_scale = torch.full((), float(query_scale), dtype=torch.float32, device=dev)
         if not (query_scale.dtype == torch.float32 and query_scale.device == dev):
             _fail(f"query_scale must be a float32 tensor on {dev}")
         if query_scale.dim() == 0:
@@ -119,6 +118,8 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
         q_ptr = query_scale.data_ptr()
     kv_mode, ks_ptr, s_block, s_head = _lib.PA_QUANT_NONE, 0, 0, 0
     if key_scale is not None:
+        if isinstance(key_scale, (int, float)):
+            key_scale = torch.full((), float(key_scale), dtype=torch.float32, device=dev)
         key_scale, kv_mode = _kv_scale(key_scale, None, "key_scale", dev)
         if key_scale.device != dev:
             _fail(f"key_scale must live on {dev}")
@@ -131,7 +132,7 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
         ks_ptr = key_scale.data_ptr()
     width = block_tables.shape[1]
     if scores is None:
-        scores = torch.empty((num_seqs, num_kv_heads, width), dtype=torch.float32, device=dev)
+        scores = torch.empty_strided((num_seqs, num_kv_heads, width), (num_kv_heads * width, width, 1), dtype=torch.float32, device=dev)
     elif not (scores.dtype == torch.float32 and scores.device == dev and scores.shape == (num_seqs, num_kv_heads, width)
               and scores.stride(2) == 1):
         _fail(f"scores must be fp32 {(num_seqs, num_kv_heads, width)} on {dev}, its last dim contiguous")
@@ -145,7 +146,7 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
         num_seqs, num_kv_heads, rows, head_size, block_size, num_blocks, width, q_dtype, q_mode, kv_mode,
         query.stride(0), key_bounds.stride(0), key_bounds.stride(1), block_tables.stride(0), q_stride, s_block, s_head,
         scores.stride(0), scores.stride(1), float(softmax_scale), 0))
-    _lib.launch(dev, _lib.lib().pa_block_scores_sm100, "pa_block_scores_sm100", C.byref(p))
+    _lib.launch(query.get_device(), _lib.lib().pa_block_scores_sm100, "pa_block_scores_sm100", C.byref(p))
     return scores
 
 
@@ -177,12 +178,12 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     if scores.stride(2) != 1:
         scores = scores.contiguous()
     if tables is None:
-        tables = torch.empty((num_seqs, num_kv_heads, top_k), dtype=torch.int32, device=dev)
+        tables = torch.empty_strided((num_seqs, num_kv_heads, top_k), (num_kv_heads * top_k, top_k, 1), dtype=torch.int32, device=dev)
     elif not (tables.dtype == torch.int32 and tables.device == dev and tables.shape == (num_seqs, num_kv_heads, top_k)
               and tables.stride(2) == 1):
         _fail(f"tables must be int32 {(num_seqs, num_kv_heads, top_k)} on {dev}, its last dim contiguous")
     if lengths is None:
-        lengths = torch.empty((num_seqs,), dtype=torch.int32, device=dev)
+        lengths = torch.empty_strided((num_seqs,), (1,), dtype=torch.int32, device=dev)
     elif not (lengths.dtype == torch.int32 and lengths.device == dev and lengths.shape == (num_seqs,) and lengths.is_contiguous()):
         _fail(f"lengths must be a contiguous int32 tensor of {num_seqs} on {dev}")
     status_ptr = _status_ptr(status, dev)
@@ -193,7 +194,7 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
         scores.data_ptr(), block_tables.data_ptr(), sequence_lengths.data_ptr(), tables.data_ptr(), lengths.data_ptr(), status_ptr,
         num_seqs, num_kv_heads, block_size, width, int(top_k), int(keep_first), int(keep_last), 0,
         scores.stride(0), scores.stride(1), block_tables.stride(0), tables.stride(0), tables.stride(1)))
-    _lib.launch(dev, _lib.lib().pa_block_select_sm100, "pa_block_select_sm100", C.byref(p))
+    _lib.launch(scores.get_device(), _lib.lib().pa_block_select_sm100, "pa_block_select_sm100", C.byref(p))
     return tables, lengths
 
 
