@@ -27,7 +27,7 @@ namespace pa {
 
 // Threads and pages per thread by the width of the table: a CTA holds THREADS * ITEMS pages at a time and
 // sweeps over more than that.
-constexpr int kSelectSmall = 128 * 4, kSelectMedium = 256 * 8, kSelectLarge = 512 * 16;
+constexpr int kSelectSmall = 128 * 4, kSelectMedium = 256 * 8, kSelectLarge = 256 * 32;
 
 struct BlockSelectParams {
   const float* scores;         // [S, Hkv, >= pages]
@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 }
 
 template <int THREADS, int ITEMS>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1)
+__global__ void __launch_bounds__(THREADS, ITEMS > 8 ? 4 : 1)
 pa_block_select_kernel(const __grid_constant__ BlockSelectParams p) {
   constexpr int kWarps = THREADS / 32, kSweep = THREADS * ITEMS, kPer = 4, kBins = kPer * THREADS;
   __shared__ __align__(16) int bins[kBins];

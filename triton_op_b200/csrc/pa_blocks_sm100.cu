@@ -230,7 +230,7 @@ int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p->max_blocks_per_seq <= pa::kSelectSmall) return launch(pa::pa_block_select_kernel<128, 4>, ctas, 128, 0, st, k);
   if (p->max_blocks_per_seq <= pa::kSelectMedium) return launch(pa::pa_block_select_kernel<256, 8>, ctas, 256, 0, st, k);
-  return launch(pa::pa_block_select_kernel<512, 16>, ctas, 512, 0, st, k);
+  return launch(pa::pa_block_select_kernel<256, 32>, ctas, 256, 0, st, k);
 }
 
 }  // extern "C"
