@@ -10,26 +10,40 @@
 // cores: pages are the 16 rows of a tile, query rows its columns.
 //
 // What bounds it: 256 bytes of bounds per (page, kv head), read once, against 2 * 256 * rows
-// operations: HBM for the query groups of a decode step.  The bounds go straight from global memory
-// to registers (16 bytes per thread and load, 128 bytes per thread in flight): the tile's k order is
-// free, so each thread takes 16 consecutive bytes of a page and the query is laid out to match;
-// nothing is staged.  e4m3 becomes f16 with shifts and masks -- the exponent field moves by one
-// place, value * 2^-8, exact and subnormals included -- because the convert instructions run at a
-// fraction of the ALUs' rate.  The query is multiplied by a power of two per row so that its
-// largest element is near 2^15: f16 then holds every bf16 element exactly that is not 2^-22 below
-// the row's largest.
+// operations: HBM for the query groups of a decode step.  One CTA per SM takes an equal share of all
+// tiles (16 pages of up to eight kv heads) of the batch, whatever the sequences' lengths; a
+// pair of producer warps runs through them with bulk copies -- a page's heads are one run of up to 2 KB -- into
+// a ring of about 170 KB, and eight warps multiply, one kv head (or every so many tiles) each.
+// (With a CTA per (sequence, 128 pages) the chain length -> page ids -> query -> bounds was paid by four or
+// five waves of CTAs: 54 us for 32 sequences of 16 K to 64 K tokens whose bounds take 27; with 16-byte
+// copies by the multiplying warps themselves their load units were the limit: 47-50 us.)
+// The tile's k order is free, so each thread takes 16 consecutive bytes of a page and the query is laid
+// out to match.  e4m3 becomes f16 with shifts and masks -- the exponent field moves by one place,
+// value * 2^-8, exact and subnormals included -- for one half of a page's bounds and with convert
+// instructions, whose pipe is slower but otherwise idle, for the other.  The query is multiplied by a
+// power of two per row so that its largest element is near 2^15: f16 then holds every bf16
+// element exactly that is not 2^-22 below the row's largest.
 #pragma once
 
 #include "../../include/pa_decode_sm100.h"
 #include "pa_common.cuh"
 #include "pa_params.cuh"
+#include "pa_tcgen05.cuh"
 
 namespace pa {
 
 constexpr int kScoreWarps = 8;
 constexpr int kScoreTilePages = 16;
+constexpr int kScoreProducers = 2;   // warps that request tiles: one warp's bulk copies go out 75-90 cycles apart
+constexpr int kScoreThreads = (kScoreWarps + kScoreProducers) * 32;
+constexpr int kScoreMaxSlots = 40;
+constexpr int kScoreRingBytes = 176 * 1024;
 constexpr int kScoreRowBytes = kD * 2 + 16;    // one query row as f16; the padding spreads the rows over the banks
-constexpr int kScoreMaxRows = 128;             // query rows (padded to 8 per kv head) that a CTA holds
+constexpr int kScoreMaxRows = 64;              // query rows (padded to 8 per kv head) that a CTA holds
+// A tile in the ring: [16 pages][heads][256 bytes], 64 bytes between pages so that neighbouring pages of
+// one head lie in different banks, then its key scales [16 pages][heads].
+__host__ __device__ constexpr int score_page_pitch(int heads) { return heads * 2 * kD + 64; }
+__host__ __device__ constexpr int score_slot_bytes(int heads) { return kScoreTilePages * (score_page_pitch(heads) + heads * 4); }
 
 struct BlockScoreParams {
   const uint8_t* q;            // [S, Hkv * rows, 128] bf16 or e4m3
@@ -42,7 +56,9 @@ struct BlockScoreParams {
   int32_t* status;
   int32_t S, Hkv, rows, block_size, num_blocks, width;
   int32_t q_is_fp8, q_quant_mode;
-  int32_t heads_per_cta, tiles_per_cta;
+  int32_t heads_per_cta;       // a power of two that divides kScoreWarps
+  int32_t slots;               // ring depth in tiles, more than kScoreWarps / heads_per_cta
+  int32_t off_index, off_ring; // shared-memory carve: query rows and factors, index of the sequences, ring
   int64_t q_stride_seq;        // bytes
   int64_t bounds_stride_block, bounds_stride_head;   // bytes
   int64_t bt_stride_seq;
@@ -58,6 +74,10 @@ __device__ __forceinline__ uint32_t e4m3_odd_to_f16(uint32_t w) {
 }
 __device__ __forceinline__ uint32_t e4m3_even_to_f16(uint32_t w) {
   return e4m3_odd_to_f16(w << 8);
+}
+// The same by the convert instruction, whose halves are bytes 0, 1 and bytes 2, 3 (true values).
+__device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ uint32_t f16x2_max0(uint32_t v) {
   uint32_t r;
@@ -81,179 +101,344 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ldg_stream128(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
 // NB8: blocks of eight query rows per kv head.
 template <int NB8>
-__global__ void __launch_bounds__(kScoreWarps * 32)
+__global__ void __launch_bounds__(kScoreThreads, 1)
 pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* factor = reinterpret_cast<float*>(smem + (size_t)p.heads_per_cta * NB8 * 8 * kScoreRowBytes);   // [heads][NB8 * 8]
+  constexpr int kRows = NB8 * 8;
+  constexpr bool kKeep = NB8 == 1;   // the query operand of a warp's head stays in registers (32 of them)
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* factor = reinterpret_cast<float*>(smem + p.heads_per_cta * kRows * kScoreRowBytes);   // [heads][kRows]
+  int* tile_off = reinterpret_cast<int*>(smem + p.off_index);   // [S + 1] tiles before each sequence
+  int* seq_pages = tile_off + p.S + 1;                          // [S]
+  __shared__ int scan[32];
+  __shared__ __align__(8) uint64_t bar_full[kScoreMaxSlots], bar_empty[kScoreMaxSlots];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int groups = (p.Hkv + p.heads_per_cta - 1) / p.heads_per_cta;
-  const int seq = (int)blockIdx.x / groups, head0 = ((int)blockIdx.x - seq * groups) * p.heads_per_cta;
-  const int heads = min(p.heads_per_cta, p.Hkv - head0);
+  const int hpc = p.heads_per_cta;
+  const uint32_t ring = smem_addr(smem) + p.off_ring;
+  const int slot_bytes = score_slot_bytes(hpc), pitch = score_page_pitch(hpc);
+  if (tid < p.slots) {
+    mbar_init(smem_addr(&bar_full[tid]), 33);     // the producer's arrival, and its lanes' key scale copies
+    mbar_init(smem_addr(&bar_empty[tid]), hpc);   // the warps that multiply the tile
+  }
+  if (tid == 0) {
+    mbar_fence_init();
+    fence_proxy_async();
+  }
   grid_dependency_wait();
   grid_launch_dependents();   // (the dependent waits for this grid's end before it reads the scores)
-  const int ctx = p.context_lens[seq];
+
+  // ---- pages of every sequence, and tiles of 16 pages summed over the sequences (every CTA for itself)
   const int64_t cap = (int64_t)p.width * p.block_size;
-  if (ctx > cap && p.status && tid == 0) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
-  const int pages = ctx <= 0 ? 0 : (int)min((int64_t)p.width, ((int64_t)ctx + p.block_size - 1) / p.block_size);
-  const int page0 = (int)blockIdx.y * p.tiles_per_cta * kScoreTilePages;
-  const int page1 = min(p.width, page0 + p.tiles_per_cta * kScoreTilePages);
-  // pages without tokens: nothing to choose
-  for (int h = 0; h < heads; ++h) {
-    float* out = p.scores + (int64_t)seq * p.out_stride_seq + (int64_t)(head0 + h) * p.out_stride_head;
-    for (int i = max(page0, pages) + tid; i < page1; i += kScoreWarps * 32) out[i] = -INFINITY;
+  {
+    const int chunk = (p.S + kScoreThreads - 1) / kScoreThreads;
+    const int beg = min(tid * chunk, p.S), end = min(beg + chunk, p.S);
+    int sum = 0;
+    for (int s = beg; s < end; ++s) {
+      const int ctx = p.context_lens[s];
+      if (ctx > cap && blockIdx.x == 0 && p.status) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
+      const int pages = ctx <= 0 ? 0 : (int)min((int64_t)p.width, ((int64_t)ctx + p.block_size - 1) / p.block_size);
+      seq_pages[s] = pages;
+      tile_off[s + 1] = (pages + kScoreTilePages - 1) / kScoreTilePages;
+      sum += tile_off[s + 1];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFullMask, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    if (tid == 0) tile_off[0] = 0;
+    __syncthreads();
+    int run = incl - sum;
+    for (int w = 0; w < warp; ++w) run += scan[w];
+    for (int s = beg; s < end; ++s) {
+      run += tile_off[s + 1];
+      tile_off[s + 1] = run;
+    }
+    __syncthreads();
   }
-  if (page0 >= pages) return;
+  const int total = tile_off[p.S];
 
-  // ---- the CTA's query rows: a quad of lanes per row, lane t the 32 dims of its quarter.  Padding rows
-  // repeat row 0, which changes no maximum.  Within each group of four dims the order is 0, 2, 1, 3
-  // (what the e4m3 unpacking below yields).
-  constexpr int kRows = NB8 * 8;
-  for (int r0 = warp * 8; r0 < heads * kRows; r0 += kScoreWarps * 8) {
-    const int r = r0 + g, h = r / kRows;
-    int row = r - h * kRows;
-    if (row >= p.rows) row = 0;
-    const int64_t grow = (int64_t)(head0 + h) * p.rows + row;
-    float x[32];
-    if (p.q_is_fp8) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * kD + t * 32);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint4 v = __ldg(src + e);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t ev = e4m3_even_to_f16(w[k]), od = e4m3_odd_to_f16(w[k]);
-          float f0, f1, f2, f3;   // times 2^-8, taken back by the factor below
-          asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(f0), "=f"(f2) : "r"(ev));
-          asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(f1), "=f"(f3) : "r"(od));
-          x[e * 16 + k * 4] = f0 * 256.f, x[e * 16 + k * 4 + 1] = f1 * 256.f;
-          x[e * 16 + k * 4 + 2] = f2 * 256.f, x[e * 16 + k * 4 + 3] = f3 * 256.f;
-        }
-      }
-    } else {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * (kD * 2) + t * 64);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint4 v = __ldg(src + e);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[e * 8 + k * 2] = bf16_lo_to_f32(w[k]), x[e * 8 + k * 2 + 1] = bf16_hi_to_f32(w[k]);
-      }
+  // ---- this CTA's share of the (head group, tile) units, the group slowest
+  const int groups = (p.Hkv + hpc - 1) / hpc;
+  const int64_t units = (int64_t)total * groups;
+  const int64_t u_beg = units * blockIdx.x / gridDim.x, u_end = units * (blockIdx.x + 1) / gridDim.x;
+  const int n_tiles = (int)(u_end - u_beg);
+  struct Place { int group, seq, tile; } at0{0, 0, 0};
+  if (n_tiles > 0) {
+    at0.group = (int)(u_beg / total);
+    const int at = (int)(u_beg - (int64_t)at0.group * total);
+    int lo = 0, hi = p.S;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tile_off[mid] <= at) lo = mid; else hi = mid;
     }
-    float amax = 0.f;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    amax = quad_max(amax);
-    // power of two that brings the row's largest element into [2^14, 2^15)
-    const int be = (int)((__float_as_uint(amax) >> 23) & 0xff);
-    float pre = 1.0f, back = 1.0f;
-    if (be > 0 && be < 255) {
-      pre = __uint_as_float((uint32_t)min(253, 254 + 14 - be) << 23);
-      back = 1.0f / pre;   // a power of two
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint4 v;
-      v.x = pack_f16x2(x[e * 8] * pre, x[e * 8 + 2] * pre);
-      v.y = pack_f16x2(x[e * 8 + 1] * pre, x[e * 8 + 3] * pre);
-      v.z = pack_f16x2(x[e * 8 + 4] * pre, x[e * 8 + 6] * pre);
-      v.w = pack_f16x2(x[e * 8 + 5] * pre, x[e * 8 + 7] * pre);
-      *reinterpret_cast<uint4*>(smem + (size_t)r * kScoreRowBytes + t * 64 + e * 16) = v;
-    }
-    if (t == 0) {
-      float qs = 1.0f;
-      if (p.q_quant_mode == PA_QUANT_PER_TENSOR) qs = __ldg(p.q_scale);
-      if (p.q_quant_mode == PA_QUANT_PER_TOKEN) qs = __ldg(p.q_scale + (int64_t)seq * p.q_scale_stride_seq + grow);
-      factor[r] = back * 256.0f * qs * p.softmax_scale;   // 2^8: the bounds' f16 values are the codes times 2^-8
-    }
+    at0.seq = lo;
+    at0.tile = at - tile_off[lo];
   }
-  __syncthreads();
+  auto next_seq = [&](Place& a) {   // the next sequence that has tiles (past the last unit nobody looks)
+    a.tile = 0;
+    do {
+      if (++a.seq == p.S) a.seq = 0, ++a.group;
+    } while (tile_off[a.seq + 1] == tile_off[a.seq] && a.group < groups);
+  };
 
-  // ---- tiles of 16 pages of one kv head, dealt to the warps with the head fastest (neighbouring
-  // warps read neighbouring heads of the same pages)
-  const int tiles = (min(pages, page1) - page0 + kScoreTilePages - 1) / kScoreTilePages;
-  const int32_t* table = p.block_tables + (int64_t)seq * p.bt_stride_seq;
-  for (int task = warp; task < tiles * heads; task += kScoreWarps) {
-    const int tile = task / heads, h = task - tile * heads;
-    const int pg[2] = {page0 + tile * kScoreTilePages + g, page0 + tile * kScoreTilePages + g + 8};
-    int id[2];
-    uint4 raw[2][2][2];   // [row half][min, max][16-byte chunk]
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      id[i] = pg[i] < pages ? __ldg(table + pg[i]) : 0;
-      if ((unsigned)id[i] >= (unsigned)p.num_blocks) {
-        id[i] = 0;
+  if (warp >= kScoreWarps) {
+    // ------------------------------------------------------------------ producers, a tile in turn: lane = page of the tile
+    const int first = warp - kScoreWarps;
+    Place a = at0;
+    auto skip = [&](int n) {
+      for (; n > 0; --n)
+        if (++a.tile >= tile_off[a.seq + 1] - tile_off[a.seq]) next_seq(a);
+    };
+    if (n_tiles > 0) skip(first);
+    const uint64_t pol = l2_policy_evict_first();
+    const bool whole = p.bounds_stride_head == 2 * kD;   // a page's heads are one run
+    // the page ids of two tiles ahead are on their way while a tile is requested
+    auto fetch = [&](int k, int& group, int& valid, int& id) {
+      valid = 0;
+      id = 0;
+      group = a.group;
+      if (k < n_tiles) {
+        valid = min(kScoreTilePages, seq_pages[a.seq] - a.tile * kScoreTilePages);
+        if (lane < valid) id = __ldg(p.block_tables + (int64_t)a.seq * p.bt_stride_seq + a.tile * kScoreTilePages + lane);
+        skip(kScoreProducers);
+      }
+    };
+    int g0, v0, id0, g1, v1, id1;
+    fetch(first, g0, v0, id0);
+    fetch(first + kScoreProducers, g1, v1, id1);
+    int slot = first;
+    uint32_t phase = 1;
+    for (int k = first; k < n_tiles; k += kScoreProducers) {
+      const int group = g0, valid = v0;
+      int id = id0;
+      g0 = g1, v0 = v1, id0 = id1;
+      fetch(k + 2 * kScoreProducers, g1, v1, id1);
+      const uint32_t full = smem_addr(&bar_full[slot]);
+      if (!__all_sync(kFullMask, mbar_wait(smem_addr(&bar_empty[slot]), phase))) {
+        if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_WAIT_TIMEOUT);
+        break;
+      }
+      if ((unsigned)id >= (unsigned)p.num_blocks) {
+        id = 0;
         if (p.status) atomicOr(p.status, PA_DEV_BAD_PAGE_ID);
       }
+      const int head0 = group * hpc, heads = min(hpc, p.Hkv - head0);
+      const uint32_t at = ring + slot * slot_bytes;
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(valid * heads * 2 * kD));
+      __syncwarp();
+      if (lane < valid) {
+        const uint8_t* src = p.bounds + (int64_t)id * p.bounds_stride_block + (int64_t)head0 * p.bounds_stride_head;
+        if (whole) {
+          bulk_g2s(at + lane * pitch, src, (uint32_t)(heads * 2 * kD), full, pol);
+        } else {
+          for (int h = 0; h < heads; ++h) bulk_g2s(at + lane * pitch + h * 2 * kD, src + (int64_t)h * p.bounds_stride_head, 2 * kD, full, pol);
+        }
+        if (p.k_scale) {
+          const float* ks = p.k_scale + (int64_t)id * p.ks_stride_block + (int64_t)head0 * p.ks_stride_head;
+          for (int h = 0; h < heads; ++h) cp_async4(at + kScoreTilePages * pitch + (lane * hpc + h) * 4, ks + (int64_t)h * p.ks_stride_head);
+        }
+      }
+      cp_async_arrive(full);
+      slot += kScoreProducers;
+      if (slot >= p.slots) slot -= p.slots, phase ^= 1;
     }
+    return;
+  }
+
+  // -------------------------------------------------------------------- the multiplying warps
+  // ---- pages without tokens: nothing to choose (a (sequence, kv head) after the other over the CTAs)
+  for (int64_t r = blockIdx.x; r < (int64_t)p.S * p.Hkv; r += gridDim.x) {
+    const int s = (int)(r / p.Hkv), h = (int)(r - (int64_t)s * p.Hkv);
+    float* out = p.scores + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
+    for (int i = seq_pages[s] + tid; i < p.width; i += kScoreWarps * 32) out[i] = -INFINITY;
+  }
+  // A warp works for one kv head of the group and takes the tiles k with k % step == sub.
+  const int g = lane >> 2, t = lane & 3;
+  const int my_head = warp & (hpc - 1), sub = warp / hpc, step = kScoreWarps / hpc;
+  Place a = at0;
+  int k = 0;                          // tiles of the CTA before the segment
+  int mine = sub, slot = sub;         // this warp's next tile and its slot
+  uint32_t phase = 0;
+  while (k < n_tiles) {
+    // a segment: tiles of one sequence and head group
+    const int seq = a.seq, tile_a = a.tile;
+    const int count = min(tile_off[seq + 1] - tile_off[seq] - tile_a, n_tiles - k);
+    const int head0 = a.group * hpc, heads = min(hpc, p.Hkv - head0);
+    const int pages = seq_pages[seq];
+
+    // ---- the group's query rows: a quad of lanes per row, lane t the 32 dims of its quarter.  Padding rows
+    // repeat row 0, which changes no maximum.  Within each group of four dims the order is 0, 2, 1, 3
+    // (what the e4m3 unpacking below yields).
+    if (k > 0) tc::named_barrier_sync(1, kScoreWarps * 32);   // the rows of the segment before are no longer read
+    for (int r0 = warp * 8; r0 < heads * kRows; r0 += kScoreWarps * 8) {
+      const int r = r0 + g, h = r / kRows;
+      int row = r - h * kRows;
+      if (row >= p.rows) row = 0;
+      const int64_t grow = (int64_t)(head0 + h) * p.rows + row;
+      float x[32];
+      if (p.q_is_fp8) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * kD + t * 32);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t* src = p.bounds + (int64_t)id[i] * p.bounds_stride_block + (int64_t)(head0 + h) * p.bounds_stride_head + t * 16;
+        for (int e = 0; e < 2; ++e) {
+          const uint4 v = __ldg(src + e);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t lo, hi;
+            e4m3_to_f16(w[j], lo, hi);
+            asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}"
+                : "=f"(x[e * 16 + j * 4]), "=f"(x[e * 16 + j * 4 + 1]) : "r"(lo));
+            asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}"
+                : "=f"(x[e * 16 + j * 4 + 2]), "=f"(x[e * 16 + j * 4 + 3]) : "r"(hi));
+          }
+        }
+      } else {
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * (kD * 2) + t * 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint4 v = __ldg(src + e);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[e * 8 + j * 2] = bf16_lo_to_f32(w[j]), x[e * 8 + j * 2 + 1] = bf16_hi_to_f32(w[j]);
+        }
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
+      amax = quad_max(amax);
+      // power of two that brings the row's largest element into [2^14, 2^15)
+      const int be = (int)((__float_as_uint(amax) >> 23) & 0xff);
+      float pre = 1.0f, back = 1.0f;
+      if (be > 0 && be < 255) {
+        pre = __uint_as_float((uint32_t)min(253, 254 + 14 - be) << 23);
+        back = 1.0f / pre;   // a power of two
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint4 v;
+        v.x = pack_f16x2(x[e * 8] * pre, x[e * 8 + 2] * pre);
+        v.y = pack_f16x2(x[e * 8 + 1] * pre, x[e * 8 + 3] * pre);
+        v.z = pack_f16x2(x[e * 8 + 4] * pre, x[e * 8 + 6] * pre);
+        v.w = pack_f16x2(x[e * 8 + 5] * pre, x[e * 8 + 7] * pre);
+        *reinterpret_cast<uint4*>(smem + r * kScoreRowBytes + t * 64 + e * 16) = v;
+      }
+      if (t == 0) {
+        float qs = 1.0f;
+        if (p.q_quant_mode == PA_QUANT_PER_TENSOR) qs = __ldg(p.q_scale);
+        if (p.q_quant_mode == PA_QUANT_PER_TOKEN) qs = __ldg(p.q_scale + (int64_t)seq * p.q_scale_stride_seq + grow);
+        factor[r] = back * 256.0f * qs * p.softmax_scale;   // 2^8: the bounds' f16 values are the codes times 2^-8
+      }
+    }
+    tc::named_barrier_sync(1, kScoreWarps * 32);
+
+    // operand fragment of (row block n, smallest / largest m, chunk c): this thread's 16 dims, four k-steps
+    // of (b0, b1); against the smallest codes the negative part of the query, against the largest the positive
+    const uint8_t* qrow = smem + (my_head * kRows + g) * kScoreRowBytes + t * 32;
+    auto load_q = [&](int n, int m, int c, uint4 (&v)[2]) {
+      const uint4* src = reinterpret_cast<const uint4*>(qrow + n * 8 * kScoreRowBytes + c * 128);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 q = src[e];
+        v[e] = m ? make_uint4(f16x2_max0(q.x), f16x2_max0(q.y), f16x2_max0(q.z), f16x2_max0(q.w))
+                 : make_uint4(f16x2_min0(q.x), f16x2_min0(q.y), f16x2_min0(q.z), f16x2_min0(q.w));
+      }
+    };
+    uint4 held[2][2][2];
+    if (kKeep) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) raw[i][m][c] = ldg_stream128(src + m * kD + c * 64);
-      }
-    }
-    float acc[NB8][4];
+        for (int c = 0; c < 2; ++c) {
+          load_q(0, m, c, held[m][c]);
+          if (m == 0) {   // dims 0, 1 and 2, 3, as the convert instruction yields them
 #pragma unroll
-    for (int n = 0; n < NB8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    const uint8_t* qrow = smem + (size_t)(h * kRows + g) * kScoreRowBytes + t * 32;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint4 qv[NB8][2];   // this thread's 16 dims of the chunk: four k-steps of (b0, b1)
-#pragma unroll
-      for (int n = 0; n < NB8; ++n) {
-        qv[n][0] = *reinterpret_cast<const uint4*>(qrow + n * 8 * kScoreRowBytes + c * 128);
-        qv[n][1] = *reinterpret_cast<const uint4*>(qrow + n * 8 * kScoreRowBytes + c * 128 + 16);
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const uint32_t w0[4] = {raw[0][m][c].x, raw[0][m][c].y, raw[0][m][c].z, raw[0][m][c].w};
-        const uint32_t w1[4] = {raw[1][m][c].x, raw[1][m][c].y, raw[1][m][c].z, raw[1][m][c].w};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t a0 = e4m3_even_to_f16(w0[u]), a1 = e4m3_even_to_f16(w1[u]);
-          const uint32_t a2 = e4m3_odd_to_f16(w0[u]), a3 = e4m3_odd_to_f16(w1[u]);
-#pragma unroll
-          for (int n = 0; n < NB8; ++n) {
-            const uint4 v = qv[n][u >> 1];
-            const uint32_t b0 = (u & 1) ? v.z : v.x, b1 = (u & 1) ? v.w : v.y;
-            // against the largest code the positive part of the query, against the smallest the negative
-            mma_f16(acc[n], a0, a1, a2, a3, m ? f16x2_max0(b0) : f16x2_min0(b0), m ? f16x2_max0(b1) : f16x2_min0(b1));
+            for (int e = 0; e < 2; ++e) {
+              const uint4 v = held[0][c][e];
+              held[0][c][e] = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632),
+                                         __byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+            }
           }
         }
       }
     }
-    float best[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < NB8; ++n) {
-      const float2 f = *reinterpret_cast<const float2*>(factor + h * kRows + n * 8 + 2 * t);
-      best[0] = fmaxf(best[0], fmaxf(acc[n][0] * f.x, acc[n][1] * f.y));
-      best[1] = fmaxf(best[1], fmaxf(acc[n][2] * f.x, acc[n][3] * f.y));
-    }
-    best[0] = quad_max(best[0]);
-    best[1] = quad_max(best[1]);
-    if (t < 2) {
-      const int i = t;
-      const int page = i ? pg[1] : pg[0];
-      if (page < pages) {
-        float ks = 1.0f;
-        if (p.k_scale) ks = __ldg(p.k_scale + (int64_t)(i ? id[1] : id[0]) * p.ks_stride_block + (int64_t)(head0 + h) * p.ks_stride_head);
-        p.scores[(int64_t)seq * p.out_stride_seq + (int64_t)(head0 + h) * p.out_stride_head + page] = (i ? best[1] : best[0]) * ks;
+    float* out = p.scores + (int64_t)seq * p.out_stride_seq + (int64_t)(head0 + my_head) * p.out_stride_head;
+#pragma unroll 1
+    while (mine < k + count) {
+      if (!__all_sync(kFullMask, mbar_wait(smem_addr(&bar_full[slot]), phase))) {
+        if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_WAIT_TIMEOUT);
+        return;
       }
+      if (my_head < heads) {
+        const uint32_t tile = ring + slot * slot_bytes;
+        const uint32_t row0 = tile + g * pitch + my_head * 2 * kD + t * 16, row1 = row0 + 8 * pitch;
+        float acc[2][NB8][4];   // the two halves of the bound: two chains of products
+#pragma unroll
+        for (int n = 0; n < NB8; ++n)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            uint4 qv[NB8][2];
+#pragma unroll
+            for (int n = 0; n < NB8; ++n) {
+              if (kKeep) qv[n][0] = held[m][c][0], qv[n][1] = held[m][c][1];
+              else load_q(n, m, c, qv[n]);
+            }
+            const uint4 r0 = lds128(row0 + m * kD + c * 64), r1 = lds128(row1 + m * kD + c * 64);
+            const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // (with one row block the unpacking, not the products, is the work: half of it goes to the
+              // convert instructions, which run beside the ALUs)
+              uint32_t a0, a1, a2, a3;
+              if (kKeep && m == 0) {
+                e4m3_to_f16(w0[e], a0, a2);
+                e4m3_to_f16(w1[e], a1, a3);
+              } else {
+                a0 = e4m3_even_to_f16(w0[e]), a1 = e4m3_even_to_f16(w1[e]);
+                a2 = e4m3_odd_to_f16(w0[e]), a3 = e4m3_odd_to_f16(w1[e]);
+              }
+#pragma unroll
+              for (int n = 0; n < NB8; ++n) {
+                const uint4 v = qv[n][e >> 1];
+                mma_f16(acc[m][n], a0, a1, a2, a3, (e & 1) ? v.z : v.x, (e & 1) ? v.w : v.y);
+              }
+            }
+          }
+        }
+        float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < NB8; ++n) {
+          const float2 f = *reinterpret_cast<const float2*>(factor + my_head * kRows + n * 8 + 2 * t);
+          constexpr float kLow = kKeep ? 0x1p-8f : 1.0f;   // converted codes carry their true value
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            best[i] = fmaxf(best[i], fmaxf(fmaf(acc[0][n][2 * i], kLow, acc[1][n][2 * i]) * f.x,
+                                           fmaf(acc[0][n][2 * i + 1], kLow, acc[1][n][2 * i + 1]) * f.y));
+        }
+        best[0] = quad_max(best[0]);
+        best[1] = quad_max(best[1]);
+        const int in_tile = g + 8 * t, page = (tile_a + mine - k) * kScoreTilePages + in_tile;   // what lanes t = 0, 1 store
+        if (t < 2 && page < pages) {
+          const float ks = p.k_scale ? __uint_as_float(lds32(tile + kScoreTilePages * pitch + (in_tile * hpc + my_head) * 4)) : 1.0f;
+          out[page] = (t ? best[1] : best[0]) * ks;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(smem_addr(&bar_empty[slot]));
+      mine += step;
+      slot += step;
+      if (slot >= p.slots) slot -= p.slots, phase ^= 1;
     }
+    k += count;
+    a.tile += count;
+    if (a.tile >= tile_off[seq + 1] - tile_off[seq]) next_seq(a);
   }
 }
 

@@ -171,29 +171,33 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
   k.out_stride_head = p->scores_stride_head;
   k.softmax_scale = p->softmax_scale;
   const int nb8 = p->rows <= 8 ? 1 : (p->rows <= 16 ? 2 : (p->rows <= 32 ? 4 : 8));
-  // kv heads per CTA: neighbouring heads of a page are neighbours in memory; as many as their query rows fit
+  // kv heads per CTA: neighbouring heads of a page are neighbours in memory; as many as their query
+  // rows fit, a power of two that divides the CTA's warps
   int heads = pa::kScoreMaxRows / (nb8 * 8);
-  if (heads > 8) heads = 8;
-  if (heads > p->num_kv_heads) heads = p->num_kv_heads;
+  while (heads > p->num_kv_heads) heads >>= 1;
   k.heads_per_cta = heads;
-  const int64_t rows_grid = (int64_t)p->num_seqs * ((p->num_kv_heads + heads - 1) / heads);
-  // tiles per CTA: preparing the query costs a CTA about as much as two tiles, so it takes up to
-  // eight while four CTAs per SM remain
   const int64_t tiles = ((int64_t)p->max_blocks_per_seq + pa::kScoreTilePages - 1) / pa::kScoreTilePages;
-  int64_t per = rows_grid * tiles / (4 * (int64_t)dev->sm_count);
-  per = per < 1 ? 1 : (per > 8 ? 8 : per);
-  while ((tiles + per - 1) / per > 65535) per *= 2;
-  k.tiles_per_cta = (int)per;
-  if (rows_grid > 0x7fffffff || per > 0x7ffffff) return PA_ERR_TOO_LARGE;
-  const dim3 grid((unsigned)rows_grid, (unsigned)((tiles + per - 1) / per));
-  const size_t smem = (size_t)heads * nb8 * 8 * (pa::kScoreRowBytes + 4);
+  const int64_t most = (int64_t)p->num_seqs * tiles * ((p->num_kv_heads + heads - 1) / heads);   // units of work, at most
+  if ((int64_t)p->num_seqs * tiles > 0x7fffffff) return PA_ERR_TOO_LARGE;
+  const int64_t grid = most < dev->sm_count ? most : dev->sm_count;
+  k.off_index = (heads * nb8 * 8 * (pa::kScoreRowBytes + 4) + 15) & ~15;
+  const int64_t off_ring = (k.off_index + ((int64_t)2 * p->num_seqs + 1) * 4 + 127) & ~(int64_t)127;
+  const int slot = pa::score_slot_bytes(heads);
+  int64_t slots = ((int64_t)dev->max_smem_optin - 1024 - off_ring) / slot;   // (1 KB: the kernel's barriers)
+  if (slots > pa::kScoreRingBytes / slot) slots = pa::kScoreRingBytes / slot;
+  if (slots > pa::kScoreMaxSlots) slots = pa::kScoreMaxSlots;
+  if (slots <= pa::kScoreWarps / heads || slots < pa::kScoreProducers) return PA_ERR_TOO_LARGE;   // the index of the sequences leaves no room
+  k.off_ring = (int)off_ring;
+  k.slots = (int)slots;
+  const int64_t smem = off_ring + slots * slot;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (nb8) {
-    case 1: return launch(pa::pa_block_score_kernel<1>, grid, pa::kScoreWarps * 32, smem, st, k);
-    case 2: return launch(pa::pa_block_score_kernel<2>, grid, pa::kScoreWarps * 32, smem, st, k);
-    case 4: return launch(pa::pa_block_score_kernel<4>, grid, pa::kScoreWarps * 32, smem, st, k);
-    default: return launch(pa::pa_block_score_kernel<8>, grid, pa::kScoreWarps * 32, smem, st, k);
-  }
+  void (*kernel)(pa::BlockScoreParams) = nb8 == 1   ? pa::pa_block_score_kernel<1>
+                                         : nb8 == 2 ? pa::pa_block_score_kernel<2>
+                                         : nb8 == 4 ? pa::pa_block_score_kernel<4>
+                                                    : pa::pa_block_score_kernel<8>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return cuda_fail(e);
+  return launch(kernel, dim3((unsigned)grid), pa::kScoreThreads, (size_t)smem, st, k);
 }
 
 int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
