@@ -106,7 +106,8 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   const int per_cta = p->block_size == 16 ? 4 : 1;
   const int threads = p->block_size == 1024 ? 512 : 128;
   int64_t grid = (units + per_cta - 1) / per_cta;
-  const int64_t cap = (int64_t)dev->sm_count * (p->block_size == 1024 ? 4 : 16);
+  if (units > (1 << 30)) return PA_ERR_TOO_LARGE;
+  const int64_t cap = (int64_t)dev->sm_count * (p->block_size == 1024 ? 1 : 5);   // what is resident at a time
   if (grid > cap) grid = cap;
   const size_t smem = (size_t)(p->num_seqs + 1) * 4;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -199,15 +199,16 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     }
     __syncthreads();
   }
-  const int64_t units = (int64_t)unit_off[p.S] * p.Hkv * 2;
+  // (32-bit unit numbers: the host refuses batches that could have more than 2^30 units)
+  const uint32_t units = (uint32_t)min((int64_t)unit_off[p.S] * p.Hkv * 2, (int64_t)1 << 30);
 
-  for (int64_t u0 = (int64_t)blockIdx.x * kUnits; u0 < units; u0 += (int64_t)gridDim.x * kUnits) {
-    const int64_t u = u0 + warp / WPU;
+  for (uint32_t u0 = blockIdx.x * kUnits; u0 < units; u0 += gridDim.x * kUnits) {
+    const uint32_t u = u0 + warp / WPU;
     bool live = u < units;
     // unit = ((page of the sequence, sequence), head, key or value), the last fastest
-    const bool is_v = live && (u & 1);
-    const int64_t ph = u >> 1;
-    const int touched = live ? (int)(ph / p.Hkv) : 0, head = live ? (int)(ph - (int64_t)touched * p.Hkv) : 0;
+    const bool is_v = live && (u & 1u);
+    const uint32_t ph = u >> 1;
+    const int touched = live ? (int)(ph / (uint32_t)p.Hkv) : 0, head = live ? (int)(ph - (uint32_t)touched * p.Hkv) : 0;
     int seq = 0;
     {
       int lo = 0, hi = p.S;
@@ -278,26 +279,44 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
       if (run < run0 || run >= run1) continue;
       load_run(run);
       loaded = run;
-      // non-negative bf16 bit patterns order like integers; infinity and NaN lie above all others
+      // non-negative bf16 bit patterns order like integers; infinity and NaN lie above all others.  A key's
+      // largest magnitude is that of its bounds (which pass over NaN).
       uint32_t any = 0;
+      if (is_v) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) any = __vmaxu2(any, raw[e] & 0x7fff7fffu);
+        for (int e = 0; e < 32; ++e) any = __vmaxu2(any, raw[e] & 0x7fff7fffu);
+      } else {
+        uint32_t lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[e] = 0x7f807f80u, hi[e] = 0xff80ff80u;   // +inf, -inf
+        bool some = run * 16 >= o0 && run * 16 + 16 <= o1;   // a whole run
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) lo[e & 7] = bf16x2_min(lo[e & 7], raw[e]), hi[e & 7] = bf16x2_max(hi[e & 7], raw[e]);
+        } else {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const int o = run * 16 + 4 * m + f;
+            if (o >= o0 && o < o1) {
+              some = true;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) lo[e] = bf16x2_min(lo[e], raw[8 * m + e]), hi[e] = bf16x2_max(hi[e], raw[8 * m + e]);
+            }
+          }
+        }
+        if (some) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) any = __vmaxu2(any, __vmaxu2(lo[e] & 0x7fff7fffu, hi[e] & 0x7fff7fffu));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], lo[e]), hi8[e] = bf16x2_max(hi8[e], hi[e]);
+      }
       if ((any & 0xffffu) >= 0x7f80u || (any >> 16) >= 0x7f80u) {
         any = 0;
 #pragma unroll
         for (int e = 0; e < 32; ++e) any = __vmaxu2(any, finite_abs2(raw[e]));
       }
       top = __vmaxu2(top, any);
-      if (want_bounds) {
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int o = run * 16 + 4 * m + f;
-          if (o >= o0 && o < o1) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], raw[8 * m + e]), hi8[e] = bf16x2_max(hi8[e], raw[8 * m + e]);
-          }
-        }
-      }
     }
     uint32_t top1 = __reduce_max_sync(kFullMask, max(top & 0xffffu, top >> 16));
     if (want_bounds) {
