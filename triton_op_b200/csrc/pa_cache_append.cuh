@@ -100,14 +100,28 @@ __device__ __forceinline__ uint32_t bf16x2_max(uint32_t a, uint32_t b) {
   return r;
 }
 
+// The larger magnitude of two, per half (the sign is of no use); passes over NaN.
+__device__ __forceinline__ uint32_t bf16x2_max_abs(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // Two words of bf16 pairs -> four e4m3 codes of x / scale.  A page's scale is a power of two, so its
-// reciprocal and the product are exact; a per-tensor scale may be anything and is divided by.
+// reciprocal and the product are exact, in bf16 too (what underflows there is far below e4m3's
+// smallest code); a per-tensor scale may be anything and is divided by.
 template <bool DIVIDE>
 __device__ __forceinline__ uint32_t quantise_four(uint32_t w0, uint32_t w1, float scale, float inv) {
   if (DIVIDE)
     return pack_e4m3x4(__fdiv_rn(bf16_lo_to_f32(w0), scale), __fdiv_rn(bf16_hi_to_f32(w0), scale),
                        __fdiv_rn(bf16_lo_to_f32(w1), scale), __fdiv_rn(bf16_hi_to_f32(w1), scale));
-  return pack_e4m3x4(bf16_lo_to_f32(w0) * inv, bf16_hi_to_f32(w0) * inv, bf16_lo_to_f32(w1) * inv, bf16_hi_to_f32(w1) * inv);
+  const uint32_t inv2 = (__float_as_uint(inv) >> 16) | (__float_as_uint(inv) & 0xffff0000u);
+  const uint32_t s0 = bf16x2_mul(w0, inv2), s1 = bf16x2_mul(w1, inv2);
+  return pack_e4m3x4(bf16_lo_to_f32(s0), bf16_hi_to_f32(s0), bf16_lo_to_f32(s1), bf16_hi_to_f32(s1));
 }
 // The smallest power of two >= s, for a positive s (what a page's scale becomes if it came as none).
 __device__ __forceinline__ float up_to_power(float s) {
@@ -202,42 +216,47 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
   // (32-bit unit numbers: the host refuses batches that could have more than 2^30 units)
   const uint32_t units = (uint32_t)min((int64_t)unit_off[p.S] * p.Hkv * 2, (int64_t)1 << 30);
 
+  // A unit, decoded: ((page of the sequence, sequence), head, key or value), the last fastest.  The next
+  // unit is decoded, and its block-table entry requested, while the rows of the current one are on
+  // their way: of the chain sequence -> page id -> rows only the rows are waited for.
+  struct Unit {
+    bool live, is_v;
+    int head, o0, o1;      // slots [o0, o1) of the page receive rows row0 ..
+    int row0, blk;
+  };
+  auto decode = [&](uint32_t u) -> Unit {
+    Unit n;
+    n.live = u < units;
+    n.is_v = (u & 1u) != 0;
+    const uint32_t ph = n.live ? u >> 1 : 0u;
+    const int touched = (int)(ph / (uint32_t)p.Hkv);
+    n.head = (int)(ph - (uint32_t)touched * p.Hkv);
+    n.o0 = n.o1 = n.row0 = n.blk = 0;
+    if (!n.live) return n;
+    int lo = 0, hi = p.S;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (unit_off[mid] <= touched) lo = mid; else hi = mid;
+    }
+    int row, count, pos;
+    rows_of(lo, row, count, pos, false);
+    const int page = pos / BS + (touched - unit_off[lo]);
+    n.blk = p.block_tables[(int64_t)lo * p.bt_stride_seq + page];
+    n.o0 = max(pos - page * BS, 0);
+    n.o1 = min(BS, pos + count - page * BS);
+    n.row0 = row + (page * BS + n.o0 - pos);
+    return n;
+  };
+  Unit next = decode(blockIdx.x * kUnits + warp / WPU);
   for (uint32_t u0 = blockIdx.x * kUnits; u0 < units; u0 += gridDim.x * kUnits) {
-    const uint32_t u = u0 + warp / WPU;
-    bool live = u < units;
-    // unit = ((page of the sequence, sequence), head, key or value), the last fastest
-    const bool is_v = live && (u & 1u);
-    const uint32_t ph = u >> 1;
-    const int touched = live ? (int)(ph / (uint32_t)p.Hkv) : 0, head = live ? (int)(ph - (uint32_t)touched * p.Hkv) : 0;
-    int seq = 0;
-    {
-      int lo = 0, hi = p.S;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (unit_off[mid] <= touched) lo = mid; else hi = mid;
-      }
-      seq = lo;
-    }
-    int row = 0, count = 0, pos = 0;
-    if (live) rows_of(seq, row, count, pos, false);
-    const int page = pos / BS + (touched - unit_off[seq]);
-    // slots [o0, o1) of the page receive rows row0 ..
-    const int o0 = max(pos - page * BS, 0), o1 = live ? min(BS, pos + count - page * BS) : o0;
-    const int row0 = row + (page * BS + o0 - pos);
-    int blk = live ? p.block_tables[(int64_t)seq * p.bt_stride_seq + page] : 0;
-    if ((unsigned)blk >= (unsigned)p.num_blocks) {
-      if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_BAD_PAGE_ID);
-      live = false;
-      blk = 0;
-    }
+    const Unit cur = next;
+    bool live = cur.live;
+    const bool is_v = cur.is_v;
+    const int head = cur.head, o0 = cur.o0, o1 = cur.o1, row0 = cur.row0;
     const uint8_t* src = (is_v ? p.value : p.key) +
                          2 * ((int64_t)row0 * (is_v ? p.value_stride_tok : p.key_stride_tok) +
                               (int64_t)head * (is_v ? p.value_stride_head : p.key_stride_head));
     const int64_t tok_bytes = 2 * (is_v ? p.value_stride_tok : p.key_stride_tok);
-    uint8_t* cache = is_v ? p.value_cache + (int64_t)blk * p.vc_stride_block + (int64_t)head * p.vc_stride_head
-                          : p.key_cache + (int64_t)blk * p.kc_stride_block + (int64_t)head * p.kc_stride_head;
-    float* scale_at = (is_v ? p.v_scale : p.k_scale) + (PER_BLOCK ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
-    const float old_scale = live ? *scale_at : 1.0f;
     // keys: lane = (chunk c of 16 dims, phase f), slots f, f + 4, f + 8, f + 12 of a run, 32 bytes each
     // values: lane = head dims 4 lane .. 4 lane + 3 of every slot of a run, 8 bytes each
     const int c = lane >> 2, f = lane & 3;
@@ -263,8 +282,24 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
       }
     };
     // runs of the page that receive rows: [run0, run1); this warp takes sub, sub + WPU, ... of all runs
-    const int run0 = o0 >> 4, run1 = live && o1 > o0 ? ((o1 - 1) >> 4) + 1 : run0;
+    const int run0 = o0 >> 4, run1 = o1 > o0 ? ((o1 - 1) >> 4) + 1 : run0;
     auto mine = [&](int k) -> int { return sub + k * WPU; };
+    int loaded = -1;
+    if (mine(0) >= run0 && mine(0) < run1) {
+      loaded = mine(0);
+      load_run(loaded);
+    }
+    next = decode(u0 + gridDim.x * kUnits + warp / WPU);
+    int blk = cur.blk;
+    if ((unsigned)blk >= (unsigned)p.num_blocks) {
+      if (live && lane == 0 && p.status) atomicOr(p.status, PA_DEV_BAD_PAGE_ID);
+      live = false;
+      blk = 0;
+    }
+    uint8_t* cache = is_v ? p.value_cache + (int64_t)blk * p.vc_stride_block + (int64_t)head * p.vc_stride_head
+                          : p.key_cache + (int64_t)blk * p.kc_stride_block + (int64_t)head * p.kc_stride_head;
+    float* scale_at = (is_v ? p.v_scale : p.k_scale) + (PER_BLOCK ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
+    const float old_scale = live ? *scale_at : 1.0f;
 
     // ---- the largest finite |x|, and the smallest and largest key of every head dim
     uint32_t top = 0;
@@ -272,19 +307,21 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) lo8[e] = 0x7f807f80u, hi8[e] = 0xff80ff80u;   // +inf, -inf
     const bool want_bounds = p.bounds != nullptr && !is_v;
-    int loaded = -1;
 #pragma unroll 1
     for (int k = 0; k < kPerWarp; ++k) {
       const int run = mine(k);
       if (run < run0 || run >= run1) continue;
-      load_run(run);
-      loaded = run;
+      if (run != loaded) {
+        load_run(run);
+        loaded = run;
+      }
       // non-negative bf16 bit patterns order like integers; infinity and NaN lie above all others.  A key's
       // largest magnitude is that of its bounds (which pass over NaN).
       uint32_t any = 0;
       if (is_v) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) any = __vmaxu2(any, raw[e] & 0x7fff7fffu);
+        for (int e = 0; e < 32; ++e) any = bf16x2_max_abs(any, raw[e]);
+        any &= 0x7fff7fffu;
       } else {
         uint32_t lo[8], hi[8];
 #pragma unroll
