@@ -184,13 +184,20 @@ def lib() -> C.CDLL:
     return L
 
 
+# The handle of torch's current stream of a device (torch.cuda.current_stream builds an object around it,
+# which costs more host time than everything else between the arguments and the launch).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def launch(index: int, fn, where: str, *args) -> None:
     """Calls a launching entry point with device ``index`` current, on torch's current stream of it."""
     if index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream), where)
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream), where)
+            status = fn(*args, _raw_stream(index))
+    if status != PA_OK:
+        raise PaError(status, where)
 
 
 def check(status: int, where: str) -> None:

@@ -110,11 +110,13 @@ _APPEND = struct.Struct("=2I11Q10i13q")
 assert _APPEND.size == C.sizeof(_lib.PaCacheAppendParams)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [T, Hkv, D] bf16 with 16-byte aligned rows (a copy where it has none)."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+def _rows(t: torch.Tensor):
+    """``t`` [T, Hkv, D] bf16 with 16-byte aligned rows (a copy where it has none), and its strides."""
+    stride = t.stride()
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        stride = t.stride()
+    return t, stride
 
 
 def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -137,26 +139,30 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     that have no place; they are skipped.  No page may get rows of two sequences in a call.  Runs on
     the current stream; there is no CPU fallback.
     """
-    dev = key.device
-    if not (key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16 and key.shape == value.shape and key.dim() == 3):
+    on, dev = key.get_device(), key.device
+    k_shape, c_shape = key.shape, key_cache.shape
+    if not (key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16 and k_shape == value.shape and len(k_shape) == 3):
         raise PaArgumentError("key and value must be bf16 [num_tokens, num_kv_heads, head_size] of one shape")
-    if not (key_cache.dim() == 5 and key_cache.dtype == FP8_DTYPE and value_cache.dtype == FP8_DTYPE):
+    if not (len(c_shape) == 5 and key_cache.dtype == FP8_DTYPE and value_cache.dtype == FP8_DTYPE):
         raise PaArgumentError(f"append_kv_cache needs {FP8_DTYPE} caches, a 5-D key_cache and a 4-D or 5-D value_cache")
-    num_tokens, num_kv_heads, head_size = key.shape
-    num_blocks, bs = key_cache.shape[0], key_cache.shape[3]
+    num_tokens, num_kv_heads, head_size = k_shape
+    num_blocks, bs = c_shape[0], c_shape[3]
     if head_size != 128 or bs not in SUPPORTED_BLOCK_SIZES:
         raise PaArgumentError(f"head_size must be 128 and block_size in {list(SUPPORTED_BLOCK_SIZES)}, but got {head_size} and {bs}")
-    if key_cache.shape != (num_blocks, num_kv_heads, head_size // 16, bs, 16):
+    if c_shape != (num_blocks, num_kv_heads, head_size // 16, bs, 16):
         raise PaArgumentError(f"key_cache must be [num_blocks, {num_kv_heads}, {head_size // 16}, block_size, 16]")
-    trans = value_cache.dim() == 5
+    v_shape = value_cache.shape
+    trans = len(v_shape) == 5
     want_v = (num_blocks, num_kv_heads, bs // 16, head_size, 16) if trans else (num_blocks, num_kv_heads, head_size, bs)
-    if value_cache.shape != want_v:
+    if v_shape != want_v:
         raise PaArgumentError(f"value_cache must be {want_v}")
-    if not (_inner_contiguous(key_cache, 2) and _inner_contiguous(value_cache, 2)):
+    kc_stride, vc_stride = key_cache.stride(), value_cache.stride()
+    if not ((kc_stride[4] == 1 and kc_stride[3] == 16 and kc_stride[2] == 16 * bs) or _inner_contiguous(key_cache, 2)) or not (
+            (not trans and vc_stride[3] == 1 and vc_stride[2] == bs) or _inner_contiguous(value_cache, 2)):
         raise PaArgumentError("the per-(block, head) slabs of the KV caches must be contiguous")
-    for name, s in (("key_scale", key_scale), ("value_scale", value_scale)):
-        if not (isinstance(s, torch.Tensor) and s.dtype == torch.float32 and s.device == dev):
-            raise PaArgumentError(f"{name} must be a float32 tensor on {dev}")
+    if not (isinstance(key_scale, torch.Tensor) and isinstance(value_scale, torch.Tensor)
+            and key_scale.dtype == torch.float32 and value_scale.dtype == torch.float32):
+        raise PaArgumentError("key_scale and value_scale must be float32 tensors")
     if key_scale.dim() == 0 and value_scale.dim() == 0:
         mode, s_block, s_head = _lib.PA_QUANT_PER_TENSOR, 0, 0
     else:
@@ -164,27 +170,32 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
         if (num_blocks > 1 and s_block == 0) or (num_kv_heads > 1 and s_head == 0):
             raise PaArgumentError("block kv scales are written: every page and kv head needs a place of its own")
         mode = _lib.PA_QUANT_PER_BLOCK
-    b_block = b_head = 0
+    b_block = b_head = b_ptr = st_ptr = 0
     if key_bounds is not None:
+        b_stride = key_bounds.stride()
         if not (key_bounds.dtype == FP8_DTYPE and key_bounds.shape == (num_blocks, num_kv_heads, 2, head_size)
-                and _inner_contiguous(key_bounds, 2) and key_bounds.device == dev):
+                and b_stride[3] == 1 and b_stride[2] == head_size and key_bounds.get_device() == on):
             raise PaArgumentError(f"key_bounds must be {FP8_DTYPE} {(num_blocks, num_kv_heads, 2, head_size)} on {dev}, its last two dims contiguous")
-        b_block, b_head = key_bounds.stride(0), key_bounds.stride(1)
-    num_seqs = block_tables.shape[0]
-    for name, t in (("block_tables", block_tables), ("sequence_lengths", sequence_lengths), ("query_start_loc", query_start_loc)):
-        if not (t.dtype == torch.int32 and t.device == dev):
-            raise PaArgumentError(f"{name} must be int32 on {dev}")
-    if not (block_tables.dim() == 2 and block_tables.shape[1] >= 1 and sequence_lengths.numel() == num_seqs
+        b_block, b_head, b_ptr = b_stride[0], b_stride[1], key_bounds.data_ptr()
+    t_shape = block_tables.shape
+    num_seqs = t_shape[0]
+    if not (block_tables.dtype == torch.int32 and sequence_lengths.dtype == torch.int32 and query_start_loc.dtype == torch.int32):
+        raise PaArgumentError("block_tables, sequence_lengths and query_start_loc must be int32")
+    if not (len(t_shape) == 2 and t_shape[1] >= 1 and sequence_lengths.numel() == num_seqs
             and query_start_loc.numel() == num_seqs + 1):
         raise PaArgumentError("block_tables must be [num_seqs, max_blocks], sequence_lengths [num_seqs] and query_start_loc [num_seqs + 1]")
-    for name, t in (("value", value), ("key_cache", key_cache), ("value_cache", value_cache)):
-        if t.device != dev:
-            raise PaArgumentError(f"{name} must live on {dev}, the key's device")
-    if status is not None and not (status.dtype == torch.int32 and status.device == dev):
-        raise PaArgumentError(f"status must be an int32 tensor on {dev}")
-    if not key.is_cuda:
+    if not (value.get_device() == on and key_cache.get_device() == on and value_cache.get_device() == on
+            and key_scale.get_device() == on and value_scale.get_device() == on and block_tables.get_device() == on
+            and sequence_lengths.get_device() == on and query_start_loc.get_device() == on):
+        raise PaArgumentError(f"all tensors must live on {dev}, the key's device")
+    if status is not None:
+        if not (status.dtype == torch.int32 and status.device == dev):
+            raise PaArgumentError(f"status must be an int32 tensor on {dev}")
+        st_ptr = status.data_ptr()
+    if on < 0:
         raise RuntimeError("append_kv_cache runs on CUDA tensors only; there is no CPU fallback")
-    key, value = _rows(key), _rows(value)
+    key, key_stride = _rows(key)
+    value, value_stride = _rows(value)
     if block_tables.stride(1) != 1:
         block_tables = block_tables.contiguous()
     if not sequence_lengths.is_contiguous():
@@ -194,10 +205,9 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     p = _lib.PaCacheAppendParams.from_buffer_copy(_APPEND.pack(
         _APPEND.size, _lib.PA_ABI_VERSION,
         key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
-        value_scale.data_ptr(), 0 if key_bounds is None else key_bounds.data_ptr(), block_tables.data_ptr(),
-        sequence_lengths.data_ptr(), query_start_loc.data_ptr(), 0 if status is None else status.data_ptr(),
-        num_tokens, num_seqs, num_kv_heads, head_size, bs, num_blocks, block_tables.shape[1], mode,
+        value_scale.data_ptr(), b_ptr, block_tables.data_ptr(), sequence_lengths.data_ptr(), query_start_loc.data_ptr(), st_ptr,
+        num_tokens, num_seqs, num_kv_heads, head_size, bs, num_blocks, t_shape[1], mode,
         _lib.PA_V_TRANSPOSED if trans else _lib.PA_V_NORMAL, 0,
-        key.stride(0), key.stride(1), value.stride(0), value.stride(1), key_cache.stride(0), key_cache.stride(1),
-        value_cache.stride(0), value_cache.stride(1), s_block, s_head, b_block, b_head, block_tables.stride(0)))
-    _lib.launch(key.get_device(), _lib.lib().pa_cache_append_sm100, "pa_cache_append_sm100", C.byref(p))
+        key_stride[0], key_stride[1], value_stride[0], value_stride[1], kc_stride[0], kc_stride[1],
+        vc_stride[0], vc_stride[1], s_block, s_head, b_block, b_head, block_tables.stride(0)))
+    _lib.launch(on, _lib.lib().pa_cache_append_sm100, "pa_cache_append_sm100", C.byref(p))

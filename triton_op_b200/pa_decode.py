@@ -436,15 +436,6 @@ _PACK = struct.Struct("=2I17Q10i19q6if6i4x")
 assert _PACK.size == C.sizeof(PaDecodeParams)
 
 
-def _slabs_dense(t: torch.Tensor, stride: tuple, bs: int) -> bool:
-    """_inner_contiguous(t, 2) for a key or value cache, the common layouts first."""
-    if len(stride) == 5 and stride[4] == 1 and stride[3] == 16 and stride[2] == 16 * t.shape[3]:
-        return True
-    if len(stride) == 4 and stride[3] == 1 and stride[2] == bs:
-        return True
-    return _inner_contiguous(t, 2)
-
-
 def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
                     query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,
                     alibi_slopes, sink_tokens, status):
@@ -470,7 +461,7 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
         _fail(f"block kv scales and block tables per kv head need {FP8_DTYPE} caches, but got {key_cache.dtype} and {value_cache.dtype}")
     if compute_type is not torch.bfloat16 and not _compute_type_matches(compute_type, torch.bfloat16):
         _fail(f"compute_type {compute_type} disagrees with output.dtype {output.dtype}")
-    q_dtype = _dtype_code(query.dtype, "query")
+    q_dtype = _lib.PA_DT_BF16 if query.dtype == torch.bfloat16 else _dtype_code(query.dtype, "query")
     if not (sequence_lengths.dtype == torch.int32 and block_tables.dtype == torch.int32):
         _fail("sequence_lengths and block_tables must be int32")
     if not (query.get_device() == on and key_cache.get_device() == on and value_cache.get_device() == on
@@ -514,7 +505,9 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
     if q_stride[2] != 1 or q_stride[1] != head_size:
         query = query.contiguous()
         q_stride = query.stride()
-    if not (_slabs_dense(key_cache, k_stride, bs) and _slabs_dense(value_cache, v_stride, bs)):
+    # (the common layouts first; _inner_contiguous knows all)
+    if not ((k_stride[4] == 1 and k_stride[3] == 16 and k_stride[2] == 16 * bs) or _inner_contiguous(key_cache, 2)) or not (
+            (v_layout == _lib.PA_V_NORMAL and v_stride[3] == 1 and v_stride[2] == bs) or _inner_contiguous(value_cache, 2)):
         _fail("the per-(block, head) slabs of the KV caches must be contiguous")
     if not sequence_lengths.is_contiguous():
         sequence_lengths = sequence_lengths.contiguous()
@@ -542,7 +535,18 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
     if (key_scale is None) != (value_scale is None):
         _fail("key_scale and value_scale go together")
     kv_mode, ks_ptr, vs_ptr, s_block, s_head = _lib.PA_QUANT_NONE, 0, 0, 0, 0
-    if key_scale is not None:
+    by_page = (num_blocks, num_kv_heads, 1, 1)
+    if (type(key_scale) is torch.Tensor and type(value_scale) is torch.Tensor and key_scale.shape == by_page
+            and value_scale.shape == by_page and num_blocks * num_kv_heads > 1):   # the common case, checked in one go
+        ks_stride, vs_stride = key_scale.stride(), value_scale.stride()
+        if not (key_scale.dtype == torch.float32 and value_scale.dtype == torch.float32
+                and key_scale.get_device() == on and value_scale.get_device() == on):
+            _fail(f"key_scale and value_scale must be float32 tensors on {dev}, the output's device")
+        kv_mode, s_block, s_head = _lib.PA_QUANT_PER_BLOCK, ks_stride[0], ks_stride[1]
+        if not (vs_stride[0] == s_block and vs_stride[1] == s_head):
+            _fail("block kv scales must share strides")
+        ks_ptr, vs_ptr = key_scale.data_ptr(), value_scale.data_ptr()
+    elif key_scale is not None:
         if isinstance(key_scale, (int, float)):
             key_scale = torch.full((), float(key_scale), dtype=torch.float32, device=dev)
         if isinstance(value_scale, (int, float)):

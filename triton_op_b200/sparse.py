@@ -36,20 +36,24 @@ def _fail(msg: str) -> None:
     raise PaArgumentError(msg)
 
 
-def _tables_and_lengths(sequence_lengths, block_tables, dev) -> Tuple[torch.Tensor, torch.Tensor]:
+def _tables_and_lengths(sequence_lengths, block_tables, on: int):
+    """(sequence_lengths, block_tables, rows, columns, row stride) after the checks."""
     if not (sequence_lengths.dtype == torch.int32 and block_tables.dtype == torch.int32):
         _fail("sequence_lengths and block_tables must be int32")
-    if not (block_tables.dim() == 2 and sequence_lengths.numel() == block_tables.shape[0]):
+    shape = block_tables.shape
+    if not (len(shape) == 2 and sequence_lengths.numel() == shape[0]):
         _fail("block_tables must be [num_seqs, max_blocks] and sequence_lengths [num_seqs]")
-    if block_tables.shape[1] < 1:
+    if shape[1] < 1:
         _fail("block_tables must have at least one column")
-    if not (sequence_lengths.device == dev and block_tables.device == dev):
-        _fail(f"sequence_lengths and block_tables must live on {dev}")
-    if sequence_lengths.dim() != 1 or sequence_lengths.stride(0) != 1:
-        sequence_lengths = sequence_lengths.reshape(-1).contiguous()
-    if block_tables.stride(1) != 1:
+    if not (sequence_lengths.get_device() == on and block_tables.get_device() == on):
+        _fail("sequence_lengths and block_tables must live on the device of the other tensors")
+    if not sequence_lengths.is_contiguous():
+        sequence_lengths = sequence_lengths.contiguous()
+    stride = block_tables.stride()
+    if stride[1] != 1:
         block_tables = block_tables.contiguous()
-    return sequence_lengths, block_tables
+        stride = block_tables.stride()
+    return sequence_lengths, block_tables, shape[0], shape[1], stride[0]
 
 
 def _status_ptr(status, dev) -> int:
@@ -73,34 +77,38 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
     ``[num_blocks, num_kv_heads, 2, head_size]``; ``key_scale`` ``None``, per tensor or
     ``[num_blocks, num_kv_heads, 1, 1]``; ``scores``: an output tensor to use.
     """
-    dev = query.device
-    if query.dim() != 3:
-        _fail(f"Expected 3D query tensor, but got shape {tuple(query.shape)}")
-    q_dtype = _dtype_code(query.dtype, "query")
-    if not (key_bounds.dim() == 4 and key_bounds.dtype == FP8_DTYPE and key_bounds.device == dev):
+    dev, on = query.device, query.get_device()
+    q_shape, b_shape = query.shape, key_bounds.shape
+    if len(q_shape) != 3:
+        _fail(f"Expected 3D query tensor, but got shape {tuple(q_shape)}")
+    q_dtype = _lib.PA_DT_BF16 if query.dtype == torch.bfloat16 else _dtype_code(query.dtype, "query")
+    if not (len(b_shape) == 4 and key_bounds.dtype == FP8_DTYPE and key_bounds.get_device() == on):
         _fail(f"key_bounds must be a 4D {FP8_DTYPE} tensor on {dev}")
-    num_blocks, num_kv_heads, two, head_size = key_bounds.shape
-    num_seqs, q_heads, q_size = query.shape
+    num_blocks, num_kv_heads, two, head_size = b_shape
+    num_seqs, q_heads, q_size = q_shape
     if not (two == 2 and head_size == 128 and q_size == 128):
         _fail("key_bounds must be [num_blocks, num_kv_heads, 2, 128] and query [num_seqs, heads, 128]")
-    if key_bounds.stride(3) != 1 or key_bounds.stride(2) != head_size:
+    b_stride = key_bounds.stride()
+    if b_stride[3] != 1 or b_stride[2] != head_size:
         _fail("the last two dims of key_bounds must be contiguous")
     if block_size not in SUPPORTED_BLOCK_SIZES:
         _fail(f"block_size == {block_size} not in {list(SUPPORTED_BLOCK_SIZES)}")
-    rows = q_heads // num_kv_heads
     if not 1 <= query_sequence_length <= 4:
         _fail(f"QUERY_SEQ_LEN={query_sequence_length}, only 1 to 4 are supported")
-    if rows * num_kv_heads != q_heads or rows < 1 or rows % query_sequence_length:
+    rows = q_heads // num_kv_heads if num_kv_heads else 0
+    if rows < 1 or rows * num_kv_heads != q_heads or rows % query_sequence_length:
         _fail("query heads must be num_kv_heads * query_sequence_length * group_size")
     if rows > 64:
         _fail(f"equivalent query group size {rows} exceeds maximum of 64")
     if not softmax_scale > 0:
         _fail(f"softmax_scale must be positive, but got {softmax_scale}")
-    sequence_lengths, block_tables = _tables_and_lengths(sequence_lengths, block_tables, dev)
-    if block_tables.shape[0] != num_seqs:
+    sequence_lengths, block_tables, table_rows, width, t_stride = _tables_and_lengths(sequence_lengths, block_tables, on)
+    if table_rows != num_seqs:
         _fail("block_tables must be [num_seqs, max_blocks] and sequence_lengths [num_seqs]")
-    if query.stride(2) != 1 or query.stride(1) != head_size or (query.stride(0) * query.element_size()) % 16 or query.data_ptr() % 16:
+    stride = query.stride()
+    if stride[2] != 1 or stride[1] != head_size or (stride[0] * query.element_size()) % 16 or query.data_ptr() % 16:
         query = query.clone(memory_format=torch.contiguous_format)
+        stride = query.stride()
     q_mode, q_ptr, q_stride = _lib.PA_QUANT_NONE, 0, 0
     if query_scale is not None:
         if isinstance(query_scale, (int, float)):
@@ -121,32 +129,33 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
         if isinstance(key_scale, (int, float)):
             key_scale = torch.full((), float(key_scale), dtype=torch.float32, device=dev)
         key_scale, kv_mode = _kv_scale(key_scale, None, "key_scale", dev)
-        if key_scale.device != dev:
+        if key_scale.get_device() != on:
             _fail(f"key_scale must live on {dev}")
         if kv_mode == _lib.PA_QUANT_PER_TOKEN:
             _fail("key bounds go with a key scale per tensor or per (block, head), not per token")
         if kv_mode == _lib.PA_QUANT_PER_BLOCK:
             if key_scale.shape != (num_blocks, num_kv_heads, 1, 1):
                 _fail(f"key_scale must be [num_blocks, num_kv_heads, 1, 1] = {(num_blocks, num_kv_heads, 1, 1)}")
-            s_block, s_head = key_scale.stride(0), key_scale.stride(1)
+            ks_stride = key_scale.stride()
+            s_block, s_head = ks_stride[0], ks_stride[1]
         ks_ptr = key_scale.data_ptr()
-    width = block_tables.shape[1]
     if scores is None:
         scores = torch.empty_strided((num_seqs, num_kv_heads, width), (num_kv_heads * width, width, 1), dtype=torch.float32, device=dev)
     elif not (scores.dtype == torch.float32 and scores.device == dev and scores.shape == (num_seqs, num_kv_heads, width)
               and scores.stride(2) == 1):
         _fail(f"scores must be fp32 {(num_seqs, num_kv_heads, width)} on {dev}, its last dim contiguous")
+    s_stride = scores.stride()
     status_ptr = _status_ptr(status, dev)
-    if not query.is_cuda:
+    if on < 0:
         raise RuntimeError("score_blocks runs on CUDA tensors only; there is no CPU fallback")
     p = _lib.PaBlockScoreParams.from_buffer_copy(_SCORE.pack(
         _SCORE.size, _lib.PA_ABI_VERSION,
         query.data_ptr(), key_bounds.data_ptr(), block_tables.data_ptr(), sequence_lengths.data_ptr(), q_ptr, ks_ptr,
         scores.data_ptr(), status_ptr,
         num_seqs, num_kv_heads, rows, head_size, block_size, num_blocks, width, q_dtype, q_mode, kv_mode,
-        query.stride(0), key_bounds.stride(0), key_bounds.stride(1), block_tables.stride(0), q_stride, s_block, s_head,
-        scores.stride(0), scores.stride(1), float(softmax_scale), 0))
-    _lib.launch(query.get_device(), _lib.lib().pa_block_scores_sm100, "pa_block_scores_sm100", C.byref(p))
+        stride[0], b_stride[0], b_stride[1], t_stride, q_stride, s_block, s_head,
+        s_stride[0], s_stride[1], float(softmax_scale), 0))
+    _lib.launch(on, _lib.lib().pa_block_scores_sm100, "pa_block_scores_sm100", C.byref(p))
     return scores
 
 
@@ -163,20 +172,22 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     ``scores`` (fp32 ``[num_seqs, num_kv_heads, max_blocks]``), NaN lowest, ties to the lower place.
     With several query tokens ``keep_last`` has to cover the last ``query_len`` tokens: 2.
     """
-    dev = scores.device
-    if not (scores.dim() == 3 and scores.dtype == torch.float32):
-        _fail(f"scores must be a 3D float32 tensor, but got {scores.dtype} of shape {tuple(scores.shape)}")
+    dev, on = scores.device, scores.get_device()
+    sc_shape = scores.shape
+    if not (len(sc_shape) == 3 and scores.dtype == torch.float32):
+        _fail(f"scores must be a 3D float32 tensor, but got {scores.dtype} of shape {tuple(sc_shape)}")
     if block_size not in SUPPORTED_BLOCK_SIZES:
         _fail(f"block_size == {block_size} not in {list(SUPPORTED_BLOCK_SIZES)}")
-    num_seqs, num_kv_heads, columns = scores.shape
-    sequence_lengths, block_tables = _tables_and_lengths(sequence_lengths, block_tables, dev)
-    width = block_tables.shape[1]
-    if block_tables.shape[0] != num_seqs or columns < width or num_kv_heads < 1:
+    num_seqs, num_kv_heads, columns = sc_shape
+    sequence_lengths, block_tables, table_rows, width, bt_stride = _tables_and_lengths(sequence_lengths, block_tables, on)
+    if table_rows != num_seqs or columns < width or num_kv_heads < 1:
         _fail("scores must be [num_seqs, num_kv_heads, >= max_blocks]")
     if keep_first < 0 or keep_last < 1 or top_k < keep_first + keep_last:
         _fail(f"top_k must hold keep_first >= 0 and keep_last >= 1 pages, but got {top_k}, {keep_first}, {keep_last}")
-    if scores.stride(2) != 1:
+    sc_stride = scores.stride()
+    if sc_stride[2] != 1:
         scores = scores.contiguous()
+        sc_stride = scores.stride()
     if tables is None:
         tables = torch.empty_strided((num_seqs, num_kv_heads, top_k), (num_kv_heads * top_k, top_k, 1), dtype=torch.int32, device=dev)
     elif not (tables.dtype == torch.int32 and tables.device == dev and tables.shape == (num_seqs, num_kv_heads, top_k)
@@ -186,15 +197,16 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
         lengths = torch.empty_strided((num_seqs,), (1,), dtype=torch.int32, device=dev)
     elif not (lengths.dtype == torch.int32 and lengths.device == dev and lengths.shape == (num_seqs,) and lengths.is_contiguous()):
         _fail(f"lengths must be a contiguous int32 tensor of {num_seqs} on {dev}")
+    t_stride = tables.stride()
     status_ptr = _status_ptr(status, dev)
-    if not scores.is_cuda:
+    if on < 0:
         raise RuntimeError("select_blocks runs on CUDA tensors only; there is no CPU fallback")
     p = _lib.PaBlockSelectParams.from_buffer_copy(_SELECT.pack(
         _SELECT.size, _lib.PA_ABI_VERSION,
         scores.data_ptr(), block_tables.data_ptr(), sequence_lengths.data_ptr(), tables.data_ptr(), lengths.data_ptr(), status_ptr,
         num_seqs, num_kv_heads, block_size, width, int(top_k), int(keep_first), int(keep_last), 0,
-        scores.stride(0), scores.stride(1), block_tables.stride(0), tables.stride(0), tables.stride(1)))
-    _lib.launch(scores.get_device(), _lib.lib().pa_block_select_sm100, "pa_block_select_sm100", C.byref(p))
+        sc_stride[0], sc_stride[1], bt_stride, t_stride[0], t_stride[1]))
+    _lib.launch(on, _lib.lib().pa_block_select_sm100, "pa_block_select_sm100", C.byref(p))
     return tables, lengths
 
 
