@@ -46,7 +46,7 @@ struct BlockSelectParams {
 // not compete: kKeyNone for places past the context, kKeyKept for the kept pages.
 constexpr uint32_t kKeyNone = 0u, kKeyNan = 1u, kKeyKept = 0xffffffffu;
 __device__ __forceinline__ uint32_t score_key(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.0f);   // (the two zeros are one value)
   if ((u & 0x7fffffffu) > 0x7f800000u) return kKeyNan;
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
