@@ -390,7 +390,7 @@ int pa_block_scores_sm100(const PaBlockScoreParams* params, void* stream);
 /*
  * Page selection (no counterpart in the reference): per (sequence, kv head) the first keep_first and
  * the last keep_last pages of the context and those with the highest scores of the others (NaN
- * lowest, ties to the lower place), top_k in all, as a block table in the order of the context.
+ * as -inf, ties to the lower place), top_k in all, as a block table in the order of the context.
  * A sequence of at most top_k pages keeps them all.  Unused entries become 0.
  *   lengths[s] = tokens in the pages of one such table (the same for every kv head)
  */

@@ -203,7 +203,7 @@ def select(score, lengths, block_tables, bs: int, top_k: int, keep_first: int = 
                 if i < keep_first or i >= pages - keep_last:
                     return (0, 0.0, i)
                 x = float(score[s, h, i])
-                return (1, -x, i) if not math.isnan(x) else (2, 0.0, i)
+                return (1, math.inf if math.isnan(x) else -x, i)      # NaN as -inf
             best = sorted(sorted(range(pages), key=rank)[:held])
             for place, i in enumerate(best):
                 tables[s, h, place] = block_tables[s, i]

@@ -3,8 +3,8 @@
 // highest scores, ties to the lower page, top_k pages in all -- written as a block table of its own
 // in the order of the context, with the number of tokens those pages hold.
 //
-// One CTA per (sequence, kv head).  Scores become unsigned keys of the same order (NaN below
-// everything).  The key of rank top_k is found by narrowing a key range: a histogram of equal bins over
+// One CTA per (sequence, kv head).  Scores become unsigned keys of the same order (NaN
+// as -inf).  The key of rank top_k is found by narrowing a key range: a histogram of equal bins over
 // [smallest, largest] key, then the bin in which the rank falls.  Bins over the ACTUAL range spread the
 // shared-memory counters, where a fixed digit would count most pages of a head in two or three of
 // them (their scores share sign and exponent), and leave few keys in the rank's bin: up to 32 of them
@@ -42,12 +42,12 @@ struct BlockSelectParams {
   int64_t out_stride_seq, out_stride_head;
 };
 
-// Unsigned key with the order of the floats, NaN below -inf.  Two keys no score has mark the pages that do
+// Unsigned key with the order of the floats, NaN as -inf.  Two keys no score has mark the pages that do
 // not compete: kKeyNone for places past the context, kKeyKept for the kept pages.
-constexpr uint32_t kKeyNone = 0u, kKeyNan = 1u, kKeyKept = 0xffffffffu;
+constexpr uint32_t kKeyNone = 0u, kKeyLowest = 0x007fffffu, kKeyKept = 0xffffffffu;
 __device__ __forceinline__ uint32_t score_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);   // (the two zeros are one value)
-  if ((u & 0x7fffffffu) > 0x7f800000u) return kKeyNan;
+  if ((u & 0x7fffffffu) > 0x7f800000u) return kKeyLowest;
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
@@ -218,6 +218,9 @@ pa_block_select_kernel(const __grid_constant__ BlockSelectParams p) {
     }
   }
   // ---- ordered pass: a taken page goes to the place that the taken pages before it leave
+  // (places first get the number of their page, in shared memory if top_k of them fit, and the page ids are
+  // looked up for all together: a look-up per row would wait for memory row after row)
+  int* list = p.top_k <= kBins ? bins : out;
   const unsigned below = (1u << lane) - 1u;
   int placed = 0, tied = 0;     // over the sweeps so far: pages above the threshold (or kept), pages on it
   for (int sweep = 0; sweep < pages; sweep += kSweep) {
@@ -243,12 +246,14 @@ pa_block_select_kernel(const __grid_constant__ BlockSelectParams p) {
       const int rank_equal = ties_before + __popc(is_equal & below);
       if (((is_above >> lane) & 1u) || (((is_equal >> lane) & 1u) && rank_equal < ties)) {
         const int place = before + __popc(is_above & below) + min(rank_equal, ties);
-        if (place < p.top_k) out[place] = __ldg(table + page_of(sweep, j));
+        if (place < p.top_k) list[place] = page_of(sweep, j);
       }
       before += __popc(is_above);
       ties_before += __popc(is_equal);
     }
   }
+  __syncthreads();
+  for (int i = tid; i < p.top_k; i += THREADS) out[i] = __ldg(table + list[i]);
 }
 
 }  // namespace pa

@@ -169,7 +169,7 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     the context (0 where a sequence has fewer pages) and int32 ``[num_seqs]``, the tokens in one
     such table -- what ``paged_attention_decode`` takes as ``block_tables`` and ``sequence_lengths``.
     The first ``keep_first`` and the last ``keep_last`` pages are always among them; the others go by
-    ``scores`` (fp32 ``[num_seqs, num_kv_heads, max_blocks]``), NaN lowest, ties to the lower place.
+    ``scores`` (fp32 ``[num_seqs, num_kv_heads, max_blocks]``), NaN as -inf, ties to the lower place.
     With several query tokens ``keep_last`` has to cover the last ``query_len`` tokens: 2.
     """
     dev, on = scores.device, scores.get_device()
