@@ -560,6 +560,23 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
   static_assert(!FUSE || (QR <= 8 && !ALIBI && !TRACE), "the single-launch form exists for 4- and 8-row items");
   static_assert(!PAIR || (!FUSE && !ALIBI && !TRACE), "the PAIR form is plain");
   static_assert(!BLK || (!PER_TOKEN && !FUSE && !PAIR && !TRACE), "block scales exist in the two-launch form");
+  // Pages of 64 tokens, keys: copied to [chunk][256 tok][16 B], an item is 32 runs of 1 KB, and an SM gets through
+  // a bulk copy only every 75-90 cycles -- more than HBM needs for the item (88 us for 27 sequences of 8 192
+  // tokens, 8 kv heads and 16 rows, whichever warps issue them; 77 with a quarter of the copies).  Here a page is ONE copy of 8 KB, as it
+  // lies in the cache: [chunk][64 tok][16 B].  An M = 128 instruction on it multiplies the page's 64 tokens in its
+  // upper 64 rows and, in the lower 64, the bytes 1 KB on, which are another chunk's.  So every page has an
+  // instruction of its own: an even page's starts at the page and its results are the rows 0-63; an odd page's
+  // starts 1 KB before the page and its results are the rows 64-127; each into its own columns, where the warps of
+  // the other 64 lanes never look.  With 16 rows, where hi and lo are products of their own, the doubled count would
+  // keep the issuing warp and the tensor core busier than HBM is (91 us): there hi and lo are the two halves of one
+  // N = 32 product again and are added in registers.
+  constexpr bool kWholePage = BLK && BS == 64;
+  constexpr bool kWide = kWholePage && QR == 16;
+  constexpr int kNS = kWide ? 2 * QR : acc_n(QR);                          // MMA N and TMEM columns of an S^T tile
+  constexpr int kSCols = kWholePage ? 4 * kNS : 2 * kNS;                   // TMEM columns of a group: S^T tiles,
+  constexpr int kGroupCols = kSCols + 2 * acc_n(QR);                       // then O^T (parity 0 | 1)
+  constexpr int kTmemCols = kGroupCols * kNG <= 256 ? 256 : 512;
+  static_assert(kTmemCols == tmem_cols(QR) || kWholePage, "the usual layout");
   constexpr bool kFinished = ALIBI || BLK;   // the logits that the maxima are taken of are complete (factor and per-token term applied)
   constexpr int NG = kNG;
   constexpr bool kSum = sums_in_tensor_core(QR);   // hi and lo products summed by the tensor core
@@ -619,7 +636,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
   // row r = t * G + g of a kv head sees token j iff j < ctx - (L - 1 - t)
   // (padding rows of the last row block see nothing)
   for (int r = tid; r < 64; r += (int)blockDim.x) row_lim[r] = r < p.eqG ? (p.L - 1 - r / p.G) : 0x7fffffff;
-  if (warp == kWarpMma) tmem_alloc(sbase + kOffTmemPtr, tmem_cols(QR));
+  if (warp == kWarpMma) tmem_alloc(sbase + kOffTmemPtr, kTmemCols);
   // Everything above touches this CTA's shared and tensor memory only and may run while the
   // kernel before this one in the stream drains.
   //
@@ -738,7 +755,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
     const bool vt = BS != 16 && is_v && p.v_trans != 0;
     auto my_page = [&]() -> int {
       if (BS == 16) return lane;
-      if (BS == 64) return is_v ? (vt ? (lane >> 2) : lane) : (lane >> 3);
+      if (BS == 64) return is_v ? (vt ? (lane >> 2) : lane) : (kWholePage ? lane : (lane >> 3));
       return 0;
     };
     auto load_page_id = [&](const TcItem& it) -> int {
@@ -789,6 +806,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         __syncwarp();
         if (is_v) {          // one swizzled box [128 d][64 tok] per page
           if (lane < npg) tma_load_4d(dst + lane * G::kVBox, &vmap, 0, 0, it.head, pid, full, pol);
+        } else if (kWholePage) {
+          if (lane < npg) bulk_g2s(dst + lane * 8192, src, 8192, full, pol);
         } else {             // (page, chunk) run of 64 tok x 16 B -> [chunk][256 tok][16 B]
           const int pg = lane >> 3, c = lane & 7;
           if (pg < npg) bulk_g2s(dst + c * 4096 + pg * 1024, src + c * 1024, 1024, full, pol);
@@ -1047,7 +1066,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
     }
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------------ MMA issue
-    constexpr uint32_t kIdesc = idesc_f32acc(128, N, 0, 0);
+    constexpr uint32_t kIdesc = idesc_f32acc(128, kNS, 0, 0);
     constexpr uint32_t kIdescPV = idesc_f32acc(128, N, 0, 0, true);   // P^T is MN-major
     const bool leader = elect_one();  // the one lane that issues every MMA and commit
     // per item i: group g = i % NG, use gu = i / NG of the group's buffers, O^T parity gu & 1.
@@ -1065,18 +1084,19 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
             !wait(bar(kBarQFull, qslot), (uint32_t)(i / kQSlots) & 1)) { fail(); break; }
         stamp(3, i, 1);
         fence_after_sync();
-        const uint64_t kd = smem_desc(k_ring + slot * kHalfSlot, G::kKLbo, G::kKSbo);
+        const uint64_t kd = smem_desc(k_ring + slot * kHalfSlot, kWholePage ? 1024 : G::kKLbo, G::kKSbo);
         const uint32_t tslot = lds32(q_ring + qslot * kQSlotBytes + kQTile + kQHdr);  // slot of the item's tile
         const uint64_t qd = smem_desc(q_ring + tslot * kQSlotBytes, 128, 1024);
-        const uint32_t d0 = tmem_base + g * 4 * N;
+        const uint32_t d0 = tmem_base + g * kGroupCols;
 #pragma unroll
-        for (int tg = 0; tg < 2; ++tg) {
+        for (int tg = 0; tg < (kWholePage ? 4 : 2); ++tg) {   // (whole pages: tg counts the pages)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint64_t ad = kd + (uint64_t)((2 * j * G::kKLbo + tg * G::kKTile1) >> 4);
+            const uint64_t ad = kd + (uint64_t)((kWholePage ? 2 * j * 1024 + tg * 8192 - (tg & 1) * 1024
+                                                            : 2 * j * G::kKLbo + tg * G::kKTile1) >> 4);
             const uint64_t bd = qd + (uint64_t)(((2 * j) * 128) >> 4);
-            if (leader) mma_f8_ss(d0 + tg * N, ad, bd, kIdesc, j > 0);
-            if (kSum && leader) mma_f8_ss(d0 + tg * N, ad, bd + (uint64_t)((QR / 8 * 1024) >> 4), kIdesc, true);   // the lo rows' tile
+            if (leader) mma_f8_ss(d0 + tg * kNS, ad, bd, kIdesc, j > 0);
+            if (kSum && !kWide && leader) mma_f8_ss(d0 + tg * kNS, ad, bd + (uint64_t)((QR / 8 * 1024) >> 4), kIdesc, true);   // the lo rows' tile
           }
         }
         if (leader) mma_commit(bar(kBarSFull, g));
@@ -1096,7 +1116,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         const uint64_t vd = v16 ? smem_desc(v_ring + vslot * kHalfSlot, 2048, 128)
                                 : smem_desc_swizzled(v_ring + vslot * kHalfSlot, G::kVSpan);
         const uint64_t pd = smem_desc(p_tiles + g * kPTile, kPLbo, kPSbo);
-        const uint32_t d0 = tmem_base + g * 4 * N + 2 * N + (int)(gu & 1) * N;
+        const uint32_t d0 = tmem_base + g * kGroupCols + kSCols + (int)(gu & 1) * N;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint64_t ad = vd + (uint64_t)((v16 ? Geo<16>::v_kstep(ks) : G::v_kstep(ks)) >> 4);
@@ -1118,7 +1138,9 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
     const int wq = warp & 3;              // TMEM lane quarter this warp may touch
     const int r = wq * 32 + lane;         // TMEM lane: S^T row (token slot) / O^T row (head dim)
     const int bar_a = 1 + grp, bar_b = 5 + grp;  // named barriers of the group
-    const uint32_t tmem_grp = tmem_base + ((uint32_t)(wq * 32) << 16) + grp * 4 * N;
+    const uint32_t tmem_grp = tmem_base + ((uint32_t)(wq * 32) << 16) + grp * kGroupCols;
+    // S^T tile of this lane's token tg (whole pages: the lower and the upper 64 lanes have their own columns)
+    const uint32_t s_tile[2] = {tmem_grp + (kWholePage ? (wq >> 1) * kNS : 0), tmem_grp + (kWholePage ? (2 + (wq >> 1)) * kNS : N)};
     // (the per-tensor key scale is part of the row factors the query producer writes)
     float v_scale_t = 1.0f;
     if (!PER_TOKEN && p.kv_quant_mode == PA_QUANT_PER_TENSOR) v_scale_t = __ldg(p.v_scale);
@@ -1274,8 +1296,12 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
       // finished logits.)
       auto raw_logits = [&](int ch, float (&s)[2][RC]) {
         uint32_t h[2][8], l[2][8];
-        load_rows(tmem_grp, ch, h[0], l[0]);
-        load_rows(tmem_grp + N, ch, h[1], l[1]);
+        load_rows(s_tile[0], ch, h[0], l[0]);
+        load_rows(s_tile[1], ch, h[1], l[1]);
+        if (kWide) {
+          tmem_ld8(s_tile[0] + QR + ch * 8, l[0]);
+          tmem_ld8(s_tile[1] + QR + ch * 8, l[1]);
+        }
         if (NCH > 1) load_row_consts(ch);
         tmem_ld_wait();
 #pragma unroll
@@ -1283,6 +1309,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
 #pragma unroll
           for (int q = 0; q < RC; ++q) {
             float v = row_value(h[tg], l[tg], q);
+            if (kWide) v += __uint_as_float(l[tg][q]);
             if (PER_TOKEN) v *= ks_tok[tg];
             if (BLK) v = fmaf(v * ks_blk[tg], row_scale[q], ALIBI ? fmaf(slope[q], rel_pos[tg], lv_blk[tg]) : lv_blk[tg]);
             else if (ALIBI) v = fmaf(v, row_scale[q], slope[q] * rel_pos[tg]);
@@ -1299,8 +1326,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
         // 16-row items: both chunks do not fit in registers, so the finished (scaled, masked) logits
         // go back into the accumulator columns they came from, and pass 2 reads them as they are
         if constexpr (kKeepInTmem) {
-          tmem_st8(tmem_grp + ch * 8, s_keep[0]);
-          tmem_st8(tmem_grp + N + ch * 8, s_keep[1]);
+          tmem_st8(s_tile[0] + ch * 8, s_keep[0]);
+          tmem_st8(s_tile[1] + ch * 8, s_keep[1]);
         }
         float mx[RC];
 #pragma unroll
@@ -1363,8 +1390,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
       for (int ch = 0; ch < NCH; ++ch) {
         if constexpr (kKeepInTmem) {
           uint32_t a[8], b[8];
-          tmem_ld8(tmem_grp + ch * 8, a);
-          tmem_ld8(tmem_grp + N + ch * 8, b);
+          tmem_ld8(s_tile[0] + ch * 8, a);
+          tmem_ld8(s_tile[1] + ch * 8, b);
           load_row_consts(ch);
           tmem_ld_wait();
 #pragma unroll
@@ -1611,7 +1638,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
                             (int64_t)it.head * p.tmp_stride_head + (int64_t)it.part * p.tmp_stride_part +
                             (int64_t)(it.rb * QR) * p.tmp_stride_row + r;
       const int64_t row_stride = p.tmp_stride_row;
-      const uint32_t otile = tmem_grp + 2 * N + (int)(gu & 1) * N;
+      const uint32_t otile = tmem_grp + kSCols + (int)(gu & 1) * N;
 #pragma unroll 1
       for (int ch = 0; ch < NCH; ++ch) {
         uint32_t h[8], l[8];
@@ -1717,7 +1744,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
     p.trace[(7 * 64 + 60) * 4 + 3] = (unsigned long long)clock64();
   if (warp == kWarpMma) {
     fence_after_sync();
-    tmem_dealloc(tmem_base, tmem_cols(QR));
+    tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
