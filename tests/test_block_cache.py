@@ -353,6 +353,53 @@ def test_bad_tables_and_lengths_are_reported():
     assert_attention(got[1:], tuple(t[1:] for t in want))
 
 
+@pytest.mark.gpu
+def test_a_single_value_is_a_scale_per_tensor():
+    """Scales of shape [1, 1, 1, 1] mean what they always did, for every cache the operator takes."""
+    g = torch.Generator().manual_seed(3)
+    kc, vc = torch.randn(9, 2, 16, 16, 8, generator=g).bfloat16().cuda(), torch.randn(9, 2, D, 16, generator=g).bfloat16().cuda()
+    q = torch.randn(1, 8, D, generator=g).bfloat16().cuda()
+    tables, lengths = torch.arange(9).int()[None].cuda(), torch.tensor([140], dtype=torch.int32).cuda()
+    outs = []
+    for shape in ((), (1, 1, 1, 1)):
+        out = torch.empty_like(q)
+        ks, vs = torch.full(shape, 0.5, device="cuda"), torch.full(shape, 2.0, device="cuda")
+        pa.paged_attention_decode(out, q, kc, vc, lengths, tables, SCALE, 1, 144, torch.bfloat16, None, ks, vs)
+        outs.append(out)
+    assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    """No sequences, no tokens: nothing happens and nothing is refused."""
+    c = Cache([40], 2, 16)
+    empty = torch.zeros(0, c.width, dtype=torch.int32).cuda()
+    none = torch.zeros(0, dtype=torch.int32).cuda()
+    kc, vc, ks, vs, bounds = cuda(c.key, c.value, c.ks, c.vs, c.bounds())
+    q = torch.zeros(0, 8, D, dtype=torch.bfloat16, device="cuda")
+    res = pa.sparse_attention_decode(torch.empty_like(q), q, kc, vc, bounds, none, empty, SCALE, 1, 4, None, ks, vs)
+    assert res["block_tables"].shape == (0, 2, 4) and res["sequence_lengths"].shape == (0,)
+    pa.paged_attention_decode(torch.empty_like(q), q, kc, vc, none, empty, SCALE, 1, 16, torch.bfloat16, None, ks, vs)
+    rows = torch.zeros(0, 2, D, dtype=torch.bfloat16, device="cuda")
+    pa.append_kv_cache(rows, rows, kc, vc, ks, vs, empty, none, torch.zeros(1, dtype=torch.int32).cuda(), key_bounds=bounds)
+    pa.append_kv_cache(rows, rows, kc, vc, ks, vs, c.tables.cuda(), c.lengths.cuda(), torch.zeros(2, dtype=torch.int32).cuda())
+    assert_same([t.cpu() for t in (kc, vc, ks, vs, bounds)], [c.key, c.value, c.ks, c.vs, c.bounds()])
+
+
+@pytest.mark.gpu
+def test_query_and_output_views():
+    """Rows that begin anywhere, sequences further apart than their rows are long."""
+    c = Cache([300, 40], 2, 16, seed=17)
+    wide = torch.randn(2, 13, D + 3, generator=c.g).bfloat16()
+    dev = wide.cuda()
+    room = torch.full((2, 11, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    pa.paged_attention_decode(room[:, 2:10], dev[:, 1:9, 3:], *cuda(c.key, c.value, c.lengths, c.tables), SCALE, 1, 300,
+                              torch.bfloat16, None, *cuda(c.ks, c.vs))
+    want = bo.attention(wide[:, 1:9, 3:], c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1)
+    assert_attention(room[:, 2:10].cpu(), want)
+    assert bool((room[:, :2] == 7).all()) and bool((room[:, 10:] == 7).all())
+
+
 # ----------------------------------------------------------------------------- GPU: tables per kv head
 @pytest.mark.gpu
 @pytest.mark.parametrize("bs", [16, 64])
@@ -493,6 +540,35 @@ def test_scores_of_many_short_sequences():
     assert ((got.double() - want).abs()[live] <= (260 * 2.0 ** -23) * terms[live]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hkv,group", [(1, 4), (2, 4), (3, 20), (1, 64), (8, 4)])
+def test_scores_of_long_contexts_are_the_same_every_time(hkv, group):
+    """Many tiles for every SM, few kv heads: rings whose slots pass between warps."""
+    g = torch.Generator().manual_seed(hkv)
+    lengths = torch.tensor([60000, 31, 45001, 70000], dtype=torch.int32)
+    width, nb = 4375, 11000
+    tables = torch.randint(0, nb, (4, width), generator=g, dtype=torch.int32)
+    bounds = random_codes((nb, hkv, 2, D), g).float().sort(2).values.to(FP8)
+    ks = torch.exp2(torch.randint(-6, -2, (nb, hkv, 1, 1), generator=g).float())
+    q = torch.randn(4, hkv * group, D, generator=g).bfloat16()
+    dev = cuda(q, bounds, lengths, tables)
+    first = pa.score_blocks(*dev, SCALE, 1, 16, key_scale=ks.cuda())
+    for _ in range(20):
+        assert torch.equal(pa.score_blocks(*dev, SCALE, 1, 16, key_scale=ks.cuda()), first)
+    # against 64 bits on the GPU, sequence by sequence
+    for s in range(4):
+        pages = -(-int(lengths[s]) // 16)
+        ids = tables[s, :pages].long().cuda()
+        b, k = dev[1].float().double()[ids], ks.cuda().double()[ids, :, 0, 0].T
+        for h in range(hkv):
+            rows = q[s, h * group:(h + 1) * group].cuda().double()
+            lo, hi = b[:, h, 0], b[:, h, 1]
+            u = rows.clamp_min(0) @ hi.T + rows.clamp_max(0) @ lo.T
+            terms = rows.clamp_min(0) @ hi.abs().T + rows.clamp_max(0).abs() @ lo.abs().T
+            want, slack = u.amax(0) * SCALE * k[h], terms.amax(0) * SCALE * k[h] * 260 * 2.0 ** -23
+            assert bool(((first[s, h, :pages].double() - want).abs() <= slack).all())
+
+
 # ----------------------------------------------------------------------------- GPU: selection
 def run_select(score, lengths, tables, bs, k, **kw):
     got = pa.select_blocks(*cuda(score, lengths, tables), bs, k, **kw)
@@ -501,7 +577,7 @@ def run_select(score, lengths, tables, bs, k, **kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("values", ["normal", "ties", "one value", "nan", "infinite", "tiny", "wide"])
-@pytest.mark.parametrize("width,top_k", [(3, 2), (40, 7), (300, 64), (600, 2), (2100, 700), (9000, 33)])
+@pytest.mark.parametrize("width,top_k", [(3, 2), (5, 40), (40, 7), (300, 64), (600, 2), (2100, 700), (9000, 33), (9000, 3000)])
 def test_selection(width, top_k, values):
     g = torch.Generator().manual_seed(width)
     pages = [width, max(1, width // 2), 1, 0, min(top_k, width), min(top_k + 1, width)]

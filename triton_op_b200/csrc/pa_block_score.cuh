@@ -57,7 +57,10 @@ struct BlockScoreParams {
   int32_t S, Hkv, rows, block_size, num_blocks, width;
   int32_t q_is_fp8, q_quant_mode;
   int32_t heads_per_cta;       // a power of two that divides kScoreWarps
-  int32_t slots;               // ring depth in tiles, more than kScoreWarps / heads_per_cta
+  // Ring depth in tiles, a multiple of kScoreWarps / heads_per_cta: a slot then holds tiles of the same warps
+  // (and, where those are not all, of the same producer) every time, so nobody waits for a phase of its
+  // barriers that is not the next one.
+  int32_t slots;
   int32_t off_index, off_ring; // shared-memory carve: query rows and factors, index of the sequences, ring
   int64_t q_stride_seq;        // bytes
   int64_t bounds_stride_block, bounds_stride_head;   // bytes
@@ -263,6 +266,7 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   int k = 0;                          // tiles of the CTA before the segment
   int mine = sub, slot = sub;         // this warp's next tile and its slot
   uint32_t phase = 0;
+  bool dead = false;                  // a wait ran out: go through the barriers, touch nothing
   while (k < n_tiles) {
     // a segment: tiles of one sequence and head group
     const int seq = a.seq, tile_a = a.tile;
@@ -368,11 +372,11 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
     float* out = p.scores + (int64_t)seq * p.out_stride_seq + (int64_t)(head0 + my_head) * p.out_stride_head;
 #pragma unroll 1
     while (mine < k + count) {
-      if (!__all_sync(kFullMask, mbar_wait(smem_addr(&bar_full[slot]), phase))) {
+      if (!dead && !__all_sync(kFullMask, mbar_wait(smem_addr(&bar_full[slot]), phase))) {
         if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_WAIT_TIMEOUT);
-        return;
+        dead = true;
       }
-      if (my_head < heads) {
+      if (my_head < heads && !dead) {
         const uint32_t tile = ring + slot * slot_bytes;
         const uint32_t row0 = tile + g * pitch + my_head * 2 * kD + t * 16, row1 = row0 + 8 * pitch;
         float acc[2][NB8][4];   // the two halves of the bound: two chains of products

@@ -187,7 +187,9 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
   int64_t slots = ((int64_t)dev->max_smem_optin - 1024 - off_ring) / slot;   // (1 KB: the kernel's barriers)
   if (slots > pa::kScoreRingBytes / slot) slots = pa::kScoreRingBytes / slot;
   if (slots > pa::kScoreMaxSlots) slots = pa::kScoreMaxSlots;
-  if (slots <= pa::kScoreWarps / heads || slots < pa::kScoreProducers) return PA_ERR_TOO_LARGE;   // the index of the sequences leaves no room
+  const int step = pa::kScoreWarps / heads;
+  slots -= slots % step;
+  if (slots < step || slots < pa::kScoreProducers) return PA_ERR_TOO_LARGE;   // the index of the sequences leaves no room
   k.off_ring = (int)off_ring;
   k.slots = (int)slots;
   const int64_t smem = off_ring + slots * slot;

@@ -151,7 +151,8 @@ def _by_block(key_scale, value_scale, block_tables) -> bool:
     for the next one (no cached parameters, workspaces of the call's own)."""
     if isinstance(block_tables, torch.Tensor) and block_tables.dim() == 3:
         return True
-    return any(isinstance(s, torch.Tensor) and s.dim() == 4 and s.shape[2] == 1 for s in (key_scale, value_scale))
+    return any(isinstance(s, torch.Tensor) and s.dim() == 4 and s.shape[2] == 1 and s.numel() > 1   # (one value is per tensor)
+               for s in (key_scale, value_scale))
 
 
 _PARAM_CACHE: Dict[tuple, PaDecodeParams] = {}
@@ -502,8 +503,8 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
     k_stride, v_stride = key_cache.stride(), value_cache.stride()
     if o_stride[2] != 1:
         _fail("output's last dim must be contiguous")
-    if q_stride[2] != 1 or q_stride[1] != head_size:
-        query = query.contiguous()
+    if (q_stride[2] != 1 or q_stride[1] != head_size or q_stride[0] % 16 or query.data_ptr() % 16):
+        query = query.clone(memory_format=torch.contiguous_format)
         q_stride = query.stride()
     # (the common layouts first; _inner_contiguous knows all)
     if not ((k_stride[4] == 1 and k_stride[3] == 16 and k_stride[2] == 16 * bs) or _inner_contiguous(key_cache, 2)) or not (
@@ -684,7 +685,8 @@ def paged_attention_decode(
                 alibi_slopes, sink_tokens, status)
             if not output.is_cuda:
                 raise RuntimeError("paged_attention_decode runs on CUDA tensors only; there is no CPU fallback")
-            _lib.launch(output.get_device(), _lib.lib().pa_decode_tables_sm100, "pa_decode_tables_sm100", C.byref(p), head_stride)
+            if output.numel() > 0:
+                _lib.launch(output.get_device(), _lib.lib().pa_decode_tables_sm100, "pa_decode_tables_sm100", C.byref(p), head_stride)
             return {"triton_decode_time": 0.0, "triton_reduce_time": 0.0, "temporary_output": ws[2],
                     "final_output": output, "exponential_sums": ws[0], "maximum_logits": ws[1],
                     "total_triton_time": 0.0, "partition_size": SEQUENCE_PARTITION_SIZE}

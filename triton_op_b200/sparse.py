@@ -236,7 +236,7 @@ def sparse_attention_decode(output: torch.Tensor, query: torch.Tensor, key_cache
     tables, lengths = select_blocks(scores, sequence_lengths, block_tables, block_size, top_k, keep_first=keep_first,
                                     keep_last=keep_last, status=status)
     res = paged_attention_decode(output, query, key_cache, value_cache, lengths, tables, softmax_scale,
-                                 query_sequence_length, top_k * block_size, torch.bfloat16, query_scale, key_scale,
+                                 query_sequence_length, min(top_k, block_tables.shape[1]) * block_size, torch.bfloat16, query_scale, key_scale,
                                  value_scale, sink_tokens=sink_tokens, status=status)
     res["block_tables"], res["sequence_lengths"] = tables, lengths
     return res
