@@ -678,6 +678,21 @@ def test_append(bs, counts, before, layout):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 64, 1024])
+@pytest.mark.parametrize("hkv,counts,before", [(1, [1500, 700], [900, 0]), (2, [64] * 40, [1000] * 40), (4, [3000], [5]), (1, [300, 0, 2], [1020, 8, 5])])
+def test_append_of_prompts(bs, hkv, counts, before):
+    """Many rows for few pages, and for many: each way of dividing a page's rows over warps and CTAs."""
+    c = Cache([a + b for a, b in zip(before, counts)], hkv, bs, seed=len(counts))
+    start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32)
+    n = sum(counts)
+    key, value = torch.randn(n, hkv, D, generator=c.g).bfloat16() * 3, torch.randn(n, hkv, D, generator=c.g).bfloat16()
+    key[n // 2, 0, 17] = 4000.0                  # one page that has to grow far
+    got, want, status = append_both(c, key, value, c.lengths, start, c.bounds())
+    assert status == 0
+    assert_same(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bs", [16, 64])
 def test_append_token_by_token_grows_pages(bs):
     """Tokens that get larger and larger: each page's scale grows again and again."""

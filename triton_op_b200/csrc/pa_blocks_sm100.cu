@@ -22,17 +22,20 @@ inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uint
 // Launch as a programmatic dependent of the kernel before it in the stream; the kernels here wait
 // (griddepcontrol.wait) before they touch global memory.
 template <typename P>
-int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t stream, const P& params) {
+int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t stream, const P& params, int cluster = 1) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? PA_OK : cuda_fail(e);
@@ -103,18 +106,27 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   int64_t pages = (int64_t)p->num_tokens / p->block_size + 2 * (int64_t)p->num_seqs;
   if (pages > p->num_tokens) pages = p->num_tokens;
   const int64_t units = pages * p->num_kv_heads * 2;
-  const int per_cta = p->block_size == 16 ? 4 : 1;
-  const int threads = p->block_size == 1024 ? 512 : 128;
-  int64_t grid = (units + per_cta - 1) / per_cta;
   if (units > (1 << 30)) return PA_ERR_TOO_LARGE;
-  const int64_t cap = (int64_t)dev->sm_count * (p->block_size == 1024 ? 1 : 5);   // what is resident at a time
-  if (grid > cap) grid = cap;
   const size_t smem = (size_t)(p->num_seqs + 1) * 4;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Pages of 1024 tokens that get many rows at a time (64 or more per sequence, on average): sixteen warps a
+  // page, or, while all pages find room at once that way, a cluster of eight CTAs.
+  if (p->block_size == 1024 && p->num_tokens >= 64 * (int64_t)p->num_seqs) {
+    constexpr int kCluster = 8;
+    if (units <= 2 * dev->sm_count / kCluster)   // (two of its CTAs fit an SM)
+      return launch(blk ? pa::pa_cache_append_kernel<1024, 64, true, kCluster> : pa::pa_cache_append_kernel<1024, 64, false, kCluster>,
+                    dim3((unsigned)(units * kCluster)), 256, smem, st, k, kCluster);
+    const int64_t grid = units < dev->sm_count ? units : dev->sm_count;
+    return launch(blk ? pa::pa_cache_append_kernel<1024, 16, true> : pa::pa_cache_append_kernel<1024, 16, false>, dim3((unsigned)grid), 512, smem, st, k);
+  }
+  const int per_cta = p->block_size == 16 ? 4 : 1;
+  int64_t grid = (units + per_cta - 1) / per_cta;
+  const int64_t cap = (int64_t)dev->sm_count * 5;   // what is resident at a time
+  if (grid > cap) grid = cap;
   switch (p->block_size) {
-    case 16: return launch(blk ? pa::pa_cache_append_kernel<16, 1, true> : pa::pa_cache_append_kernel<16, 1, false>, dim3((unsigned)grid), threads, smem, st, k);
-    case 64: return launch(blk ? pa::pa_cache_append_kernel<64, 4, true> : pa::pa_cache_append_kernel<64, 4, false>, dim3((unsigned)grid), threads, smem, st, k);
-    default: return launch(blk ? pa::pa_cache_append_kernel<1024, 16, true> : pa::pa_cache_append_kernel<1024, 16, false>, dim3((unsigned)grid), threads, smem, st, k);
+    case 16: return launch(blk ? pa::pa_cache_append_kernel<16, 1, true> : pa::pa_cache_append_kernel<16, 1, false>, dim3((unsigned)grid), 128, smem, st, k);
+    case 64: return launch(blk ? pa::pa_cache_append_kernel<64, 4, true> : pa::pa_cache_append_kernel<64, 4, false>, dim3((unsigned)grid), 128, smem, st, k);
+    default: return launch(blk ? pa::pa_cache_append_kernel<1024, 4, true> : pa::pa_cache_append_kernel<1024, 4, false>, dim3((unsigned)grid), 128, smem, st, k);
   }
 }
 

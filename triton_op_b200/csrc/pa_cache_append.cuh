@@ -18,12 +18,18 @@
 // A unit of work is (page, kv head, key or value), and all of it belongs to one group of warps: the
 // scale is a maximum over every row the page gets, and two writers of one page would race on it.
 // Each warp takes 16 consecutive slots of the page, whose rows stay in registers between the
-// maximum and the store (pages of 1024 tokens: four such runs per warp, read twice).  Keys are
+// maximum and the store.  A page of 1024 tokens is 64 such runs.  Sixteen warps take four each and read
+// the rows twice; where there are fewer pages than could keep the GPU busy that way, a page is shared by
+// a cluster of eight CTAs that find the maximum through each other's shared memory (9 us against 17 for
+// two prompts of 2 200 and 3 300 tokens, one kv head; for many pages the clusters' barriers cost more than they save);
+// with a few rows per sequence, where most warps would have nothing to do, four warps take the runs in turn.  Keys are
 // stored as 16-byte chunks [d/16][token][16], values as 16 tokens of a head dim, 16 bytes too;
 // values of a run that is not whole are merged with the bytes that are there.
 // What bounds it: 512 bytes read and 256 written per (token, kv head) -- HBM for a prompt; a decode
 // step of a few hundred rows is launch latency and one chain of loads.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "../../include/pa_decode_sm100.h"
 #include "pa_common.cuh"
@@ -148,20 +154,24 @@ static __device__ __noinline__ void rescale_runs(uint8_t* cache, bool is_v, bool
 }
 
 // BS: tokens per page.  WPU: warps per unit.  PER_BLOCK: scales per (page, kv head), else per tensor.
-template <int BS, int WPU, bool PER_BLOCK>
-__global__ void __launch_bounds__(WPU > 4 ? WPU * 32 : 128, WPU > 4 ? 1 : 5)
+// CLUSTER: CTAs that share a unit.
+template <int BS, int WPU, bool PER_BLOCK, int CLUSTER = 1>
+__global__ void __launch_bounds__(WPU / CLUSTER > 4 ? WPU / CLUSTER * 32 : 128, CLUSTER > 1 ? 2 : (WPU > 4 ? 1 : 5))
 pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
-  constexpr int kThreads = WPU > 4 ? WPU * 32 : 128;
-  constexpr int kUnits = kThreads / 32 / WPU;                       // units a CTA works on at a time
+  constexpr int kCtaWarps = WPU / CLUSTER;                          // warps of a unit in one CTA
+  constexpr int kThreads = kCtaWarps > 4 ? kCtaWarps * 32 : 128;
+  constexpr int kUnits = CLUSTER > 1 ? 1 : kThreads / 32 / WPU;     // units a CTA (or cluster) works on at a time
   constexpr int kRuns = BS / 16;                                    // 16-slot runs of a page
   constexpr int kPerWarp = (kRuns + WPU - 1) / WPU;                 // ... that a warp takes
   extern __shared__ int index_smem[];
   int* unit_off = index_smem;          // [S + 1] pages touched before each sequence
   __shared__ int scan[32];
   __shared__ uint32_t red_max[kThreads / 32];
-  __shared__ uint32_t red_lo[WPU > 1 ? WPU : 1][64], red_hi[WPU > 1 ? WPU : 1][64];
+  __shared__ uint32_t red_lo[kCtaWarps][64], red_hi[kCtaWarps][64];
+  __shared__ uint32_t cta_max, cta_lo[64], cta_hi[64];              // CLUSTER: this CTA's share
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int sub = warp % WPU;          // warp inside its unit
+  const int team = (int)blockIdx.x / CLUSTER, teams = (int)gridDim.x / CLUSTER, rank = (int)blockIdx.x - team * CLUSTER;
+  const int sub = CLUSTER > 1 ? rank * kCtaWarps + warp : warp % WPU;   // warp inside its unit
 
   grid_dependency_wait();
   // rows of a sequence: [first row, count), and its first new token's position
@@ -247,8 +257,9 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     n.row0 = row + (page * BS + n.o0 - pos);
     return n;
   };
-  Unit next = decode(blockIdx.x * kUnits + warp / WPU);
-  for (uint32_t u0 = blockIdx.x * kUnits; u0 < units; u0 += gridDim.x * kUnits) {
+  const uint32_t in_team = CLUSTER > 1 ? 0u : (uint32_t)(warp / WPU);
+  Unit next = decode(team * kUnits + in_team);
+  for (uint32_t u0 = team * kUnits; u0 < units; u0 += teams * kUnits) {
     const Unit cur = next;
     bool live = cur.live;
     const bool is_v = cur.is_v;
@@ -289,7 +300,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
       loaded = mine(0);
       load_run(loaded);
     }
-    next = decode(u0 + gridDim.x * kUnits + warp / WPU);
+    next = decode(u0 + teams * kUnits + in_team);
     int blk = cur.blk;
     if ((unsigned)blk >= (unsigned)p.num_blocks) {
       if (live && lane == 0 && p.status) atomicOr(p.status, PA_DEV_BAD_PAGE_ID);
@@ -366,20 +377,43 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
         }
       }
     }
-    if (WPU > 1) {   // over the warps of the unit (a CTA then has one unit)
+    if (WPU > 1) {   // over the warps of the unit (a CTA, or a cluster, then has one unit)
       if (lane == 0) red_max[warp] = top1;
       if (want_bounds && f == 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) red_lo[sub][c * 8 + e] = lo8[e], red_hi[sub][c * 8 + e] = hi8[e];
+        for (int e = 0; e < 8; ++e) red_lo[warp % kCtaWarps][c * 8 + e] = lo8[e], red_hi[warp % kCtaWarps][c * 8 + e] = hi8[e];
       }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WPU; ++w) top1 = max(top1, red_max[w]);
-      if (want_bounds && sub == 0) {
+      for (int w = 0; w < kCtaWarps; ++w) top1 = max(top1, red_max[w]);
+      if (want_bounds && warp == 0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
 #pragma unroll 1
-          for (int w = 0; w < WPU; ++w) lo8[e] = bf16x2_min(lo8[e], red_lo[w][c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], red_hi[w][c * 8 + e]);
+          for (int w = 0; w < kCtaWarps; ++w) lo8[e] = bf16x2_min(lo8[e], red_lo[w][c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], red_hi[w][c * 8 + e]);
+        }
+      }
+      if constexpr (CLUSTER > 1) {
+        namespace cg = cooperative_groups;
+        const cg::cluster_group cluster = cg::this_cluster();
+        if (warp == 0) {
+          if (lane == 0) cta_max = top1;
+          if (want_bounds && f == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) cta_lo[c * 8 + e] = lo8[e], cta_hi[c * 8 + e] = hi8[e];
+          }
+        }
+        cluster.sync();
+        const uint32_t theirs = lane < CLUSTER ? *cluster.map_shared_rank(&cta_max, lane) : 0u;
+        top1 = __reduce_max_sync(kFullMask, theirs);
+        if (want_bounds && sub == 0) {
+#pragma unroll 1
+          for (int r = 1; r < CLUSTER; ++r) {
+            const uint32_t* lo = cluster.map_shared_rank(cta_lo, r);
+            const uint32_t* hi = cluster.map_shared_rank(cta_hi, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], lo[c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], hi[c * 8 + e]);
+          }
         }
       }
     }
@@ -478,7 +512,9 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     // warp, by the lanes above): the new one may go there
     __syncwarp();
     if (PER_BLOCK && live && o1 > o0 && sub == 0 && lane == 0) *scale_at = scale;
-    if (WPU > 1) __syncthreads();   // the reduction buffers are free for the next unit
+    // the reduction buffers are free for the next unit (and nobody leaves while they may be read)
+    if constexpr (CLUSTER > 1) cooperative_groups::this_cluster().sync();
+    else if (WPU > 1) __syncthreads();
   }
 }
 
