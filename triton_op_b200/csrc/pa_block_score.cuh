@@ -13,7 +13,7 @@
 // operations: HBM for the query groups of a decode step.  One CTA per SM takes an equal share of all
 // tiles (16 pages of up to eight kv heads) of the batch, whatever the sequences' lengths; a
 // pair of producer warps runs through them with bulk copies -- a page's heads are one run of up to 2 KB -- into
-// a ring of about 170 KB, and eight warps multiply, one kv head (or every so many tiles) each.
+// a ring of about 170 KB, and eight or sixteen warps multiply, one kv head (or every so many tiles) each.
 // (With a CTA per (sequence, 128 pages) the chain length -> page ids -> query -> bounds was paid by four or
 // five waves of CTAs: 54 us for 32 sequences of 16 K to 64 K tokens whose bounds take 27; with 16-byte
 // copies by the multiplying warps themselves their load units were the limit: 47-50 us.)
@@ -32,10 +32,14 @@
 
 namespace pa {
 
-constexpr int kScoreWarps = 8;
+// Warps that multiply, by the blocks of eight query rows: with one block its operand stays in registers and eight
+// warps keep up with HBM; two blocks take sixteen; with more of them the accumulators leave room for eight.
+__host__ __device__ constexpr int score_warps(int nb8) { return nb8 == 2 ? 16 : 8; }
 constexpr int kScoreTilePages = 16;
-constexpr int kScoreProducers = 2;   // warps that request tiles: one warp's bulk copies go out 75-90 cycles apart
-constexpr int kScoreThreads = (kScoreWarps + kScoreProducers) * 32;
+// Warps that request tiles.  Two are enough for tiles of eight heads (31.8 us against 47.3 with one, whose bulk copies
+// go out 75-90 cycles apart, and 32.5 with four); smaller tiles are more of them (one kv head: 16.9 us with
+// two, 11.8 with four, 11.3 with eight; sixteen rows, four heads: 54, 41 and 43).
+__host__ __device__ constexpr int score_producers(int heads_per_cta) { return heads_per_cta == 8 ? 2 : 4; }
 constexpr int kScoreMaxSlots = 40;
 constexpr int kScoreRingBytes = 176 * 1024;
 constexpr int kScoreRowBytes = kD * 2 + 16;    // one query row as f16; the padding spreads the rows over the banks
@@ -56,10 +60,11 @@ struct BlockScoreParams {
   int32_t* status;
   int32_t S, Hkv, rows, block_size, num_blocks, width;
   int32_t q_is_fp8, q_quant_mode;
-  int32_t heads_per_cta;       // a power of two that divides kScoreWarps
-  // Ring depth in tiles, a multiple of kScoreWarps / heads_per_cta: a slot then holds tiles of the same warps
-  // (and, where those are not all, of the same producer) every time, so nobody waits for a phase of its
-  // barriers that is not the next one.
+  int32_t heads_per_cta;       // a power of two that divides the warps
+  // Ring depth in tiles, a multiple of warps / heads_per_cta: a slot then holds tiles of the same warps
+  // every time, and not less than the producers.  So nobody waits for a phase of its barriers that is not the
+  // next one: a warp has waited for the slot's tile before itself, and a producer that comes to a slot has
+  // filled it the last time, or has since filled a slot that was free only after this one was.
   int32_t slots;
   int32_t off_index, off_ring; // shared-memory carve: query rows and factors, index of the sequences, ring
   int64_t q_stride_seq;        // bytes
@@ -104,11 +109,16 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// NB8: blocks of eight query rows per kv head.
-template <int NB8>
-__global__ void __launch_bounds__(kScoreThreads, 1)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// NB8: blocks of eight query rows per kv head.  PRODUCERS: warps that request tiles.
+template <int NB8, int PRODUCERS>
+__global__ void __launch_bounds__((score_warps(NB8) + PRODUCERS) * 32, 1)
 pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
-  constexpr int kRows = NB8 * 8;
+  constexpr int kRows = NB8 * 8, kScoreWarps = score_warps(NB8);
+  constexpr int threads = (kScoreWarps + PRODUCERS) * 32, producers = PRODUCERS;
   constexpr bool kKeep = NB8 == 1;   // the query operand of a warp's head stays in registers (32 of them)
   extern __shared__ __align__(128) uint8_t smem[];
   float* factor = reinterpret_cast<float*>(smem + p.heads_per_cta * kRows * kScoreRowBytes);   // [heads][kRows]
@@ -134,7 +144,7 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   // ---- pages of every sequence, and tiles of 16 pages summed over the sequences (every CTA for itself)
   const int64_t cap = (int64_t)p.width * p.block_size;
   {
-    const int chunk = (p.S + kScoreThreads - 1) / kScoreThreads;
+    const int chunk = (p.S + threads - 1) / threads;
     const int beg = min(tid * chunk, p.S), end = min(beg + chunk, p.S);
     int sum = 0;
     for (int s = beg; s < end; ++s) {
@@ -198,7 +208,10 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
     };
     if (n_tiles > 0) skip(first);
     const uint64_t pol = l2_policy_evict_first();
-    const bool whole = p.bounds_stride_head == 2 * kD;   // a page's heads are one run
+    // A page's heads are one run of up to 2 KB, brought by a bulk copy.  An SM gets through one every 75-90
+    // cycles, so runs of one or two heads, and heads that lie apart, come in 16-byte pieces instead, two
+    // pages' worth with every instruction (32 contexts of 16 K to 64 K tokens, one kv head: 17 us against 23).
+    const bool whole = p.bounds_stride_head == 2 * kD && hpc > 2;
     // the page ids of two tiles ahead are on their way while a tile is requested
     auto fetch = [&](int k, int& group, int& valid, int& id) {
       valid = 0;
@@ -207,19 +220,19 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       if (k < n_tiles) {
         valid = min(kScoreTilePages, seq_pages[a.seq] - a.tile * kScoreTilePages);
         if (lane < valid) id = __ldg(p.block_tables + (int64_t)a.seq * p.bt_stride_seq + a.tile * kScoreTilePages + lane);
-        skip(kScoreProducers);
+        skip(producers);
       }
     };
     int g0, v0, id0, g1, v1, id1;
     fetch(first, g0, v0, id0);
-    fetch(first + kScoreProducers, g1, v1, id1);
+    fetch(first + producers, g1, v1, id1);
     int slot = first;
     uint32_t phase = 1;
-    for (int k = first; k < n_tiles; k += kScoreProducers) {
+    for (int k = first; k < n_tiles; k += producers) {
       const int group = g0, valid = v0;
       int id = id0;
       g0 = g1, v0 = v1, id0 = id1;
-      fetch(k + 2 * kScoreProducers, g1, v1, id1);
+      fetch(k + 2 * producers, g1, v1, id1);
       const uint32_t full = smem_addr(&bar_full[slot]);
       if (!__all_sync(kFullMask, mbar_wait(smem_addr(&bar_empty[slot]), phase))) {
         if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_WAIT_TIMEOUT);
@@ -231,22 +244,32 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       }
       const int head0 = group * hpc, heads = min(hpc, p.Hkv - head0);
       const uint32_t at = ring + slot * slot_bytes;
-      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(valid * heads * 2 * kD));
-      __syncwarp();
-      if (lane < valid) {
-        const uint8_t* src = p.bounds + (int64_t)id * p.bounds_stride_block + (int64_t)head0 * p.bounds_stride_head;
-        if (whole) {
-          bulk_g2s(at + lane * pitch, src, (uint32_t)(heads * 2 * kD), full, pol);
-        } else {
-          for (int h = 0; h < heads; ++h) bulk_g2s(at + lane * pitch + h * 2 * kD, src + (int64_t)h * p.bounds_stride_head, 2 * kD, full, pol);
+      const uint8_t* src = p.bounds + (int64_t)id * p.bounds_stride_block + (int64_t)head0 * p.bounds_stride_head;
+      if (whole) {
+        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(valid * heads * 2 * kD));
+        __syncwarp();
+        if (lane < valid) bulk_g2s(at + lane * pitch, src, (uint32_t)(heads * 2 * kD), full, pol);
+      } else {
+        // lane = (page of a pair, piece of its 256 bytes)
+        const uint64_t mine = reinterpret_cast<uint64_t>(src);
+        for (int h = 0; h < heads; ++h) {
+#pragma unroll
+          for (int j = 0; j < kScoreTilePages / 2; ++j) {
+            const int page = 2 * j + (lane >> 4);
+            const uint64_t from = __shfl_sync(kFullMask, mine, page) + (uint64_t)((int64_t)h * p.bounds_stride_head) + (lane & 15) * 16;
+            if (page < valid) cp_async16(at + page * pitch + h * 2 * kD + (lane & 15) * 16, reinterpret_cast<const void*>(from));
+          }
         }
+        if (lane == 0) tc::mbar_arrive(full);
+      }
+      if (lane < valid) {
         if (p.k_scale) {
           const float* ks = p.k_scale + (int64_t)id * p.ks_stride_block + (int64_t)head0 * p.ks_stride_head;
           for (int h = 0; h < heads; ++h) cp_async4(at + kScoreTilePages * pitch + (lane * hpc + h) * 4, ks + (int64_t)h * p.ks_stride_head);
         }
       }
       cp_async_arrive(full);
-      slot += kScoreProducers;
+      slot += producers;
       if (slot >= p.slots) slot -= p.slots, phase ^= 1;
     }
     return;

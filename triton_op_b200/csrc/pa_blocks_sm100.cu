@@ -185,9 +185,9 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
   k.softmax_scale = p->softmax_scale;
   const int nb8 = p->rows <= 8 ? 1 : (p->rows <= 16 ? 2 : (p->rows <= 32 ? 4 : 8));
   // kv heads per CTA: neighbouring heads of a page are neighbours in memory; as many as their query
-  // rows fit, a power of two that divides the CTA's warps
+  // rows fit, a power of two that divides the CTA's warps (three heads take the places of four)
   int heads = pa::kScoreMaxRows / (nb8 * 8);
-  while (heads > p->num_kv_heads) heads >>= 1;
+  while (heads / 2 >= p->num_kv_heads) heads >>= 1;
   k.heads_per_cta = heads;
   const int64_t tiles = ((int64_t)p->max_blocks_per_seq + pa::kScoreTilePages - 1) / pa::kScoreTilePages;
   const int64_t most = (int64_t)p->num_seqs * tiles * ((p->num_kv_heads + heads - 1) / heads);   // units of work, at most
@@ -199,20 +199,21 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
   int64_t slots = ((int64_t)dev->max_smem_optin - 1024 - off_ring) / slot;   // (1 KB: the kernel's barriers)
   if (slots > pa::kScoreRingBytes / slot) slots = pa::kScoreRingBytes / slot;
   if (slots > pa::kScoreMaxSlots) slots = pa::kScoreMaxSlots;
-  const int step = pa::kScoreWarps / heads;
+  const int warps = pa::score_warps(nb8), step = warps / heads;
   slots -= slots % step;
-  if (slots < step || slots < pa::kScoreProducers) return PA_ERR_TOO_LARGE;   // the index of the sequences leaves no room
+  const int producers = pa::score_producers(heads);
+  if (slots < step || slots < producers) return PA_ERR_TOO_LARGE;   // the index of the sequences leaves no room
   k.off_ring = (int)off_ring;
   k.slots = (int)slots;
   const int64_t smem = off_ring + slots * slot;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  void (*kernel)(pa::BlockScoreParams) = nb8 == 1   ? pa::pa_block_score_kernel<1>
-                                         : nb8 == 2 ? pa::pa_block_score_kernel<2>
-                                         : nb8 == 4 ? pa::pa_block_score_kernel<4>
-                                                    : pa::pa_block_score_kernel<8>;
+  void (*kernel)(pa::BlockScoreParams) = nb8 == 1   ? (heads == 8 ? pa::pa_block_score_kernel<1, 2> : pa::pa_block_score_kernel<1, 4>)
+                                         : nb8 == 2 ? pa::pa_block_score_kernel<2, 4>
+                                         : nb8 == 4 ? pa::pa_block_score_kernel<4, 4>
+                                                    : pa::pa_block_score_kernel<8, 4>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_fail(e);
-  return launch(kernel, dim3((unsigned)grid), pa::kScoreThreads, (size_t)smem, st, k);
+  return launch(kernel, dim3((unsigned)grid), (warps + producers) * 32, (size_t)smem, st, k);
 }
 
 int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
