@@ -859,6 +859,59 @@ def test_serving_steps(bs, query_len, group):
         assert_attention(out, bo.attention(q, kc, vc, ks, vs, got, tokens, SCALE, query_len))
 
 
+class NotTaken:
+    """Host calls that take nothing: every call goes through the Python functions."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["plain", "transposed", "status", "per tensor", "two tokens"])
+def test_both_ways_to_the_library_give_the_same_bits(monkeypatch, form):
+    """Ordinary calls go from the tensors to the library in C++, the others through Python."""
+    lib_calls = _lib.calls()
+    query_len = 2 if form == "two tokens" else 1
+    c = Cache([300, 17, 700], 2, 64 if form == "transposed" else 16, seed=23)
+    value = transposed(c.value) if form == "transposed" else c.value
+    q = c.query(4, query_len).cuda()
+    rows = torch.randn(9, 2, D, generator=c.g).bfloat16().cuda()
+    start = torch.tensor([0, 4, 4, 9], dtype=torch.int32).cuda()
+    tables, lengths = cuda(c.tables, c.lengths)
+    got = []
+    for calls in (lib_calls, NotTaken()):
+        monkeypatch.setattr(_lib, "_CALLS", calls)
+        kc, vc, ks, vs, bounds = cuda(c.key.clone(), value.clone(), c.ks.clone(), c.vs.clone(), c.bounds())
+        if form == "per tensor":
+            ks, vs = torch.tensor(0.02, device="cuda"), torch.tensor(0.03, device="cuda")
+        status = torch.zeros((), dtype=torch.int32, device="cuda") if form == "status" else None
+        pa.append_kv_cache(rows, rows, kc, vc, ks, vs, tables, lengths, start, key_bounds=bounds, status=status)
+        out = torch.full_like(q, math.nan)
+        res = pa.sparse_attention_decode(out, q, kc, vc, bounds, lengths, tables, SCALE, query_len, 5, None, ks, vs, status=status)
+        score = pa.score_blocks(q, bounds, lengths, tables, SCALE, query_len, c.bs, key_scale=ks, status=status)
+        full = torch.full_like(q, math.nan)
+        if form != "per tensor":
+            pa.paged_attention_decode(full, q, kc, vc, lengths, tables, SCALE, query_len, 700, torch.bfloat16, None, ks, vs, status=status)
+        got.append([kc, vc, ks, vs, bounds, out, res["block_tables"], res["sequence_lengths"], res["exponential_sums"].shape, score, full])
+    for a, b in zip(*got):
+        if isinstance(a, torch.Tensor):
+            assert torch.equal(a.view(torch.uint8) if a.dim() else a, b.view(torch.uint8) if b.dim() else b)
+        else:
+            assert a == b
+
+
+@pytest.mark.gpu
+def test_errors_of_the_library_are_raised_either_way(monkeypatch):
+    c = Cache([300], 2, 16)
+    room = torch.zeros(c.nb * 2 * 2 * D + 8, dtype=torch.uint8, device="cuda")
+    bounds = room[8:].view(FP8).view(c.nb, 2, 2, D)              # not on a 16-byte boundary
+    q = c.query(2).cuda()
+    for calls in (_lib.calls(), NotTaken()):
+        monkeypatch.setattr(_lib, "_CALLS", calls)
+        with pytest.raises(_lib.PaError, match="16-byte|align"):
+            pa.score_blocks(q, bounds, *cuda(c.lengths, c.tables), SCALE, 1, 16, key_scale=c.ks.cuda())
+
+
 @pytest.mark.gpu
 def test_few_pages_are_all_read():
     """top_k at least the number of pages: the full attention, bit for bit."""

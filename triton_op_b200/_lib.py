@@ -6,11 +6,13 @@ the operator fails with an explicit error -- there is no Python or CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
 
-from .build import LIB_PATH
+from .build import CALLS_PATH, LIB_PATH
 
 PA_ABI_VERSION = 3
 
@@ -182,6 +184,26 @@ def lib() -> C.CDLL:
         raise ImportError("libpa_decode_sm100.so was built from a different ABI version; rebuild it")
     _LIB = L
     return L
+
+
+_CALLS = None
+
+
+def calls():
+    """The host calls (``csrc/pa_calls.cpp``), bound to the loaded library; raises if they have not been built.
+    Each takes an ordinary call whole, or answers None and leaves it to the Python function."""
+    global _CALLS
+    if _CALLS is None:
+        L = lib()
+        if not os.path.exists(CALLS_PATH):
+            raise ImportError(f"{CALLS_PATH} is missing: run `python -m triton_op_b200.build`.")
+        loader = importlib.machinery.ExtensionFileLoader("pa_calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("pa_calls", loader))
+        loader.exec_module(module)
+        module.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in (
+            "pa_decode_tables_sm100", "pa_cache_append_sm100", "pa_block_scores_sm100", "pa_block_select_sm100")), PA_ABI_VERSION)
+        _CALLS = module
+    return _CALLS
 
 
 # The handle of torch's current stream of a device (torch.cuda.current_stream builds an object around it,

@@ -139,6 +139,12 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     that have no place; they are skipped.  No page may get rows of two sequences in a call.  Runs on
     the current stream; there is no CPU fallback.
     """
+    done = _lib.calls().append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables, sequence_lengths,
+                               query_start_loc, key_bounds, status)
+    if type(done) is tuple:
+        return
+    if done is not None:
+        raise _lib.PaError(done, "pa_cache_append_sm100")
     on, dev = key.get_device(), key.device
     k_shape, c_shape = key.shape, key_cache.shape
     if not (key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16 and k_shape == value.shape and len(k_shape) == 3):

@@ -441,7 +441,7 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
                     query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,
                     alibi_slopes, sink_tokens, status):
     """(parameter block, elements between the kv heads' tables, tensors to keep alive, workspaces) of
-    a call with scales per (page, kv head) and / or a block table per kv head.
+    a call with scales per (page, kv head) and / or a block table per kv head that the host calls have not taken.
 
     Every call validates its arguments, so each shape and stride tuple is fetched once: the host
     time of a small call is mostly such accesses."""
@@ -679,6 +679,16 @@ def paged_attention_decode(
         if partition_size <= 0 or partition_size % SEQUENCE_PARTITION_SIZE:
             _fail(f"block kv scales and block tables per kv head run in partitions of {SEQUENCE_PARTITION_SIZE} tokens, but got partition_size {partition_size}")
         if not special:
+            if (query_scale is None and alibi_slopes is None and sink_tokens is None
+                    and (compute_type is torch.bfloat16 or compute_type is None)):
+                ws = _lib.calls().decode(output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
+                                         query_sequence_length, max_sequence_length, key_scale, value_scale, status)
+                if type(ws) is tuple:
+                    return {"triton_decode_time": 0.0, "triton_reduce_time": 0.0, "temporary_output": ws[2],
+                            "final_output": output, "exponential_sums": ws[0], "maximum_logits": ws[1],
+                            "total_triton_time": 0.0, "partition_size": SEQUENCE_PARTITION_SIZE}
+                if ws is not None:
+                    raise _lib.PaError(ws, "pa_decode_tables_sm100")
             p, head_stride, keep, ws = _build_by_block(
                 output, query, key_cache, value_cache, sequence_lengths, block_tables, softmax_scale,
                 query_sequence_length, max_sequence_length, compute_type, query_scale, key_scale, value_scale,

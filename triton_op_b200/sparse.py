@@ -77,6 +77,13 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
     ``[num_blocks, num_kv_heads, 2, head_size]``; ``key_scale`` ``None``, per tensor or
     ``[num_blocks, num_kv_heads, 1, 1]``; ``scores``: an output tensor to use.
     """
+    if query_scale is None and scores is None:
+        done = _lib.calls().scores(query, key_bounds, sequence_lengths, block_tables, softmax_scale, query_sequence_length,
+                                   block_size, key_scale, status)
+        if type(done) is tuple:
+            return done[0]
+        if done is not None:
+            raise _lib.PaError(done, "pa_block_scores_sm100")
     dev, on = query.device, query.get_device()
     q_shape, b_shape = query.shape, key_bounds.shape
     if len(q_shape) != 3:
@@ -172,6 +179,12 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     ``scores`` (fp32 ``[num_seqs, num_kv_heads, max_blocks]``), NaN as -inf, ties to the lower place.
     With several query tokens ``keep_last`` has to cover the last ``query_len`` tokens: 2.
     """
+    if tables is None and lengths is None:
+        done = _lib.calls().select(scores, sequence_lengths, block_tables, block_size, top_k, keep_first, keep_last, status)
+        if type(done) is tuple:
+            return done
+        if done is not None:
+            raise _lib.PaError(done, "pa_block_select_sm100")
     dev, on = scores.device, scores.get_device()
     sc_shape = scores.shape
     if not (len(sc_shape) == 3 and scores.dtype == torch.float32):
