@@ -693,6 +693,40 @@ def test_append_of_prompts(bs, hkv, counts, before):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["normal", "transposed"])
+@pytest.mark.parametrize("bs", [16, 64, 1024])
+@pytest.mark.parametrize("per_tensor", [None, 0.013])
+def test_append_of_a_few_rows_to_many_pages(bs, layout, per_tensor):
+    """More (page, head) pairs than are worked on at once, a few rows each; pages that grow and pages that stay."""
+    counts = [(7 * i) % 25 if i % 9 else 0 for i in range(60)]
+    before = [(37 * i) % 150 for i in range(60)]
+    c = Cache([a + b for a, b in zip(before, counts)], 7, bs, seed=5)
+    start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32)
+    n = sum(counts)
+    size = torch.exp2(torch.randint(-7, 3, (n, 1, 1), generator=c.g).float())      # some pages' scales stay, some grow
+    key = (torch.randn(n, 7, D, generator=c.g) * size).bfloat16()
+    value = (torch.randn(n, 7, D, generator=c.g) * size).bfloat16()
+    vc = transposed(c.value) if layout == "transposed" else None
+    got, want, status = append_both(c, key, value, c.lengths, start, c.bounds(), value_cache=vc, per_tensor=per_tensor)
+    assert status == 0
+    assert_same(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("per_tensor", [None, 0.013])
+@pytest.mark.parametrize("bs,count,seqs", [(64, 15, 40), (64, 30, 3), (1024, 60, 10), (1024, 260, 10), (1024, 260, 2), (1024, 1030, 6)])
+def test_append_begins_and_ends_inside_runs(bs, count, seqs, per_tensor):
+    """Values that share a 16-token run with older ones at the first row and with none at the last, on scales that stay."""
+    c = Cache([8 + count] * seqs, 11, bs, seed=count)
+    start = torch.arange(seqs + 1, dtype=torch.int32) * count
+    key = torch.randn(seqs * count, 11, D, generator=c.g).bfloat16() * 0.05
+    value = torch.randn(seqs * count, 11, D, generator=c.g).bfloat16() * 0.05
+    got, want, status = append_both(c, key, value, c.lengths, start, c.bounds(), per_tensor=per_tensor)
+    assert status == 0
+    assert_same(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bs", [16, 64])
 def test_append_token_by_token_grows_pages(bs):
     """Tokens that get larger and larger: each page's scale grows again and again."""

@@ -119,13 +119,19 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
     const int64_t grid = units < dev->sm_count ? units : dev->sm_count;
     return launch(blk ? pa::pa_cache_append_kernel<1024, 16, true> : pa::pa_cache_append_kernel<1024, 16, false>, dim3((unsigned)grid), 512, smem, st, k);
   }
-  const int per_cta = p->block_size == 16 ? 4 : 1;
-  int64_t grid = (units + per_cta - 1) / per_cta;
   const int64_t cap = (int64_t)dev->sm_count * 5;   // what is resident at a time
+  // Pages of 64 tokens that get a few rows each (fewer than a run of 16 per sequence, on average), more of them
+  // than four warps apiece could take at once: a warp each (5.3 us against 7.5 for a row of 64 sequences with
+  // eight kv heads; prompts, whose pages have four full runs, would lose: 31 us against 25 for 16 000 rows).
+  const bool lone = p->block_size == 64 && p->num_tokens < 16 * (int64_t)p->num_seqs && units > cap;
+  const int per_cta = p->block_size == 16 || lone ? 4 : 1;
+  int64_t grid = (units + per_cta - 1) / per_cta;
   if (grid > cap) grid = cap;
   switch (p->block_size) {
     case 16: return launch(blk ? pa::pa_cache_append_kernel<16, 1, true> : pa::pa_cache_append_kernel<16, 1, false>, dim3((unsigned)grid), 128, smem, st, k);
-    case 64: return launch(blk ? pa::pa_cache_append_kernel<64, 4, true> : pa::pa_cache_append_kernel<64, 4, false>, dim3((unsigned)grid), 128, smem, st, k);
+    case 64:
+      if (lone) return launch(blk ? pa::pa_cache_append_kernel<64, 1, true> : pa::pa_cache_append_kernel<64, 1, false>, dim3((unsigned)grid), 128, smem, st, k);
+      return launch(blk ? pa::pa_cache_append_kernel<64, 4, true> : pa::pa_cache_append_kernel<64, 4, false>, dim3((unsigned)grid), 128, smem, st, k);
     default: return launch(blk ? pa::pa_cache_append_kernel<1024, 4, true> : pa::pa_cache_append_kernel<1024, 4, false>, dim3((unsigned)grid), 128, smem, st, k);
   }
 }

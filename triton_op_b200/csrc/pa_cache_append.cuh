@@ -21,12 +21,15 @@
 // maximum and the store.  A page of 1024 tokens is 64 such runs.  Sixteen warps take four each and read
 // the rows twice; where there are fewer pages than could keep the GPU busy that way, a page is shared by
 // a cluster of eight CTAs that find the maximum through each other's shared memory (9 us against 17 for
-// two prompts of 2 200 and 3 300 tokens, one kv head; for many pages the clusters' barriers cost more than they save);
-// with a few rows per sequence, where most warps would have nothing to do, four warps take the runs in turn.  Keys are
+// two prompts of 2 200 and 3 300 tokens, one kv head, when that was chosen, 5.9 since; for many pages the clusters'
+// barriers cost more than they save); with a few rows per sequence, where most warps would have nothing to do, four
+// warps take the runs in turn.  A page of 64 has four warps, or one where each gets a few rows.  Keys are
 // stored as 16-byte chunks [d/16][token][16], values as 16 tokens of a head dim, 16 bytes too;
 // values of a run that is not whole are merged with the bytes that are there.
-// What bounds it: 512 bytes read and 256 written per (token, kv head) -- HBM for a prompt; a decode
-// step of a few hundred rows is launch latency and one chain of loads.
+// What bounds it: 512 bytes read and 256 written per (token, kv head).  A prompt is bound by the
+// instructions that quantise it: 16 000 tokens of eight kv heads take 22 us in pages of 16, 25 in pages of 64 and 34 in
+// pages of 1024 (15 at the copy bandwidth).  A row for each of 64 sequences takes 4.3, 5.1 and 9.1 us: launch
+// latency and one chain of loads, which is why whatever a page holds already is asked for at once.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -135,20 +138,30 @@ __device__ __forceinline__ float up_to_power(float s) {
   return (u & 0x7fffffu) == 0u ? s : __uint_as_float(min((u >> 23) + 1u, 254u) << 23);
 }
 
-// Brings a page's codes to a larger scale: runs first, first + step, ... of 16 slots.  A rare path, out
-// of line so that the common one keeps its registers.  Each thread touches the 16-byte pieces that
-// it writes in the kernel below, so nothing has to be waited for in between.
-template <int BS>
-static __device__ __noinline__ void rescale_runs(uint8_t* cache, bool is_v, bool v_trans, int first, int step, float ratio, int lane) {
+// Brings a page's codes to a larger scale: runs first, first + WPU, ... of 16 slots.  A rare path, out
+// of line so that the common one keeps its registers, but one that a step over many pages nearly always
+// takes somewhere: a run's four pieces (two where a page is one run) are read before the first is written, so that
+// their latencies overlap; more at a time cost the kernel registers, and a prompt 1 to 5 % of its time.
+// Each thread touches the 16-byte pieces that it writes in the kernel below, so nothing has to be
+// waited for in between.
+template <int BS, int WPU>
+static __device__ __noinline__ void rescale_runs(uint8_t* cache, bool is_v, bool v_trans, int first, float ratio, int lane) {
+  constexpr int kAtOnce = BS == 16 ? 2 : 4;
+  auto piece = [&](int run, int e) -> uint4* {
+    const int d = 4 * lane + e;
+    return reinterpret_cast<uint4*>(
+        is_v ? (v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16)
+             : cache + ((int64_t)(lane >> 2) * BS + run * 16 + 4 * e + (lane & 3)) * 16);
+  };
 #pragma unroll 1
-  for (int run = first; run < BS / 16; run += step) {
+  for (int run = first; run < BS / 16; run += WPU) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = 4 * lane + e;
-      uint4* at = reinterpret_cast<uint4*>(
-          is_v ? (v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16)
-               : cache + ((int64_t)(lane >> 2) * BS + run * 16 + 4 * e + (lane & 3)) * 16);
-      *at = rescale_e4m3x16(*at, ratio);
+    for (int at = 0; at < 4; at += kAtOnce) {
+      uint4 was[kAtOnce];
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) was[e] = *piece(run, at + e);
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) *piece(run, at + e) = rescale_e4m3x16(was[e], ratio);
     }
   }
 }
@@ -167,8 +180,9 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
   int* unit_off = index_smem;          // [S + 1] pages touched before each sequence
   __shared__ int scan[32];
   __shared__ uint32_t red_max[kThreads / 32];
-  __shared__ uint32_t red_lo[kCtaWarps][64], red_hi[kCtaWarps][64];
-  __shared__ uint32_t cta_max, cta_lo[64], cta_hi[64];              // CLUSTER: this CTA's share
+  __shared__ uint4 red_bounds[kCtaWarps][32];
+  __shared__ uint32_t cta_max;                                      // CLUSTER: this CTA's share
+  __shared__ uint4 cta_bounds[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int team = (int)blockIdx.x / CLUSTER, teams = (int)gridDim.x / CLUSTER, rank = (int)blockIdx.x - team * CLUSTER;
   const int sub = CLUSTER > 1 ? rank * kCtaWarps + warp : warp % WPU;   // warp inside its unit
@@ -296,8 +310,9 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     const int run0 = o0 >> 4, run1 = o1 > o0 ? ((o1 - 1) >> 4) + 1 : run0;
     auto mine = [&](int k) -> int { return sub + k * WPU; };
     int loaded = -1;
-    if (mine(0) >= run0 && mine(0) < run1) {
-      loaded = mine(0);
+    const int first = mine(kPerWarp > 1 && run0 > sub ? (run0 - sub + WPU - 1) / WPU : 0);   // the warp's first run with rows
+    if (first >= run0 && first < run1) {
+      loaded = first;
       load_run(loaded);
     }
     next = decode(u0 + teams * kUnits + in_team);
@@ -311,13 +326,43 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
                           : p.key_cache + (int64_t)blk * p.kc_stride_block + (int64_t)head * p.kc_stride_head;
     float* scale_at = (is_v ? p.v_scale : p.k_scale) + (PER_BLOCK ? (int64_t)blk * p.ks_stride_block + (int64_t)head * p.ks_stride_head : 0);
     const float old_scale = live ? *scale_at : 1.0f;
+    const bool want_bounds = p.bounds != nullptr && !is_v;
+    const bool fresh = o0 == 0;
+    // the page's bounds of head dims 4 lane .. 4 lane + 3, asked for with its scale
+    uint32_t* bounds_at = want_bounds ? reinterpret_cast<uint32_t*>(p.bounds + (int64_t)blk * p.b_stride_block + (int64_t)head * p.b_stride_head) + lane : nullptr;
+    uint32_t old_lo = 0, old_hi = 0;
+    if (want_bounds && live && !fresh && sub == 0) old_lo = bounds_at[0], old_hi = bounds_at[kD / 4];
+
+    auto v_piece = [&](int run, int e) -> uint4* {      // where the codes of head dim 4 lane + e, slots of a run, are
+      const int d = 4 * lane + e;
+      return reinterpret_cast<uint4*>(p.v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16);
+    };
+    auto partial = [&](int run) -> bool { return run * 16 < o0 || run * 16 + 16 > o1; };
+    // Registers that keys use for the smallest (0 .. 7) and largest (8 .. 15) of a lane's head dims, and
+    // values for the codes that share a run with new ones.  Those are asked for here, with the scale: after
+    // the barrier below they would be read from sectors that another warp has just written half of, which took
+    // 67 us where this takes 49 (64 sequences of 448 rows into pages of 64, the first page begun inside a run).
+    uint32_t ext[16];
+    // (A page of 16 belongs to one warp, which reads its codes when it needs them: the registers are worth more.)
+    constexpr bool kEarly = BS > 16;
+    int held = -1;                                      // the run whose codes are in ext
+    if (!is_v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ext[e] = 0x7f807f80u, ext[8 + e] = 0xff80ff80u;   // +inf, -inf
+    } else if (kEarly && live && run1 > run0) {
+      if (partial(run0) && run0 % WPU == sub) held = run0;
+      else if (partial(run1 - 1) && (run1 - 1) % WPU == sub) held = run1 - 1;
+      if (held >= 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint4 was = *v_piece(held, e);
+          ext[4 * e] = was.x, ext[4 * e + 1] = was.y, ext[4 * e + 2] = was.z, ext[4 * e + 3] = was.w;
+        }
+      }
+    }
 
     // ---- the largest finite |x|, and the smallest and largest key of every head dim
     uint32_t top = 0;
-    uint32_t lo8[8], hi8[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) lo8[e] = 0x7f807f80u, hi8[e] = 0xff80ff80u;   // +inf, -inf
-    const bool want_bounds = p.bounds != nullptr && !is_v;
 #pragma unroll 1
     for (int k = 0; k < kPerWarp; ++k) {
       const int run = mine(k);
@@ -357,7 +402,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
           for (int e = 0; e < 8; ++e) any = __vmaxu2(any, __vmaxu2(lo[e] & 0x7fff7fffu, hi[e] & 0x7fff7fffu));
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], lo[e]), hi8[e] = bf16x2_max(hi8[e], hi[e]);
+        for (int e = 0; e < 8; ++e) ext[e] = bf16x2_min(ext[e], lo[e]), ext[8 + e] = bf16x2_max(ext[8 + e], hi[e]);
       }
       if ((any & 0xffffu) >= 0x7f80u || (any >> 16) >= 0x7f80u) {
         any = 0;
@@ -367,57 +412,56 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
       top = __vmaxu2(top, any);
     }
     uint32_t top1 = __reduce_max_sync(kFullMask, max(top & 0xffffu, top >> 16));
+    // The bounds over the four lanes of a chunk, halved at each step: lane f keeps words 2 f, 2 f + 1 of
+    // the chunk's eight, which are head dims 4 lane .. 4 lane + 3 (12 exchanges; 32 if all lanes kept all).
+    uint4 bound = make_uint4(0x7f807f80u, 0x7f807f80u, 0xff80ff80u, 0xff80ff80u);   // min, min, max, max
+    auto join = [](const uint4& a, const uint4& b) -> uint4 {
+      return make_uint4(bf16x2_min(a.x, b.x), bf16x2_min(a.y, b.y), bf16x2_max(a.z, b.z), bf16x2_max(a.w, b.w));
+    };
     if (want_bounds) {
+      const bool up2 = (f & 2) != 0, up1 = (f & 1) != 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-#pragma unroll
-        for (int o = 1; o <= 2; o <<= 1) {
-          lo8[e] = bf16x2_min(lo8[e], __shfl_xor_sync(kFullMask, lo8[e], o));
-          hi8[e] = bf16x2_max(hi8[e], __shfl_xor_sync(kFullMask, hi8[e], o));
-        }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t l = __shfl_xor_sync(kFullMask, up2 ? ext[e] : ext[e + 4], 2);
+        const uint32_t h = __shfl_xor_sync(kFullMask, up2 ? ext[e + 8] : ext[e + 12], 2);
+        ext[e] = bf16x2_min(up2 ? ext[e + 4] : ext[e], l);
+        ext[e + 8] = bf16x2_max(up2 ? ext[e + 12] : ext[e + 8], h);
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t l = __shfl_xor_sync(kFullMask, up1 ? ext[e] : ext[e + 2], 1);
+        const uint32_t h = __shfl_xor_sync(kFullMask, up1 ? ext[e + 8] : ext[e + 10], 1);
+        ext[e] = bf16x2_min(up1 ? ext[e + 2] : ext[e], l);
+        ext[e + 8] = bf16x2_max(up1 ? ext[e + 10] : ext[e + 8], h);
+      }
+      bound = make_uint4(ext[0], ext[1], ext[8], ext[9]);
     }
     if (WPU > 1) {   // over the warps of the unit (a CTA, or a cluster, then has one unit)
       if (lane == 0) red_max[warp] = top1;
-      if (want_bounds && f == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) red_lo[warp % kCtaWarps][c * 8 + e] = lo8[e], red_hi[warp % kCtaWarps][c * 8 + e] = hi8[e];
-      }
+      if (want_bounds) red_bounds[warp % kCtaWarps][lane] = bound;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kCtaWarps; ++w) top1 = max(top1, red_max[w]);
       if (want_bounds && warp == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-#pragma unroll 1
-          for (int w = 0; w < kCtaWarps; ++w) lo8[e] = bf16x2_min(lo8[e], red_lo[w][c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], red_hi[w][c * 8 + e]);
-        }
+#pragma unroll 4
+        for (int w = 1; w < kCtaWarps; ++w) bound = join(bound, red_bounds[w][lane]);
       }
       if constexpr (CLUSTER > 1) {
         namespace cg = cooperative_groups;
         const cg::cluster_group cluster = cg::this_cluster();
         if (warp == 0) {
           if (lane == 0) cta_max = top1;
-          if (want_bounds && f == 0) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) cta_lo[c * 8 + e] = lo8[e], cta_hi[c * 8 + e] = hi8[e];
-          }
+          if (want_bounds) cta_bounds[lane] = bound;
         }
         cluster.sync();
         const uint32_t theirs = lane < CLUSTER ? *cluster.map_shared_rank(&cta_max, lane) : 0u;
         top1 = __reduce_max_sync(kFullMask, theirs);
         if (want_bounds && sub == 0) {
-#pragma unroll 1
-          for (int r = 1; r < CLUSTER; ++r) {
-            const uint32_t* lo = cluster.map_shared_rank(cta_lo, r);
-            const uint32_t* hi = cluster.map_shared_rank(cta_hi, r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) lo8[e] = bf16x2_min(lo8[e], lo[c * 8 + e]), hi8[e] = bf16x2_max(hi8[e], hi[c * 8 + e]);
-          }
+          for (int r = 1; r < CLUSTER; ++r) bound = join(bound, *cluster.map_shared_rank(&cta_bounds[lane], r));
         }
       }
     }
-    const bool fresh = o0 == 0;
     float scale = old_scale, ratio = 1.0f;
     bool grew = false;
     if (PER_BLOCK) {
@@ -428,10 +472,10 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     }
     if (live && o1 > o0) {
       const float inv = 1.0f / scale;
-      if (PER_BLOCK && grew) rescale_runs<BS>(cache, is_v, p.v_trans != 0, sub, WPU, ratio, lane);
+      if (PER_BLOCK && grew) rescale_runs<BS, WPU>(cache, is_v, p.v_trans != 0, sub, ratio, lane);
       auto four = [&](uint32_t w0, uint32_t w1) -> uint32_t { return quantise_four<!PER_BLOCK>(w0, w1, scale, inv); };
 #pragma unroll 1
-      for (int k = 0; k < kPerWarp; ++k) {
+      for (int k = kPerWarp - 1; k >= 0; --k) {   // backwards: the last run's rows are still here
         const int run = mine(k);
         if (run < run0 || run >= run1) continue;
         if (run != loaded) {
@@ -450,62 +494,57 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
           }
         } else {
           const int a = max(o0 - run * 16, 0), b = min(o1 - run * 16, 16);   // slots [a, b) of the run are new
-          const bool merge = a > 0 || b < 16;
           uint32_t qv[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) qv[i] = four(raw[2 * i], raw[2 * i + 1]);
+          auto word = [&](int e, int j) -> uint32_t {       // the new codes of head dim 4 lane + e, slots 4 j ..
+            const uint32_t lo = __byte_perm(qv[4 * j], qv[4 * j + 1], 0x0040 + 0x0011 * e);
+            const uint32_t hi = __byte_perm(qv[4 * j + 2], qv[4 * j + 3], 0x0040 + 0x0011 * e);
+            return __byte_perm(lo, hi, 0x5410);
+          };
+          if (!partial(run)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 4 * lane + e;
-            uint4* dst = reinterpret_cast<uint4*>(p.v_trans ? cache + ((int64_t)run * kD + d) * 16 : cache + (int64_t)d * BS + run * 16);
-            uint32_t w[4];
+            for (int e = 0; e < 4; ++e) *v_piece(run, e) = make_uint4(word(e, 0), word(e, 1), word(e, 2), word(e, 3));
+          } else {
+            if (!kEarly || grew || (kPerWarp > 1 && run != held)) {   // all four before the first is written
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint4 was = *v_piece(run, e);
+                ext[4 * e] = was.x, ext[4 * e + 1] = was.y, ext[4 * e + 2] = was.z, ext[4 * e + 3] = was.w;
+              }
+              held = -1;
+            }
+            uint32_t fresh_bytes[4];                        // bytes of word j that are new: slots 4 j .. 4 j + 3 inside [a, b)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint32_t lo = __byte_perm(qv[4 * j], qv[4 * j + 1], 0x0040 + 0x0011 * e);
-              const uint32_t hi = __byte_perm(qv[4 * j + 2], qv[4 * j + 3], 0x0040 + 0x0011 * e);
-              w[j] = __byte_perm(lo, hi, 0x5410);
+              const int from = min(max(a - 4 * j, 0), 4), to = min(max(b - 4 * j, 0), 4);
+              const uint32_t below_to = to >= 4 ? 0xffffffffu : (1u << (8 * to)) - 1u;
+              const uint32_t below_from = from >= 4 ? 0xffffffffu : (1u << (8 * from)) - 1u;
+              fresh_bytes[j] = below_to & ~below_from;
             }
-            if (merge) {
-              const uint4 was = *dst;
-              const uint32_t o4[4] = {was.x, was.y, was.z, was.w};
+            auto mix = [&](uint32_t now, uint32_t then, int j) -> uint32_t { return (now & fresh_bytes[j]) | (then & ~fresh_bytes[j]); };
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                // bytes of word j that are new: slots 4 j .. 4 j + 3 inside [a, b)
-                const int from = min(max(a - 4 * j, 0), 4), to = min(max(b - 4 * j, 0), 4);
-                const uint32_t below_to = to >= 4 ? 0xffffffffu : (1u << (8 * to)) - 1u;
-                const uint32_t below_from = from >= 4 ? 0xffffffffu : (1u << (8 * from)) - 1u;
-                const uint32_t fresh_bytes = below_to & ~below_from;
-                w[j] = (w[j] & fresh_bytes) | (o4[j] & ~fresh_bytes);
-              }
-            }
-            *dst = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; ++e)
+              *v_piece(run, e) = make_uint4(mix(word(e, 0), ext[4 * e], 0), mix(word(e, 1), ext[4 * e + 1], 1),
+                                            mix(word(e, 2), ext[4 * e + 2], 2), mix(word(e, 3), ext[4 * e + 3], 3));
           }
         }
       }
-      if (want_bounds && sub == 0 && f == 0) {
-        uint4* at_lo = reinterpret_cast<uint4*>(p.bounds + (int64_t)blk * p.b_stride_block + (int64_t)head * p.b_stride_head + c * 16);
-        uint4* at_hi = at_lo + kD / 16;
-        uint32_t l4[4], h4[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l4[j] = four(lo8[2 * j], lo8[2 * j + 1]), h4[j] = four(hi8[2 * j], hi8[2 * j + 1]);
+      if (want_bounds && sub == 0) {
+        uint32_t l4 = four(bound.x, bound.y), h4 = four(bound.z, bound.w);
         if (!fresh) {
-          uint4 ol = *at_lo, oh = *at_hi;
-          if (grew) ol = rescale_e4m3x16(ol, ratio), oh = rescale_e4m3x16(oh, ratio);
-          const uint32_t wl[4] = {ol.x, ol.y, ol.z, ol.w}, wh[4] = {oh.x, oh.y, oh.z, oh.w};
+          if (grew) old_lo = rescale_e4m3x4(old_lo, ratio), old_hi = rescale_e4m3x4(old_hi, ratio);
+          float a[4], b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float a[4], b[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              a[e] = fminf(e4m3_to_f32(l4[j] >> (8 * e)), e4m3_to_f32(wl[j] >> (8 * e)));
-              b[e] = fmaxf(e4m3_to_f32(h4[j] >> (8 * e)), e4m3_to_f32(wh[j] >> (8 * e)));
-            }
-            l4[j] = pack_e4m3x4(a[0], a[1], a[2], a[3]);
-            h4[j] = pack_e4m3x4(b[0], b[1], b[2], b[3]);
+          for (int e = 0; e < 4; ++e) {
+            a[e] = fminf(e4m3_to_f32(l4 >> (8 * e)), e4m3_to_f32(old_lo >> (8 * e)));
+            b[e] = fmaxf(e4m3_to_f32(h4 >> (8 * e)), e4m3_to_f32(old_hi >> (8 * e)));
           }
+          l4 = pack_e4m3x4(a[0], a[1], a[2], a[3]);
+          h4 = pack_e4m3x4(b[0], b[1], b[2], b[3]);
         }
-        *at_lo = make_uint4(l4[0], l4[1], l4[2], l4[3]);
-        *at_hi = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+        bounds_at[0] = l4;
+        bounds_at[kD / 4] = h4;
       }
     }
     // every warp of the unit has read the old scale (before the barrier of the maximum, or, with one
