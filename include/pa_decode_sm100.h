@@ -360,7 +360,8 @@ int pa_cache_append_sm100(const PaCacheAppendParams* params, void* stream);
  * token of its context
  *   scores[s, h, i] = key_scale[page, h] * max_r softmax_scale * qs_r * sum_d max(q_rd lo_d, q_rd hi_d)
  * over the query rows r of kv head h, where (lo, hi) = key_bounds[page, h]: no logit of the group
- * with a key of the page is larger.  Entries past the last such page become -inf.
+ * with a key of the page is larger.  Entries past the last such page become -inf; a query row that
+ * holds a NaN makes the scores of its kv head NaN.
  */
 typedef struct PaBlockScoreParams {
   uint32_t struct_size, abi_version;

@@ -541,6 +541,27 @@ def test_scores_of_many_short_sequences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["bf16", "fp8", "fp8, a scale a row"])
+@pytest.mark.parametrize("hkv,group", [(8, 4), (3, 2), (2, 16), (1, 30), (2, 40)])
+def test_scores_of_many_sequences_and_queries(hkv, group, rows):
+    """A CTA goes from one sequence's query (and its scales) to the next; what lies past a short context is -inf."""
+    lengths = [(41 * i) % 700 if i % 5 else 0 for i in range(500)]
+    c = Cache(lengths, hkv, 16, seed=hkv, width=1500)
+    q = c.query(group) * torch.exp2(torch.randint(-4, 5, (500, hkv * group, 1), generator=c.g).float()).bfloat16()
+    scale = None
+    if rows != "bf16":
+        q = (q.float() * 8).to(FP8)
+        scale = torch.rand(500, hkv * group, 1, generator=c.g) + 0.1 if rows == "fp8, a scale a row" else torch.tensor(0.125)
+    out = torch.full((500, hkv, 1500), 7.0, device="cuda")
+    kw = dict(key_scale=c.ks.cuda(), scores=out, query_scale=None if scale is None else scale.cuda())
+    got = pa.score_blocks(*cuda(q, c.bounds(), c.lengths, c.tables), SCALE, 1, 16, **kw).cpu()
+    want, terms = bo.scores(q, c.bounds(), c.lengths, c.tables, SCALE, 16, c.ks, **({} if scale is None else dict(query_scale=scale)))
+    live = want > -math.inf
+    assert torch.equal(got > -math.inf, live)
+    assert ((got.double() - want).abs()[live] <= (260 * 2.0 ** -23) * terms[live]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hkv,group", [(1, 4), (2, 4), (3, 20), (1, 64), (8, 4)])
 def test_scores_of_long_contexts_are_the_same_every_time(hkv, group):
     """Many tiles for every SM, few kv heads: rings whose slots pass between warps."""

@@ -97,6 +97,16 @@ __device__ __forceinline__ uint32_t f16x2_min0(uint32_t v) {
   asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0u));
   return r;
 }
+// The larger of two, NaN if one is: a query row that is no number has no bound, and its pages' scores say so.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float quad_max_or_nan(float v) {
+  v = max_or_nan(v, __shfl_xor_sync(kFullMask, v, 1));
+  return max_or_nan(v, __shfl_xor_sync(kFullMask, v, 2));
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
@@ -141,18 +151,27 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   grid_dependency_wait();
   grid_launch_dependents();   // (the dependent waits for this grid's end before it reads the scores)
 
-  // ---- pages of every sequence, and tiles of 16 pages summed over the sequences (every CTA for itself)
+  // ---- pages of every sequence, and tiles of 16 pages summed over the sequences (every CTA for itself).  The
+  // lengths are read side by side before anything is summed: 1 024 sequences of 128 to 512 tokens take 22 us, and
+  // took 34 when a thread read its four one after the other and CTAs, not warps, went over the rows for -inf.
   const int64_t cap = (int64_t)p.width * p.block_size;
   {
+    bool too_long = false;
+#pragma unroll 4
+    for (int s = tid; s < p.S; s += threads) {
+      const int ctx = __ldg(p.context_lens + s);
+      too_long = too_long || ctx > cap;
+      const uint32_t len = ctx <= 0 ? 0u : (uint32_t)ctx;
+      const uint32_t pages = len / (uint32_t)p.block_size + (len % (uint32_t)p.block_size ? 1u : 0u);
+      seq_pages[s] = (int)min((uint32_t)p.width, pages);
+    }
+    if (too_long && blockIdx.x == 0 && p.status) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
     const int chunk = (p.S + threads - 1) / threads;
+    if (chunk > 1) __syncthreads();   // (else each thread has written what it reads)
     const int beg = min(tid * chunk, p.S), end = min(beg + chunk, p.S);
     int sum = 0;
     for (int s = beg; s < end; ++s) {
-      const int ctx = p.context_lens[s];
-      if (ctx > cap && blockIdx.x == 0 && p.status) atomicOr(p.status, PA_DEV_CTX_TOO_LONG);
-      const int pages = ctx <= 0 ? 0 : (int)min((int64_t)p.width, ((int64_t)ctx + p.block_size - 1) / p.block_size);
-      seq_pages[s] = pages;
-      tile_off[s + 1] = (pages + kScoreTilePages - 1) / kScoreTilePages;
+      tile_off[s + 1] = (seq_pages[s] + kScoreTilePages - 1) / kScoreTilePages;
       sum += tile_off[s + 1];
     }
     int incl = sum;
@@ -276,11 +295,12 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   }
 
   // -------------------------------------------------------------------- the multiplying warps
-  // ---- pages without tokens: nothing to choose (a (sequence, kv head) after the other over the CTAs)
-  for (int64_t r = blockIdx.x; r < (int64_t)p.S * p.Hkv; r += gridDim.x) {
-    const int s = (int)(r / p.Hkv), h = (int)(r - (int64_t)s * p.Hkv);
+  // ---- pages without tokens: nothing to choose ((sequence, kv head, 1024 pages) after the other over the warps)
+  const int parts = (p.width + 1023) >> 10;
+  for (int64_t r = (int64_t)blockIdx.x * kScoreWarps + warp; r < (int64_t)p.S * parts * p.Hkv; r += (int64_t)gridDim.x * kScoreWarps) {
+    const int sp = (int)(r / p.Hkv), h = (int)(r - (int64_t)sp * p.Hkv), s = sp / parts, beg = (sp - s * parts) << 10;
     float* out = p.scores + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
-    for (int i = seq_pages[s] + tid; i < p.width; i += kScoreWarps * 32) out[i] = -INFINITY;
+    for (int i = max(seq_pages[s], beg) + lane; i < min(p.width, beg + 1024); i += 32) out[i] = -INFINITY;
   }
   // A warp works for one kv head of the group and takes the tiles k with k % step == sub.
   const int g = lane >> 2, t = lane & 3;
@@ -290,6 +310,32 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   int mine = sub, slot = sub;         // this warp's next tile and its slot
   uint32_t phase = 0;
   bool dead = false;                  // a wait ran out: go through the barriers, touch nothing
+  // A segment's query rows, eight a warp (there are at most 64): a quad of lanes per row, lane t the 32 dims of its
+  // quarter.  Padding rows repeat row 0, which changes no maximum.  They are requested a segment ahead:
+  // 32 long sequences take 31.8 us so and 33.1 without, 256 of 1 024 to 4 096 tokens 23.4 and 24.5.
+  static_assert(kScoreWarps * 8 >= kScoreMaxRows, "a warp's rows of the query are one group of eight");
+  uint4 raw[4];
+  float raw_scale = 1.0f;
+  auto fetch_query = [&](const Place& at) {
+    const int head0 = at.group * hpc, heads = min(hpc, p.Hkv - head0);
+    const int r = warp * 8 + g, h = r / kRows;
+    if (warp * 8 >= heads * kRows) return;
+    int row = r - h * kRows;
+    if (row >= p.rows) row = 0;
+    const int64_t grow = (int64_t)(head0 + h) * p.rows + row;
+    const uint8_t* src = p.q + (int64_t)at.seq * p.q_stride_seq;
+    if (p.q_is_fp8) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) raw[e] = __ldg(reinterpret_cast<const uint4*>(src + grow * kD + t * 32) + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw[e] = __ldg(reinterpret_cast<const uint4*>(src + grow * (kD * 2) + t * 64) + e);
+    }
+    if (p.q_quant_mode == PA_QUANT_PER_TENSOR) raw_scale = __ldg(p.q_scale);
+    if (p.q_quant_mode == PA_QUANT_PER_TOKEN) raw_scale = __ldg(p.q_scale + (int64_t)at.seq * p.q_scale_stride_seq + grow);
+  };
+  constexpr bool kAhead = NB8 <= 4;   // (64 rows need the registers)
+  if (kAhead && n_tiles > 0) fetch_query(a);
   while (k < n_tiles) {
     // a segment: tiles of one sequence and head group
     const int seq = a.seq, tile_a = a.tile;
@@ -297,22 +343,17 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
     const int head0 = a.group * hpc, heads = min(hpc, p.Hkv - head0);
     const int pages = seq_pages[seq];
 
-    // ---- the group's query rows: a quad of lanes per row, lane t the 32 dims of its quarter.  Padding rows
-    // repeat row 0, which changes no maximum.  Within each group of four dims the order is 0, 2, 1, 3
-    // (what the e4m3 unpacking below yields).
+    // ---- the group's query rows.  Within each group of four dims the order is 0, 2, 1, 3 (what the e4m3
+    // unpacking below yields).
+    if (!kAhead) fetch_query(a);
     if (k > 0) tc::named_barrier_sync(1, kScoreWarps * 32);   // the rows of the segment before are no longer read
-    for (int r0 = warp * 8; r0 < heads * kRows; r0 += kScoreWarps * 8) {
-      const int r = r0 + g, h = r / kRows;
-      int row = r - h * kRows;
-      if (row >= p.rows) row = 0;
-      const int64_t grow = (int64_t)(head0 + h) * p.rows + row;
+    if (warp * 8 < heads * kRows) {
+      const int r = warp * 8 + g;
       float x[32];
       if (p.q_is_fp8) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * kD + t * 32);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint4 v = __ldg(src + e);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t lo, hi;
@@ -324,25 +365,25 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
           }
         }
       } else {
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)seq * p.q_stride_seq + grow * (kD * 2) + t * 64);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint4 v = __ldg(src + e);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[e * 8 + j * 2] = bf16_lo_to_f32(w[j]), x[e * 8 + j * 2 + 1] = bf16_hi_to_f32(w[j]);
         }
       }
       float amax = 0.f;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
-      amax = quad_max(amax);
+      for (int e = 0; e < 32; ++e) amax = max_or_nan(amax, fabsf(x[e]));
+      amax = quad_max_or_nan(amax);
       // power of two that brings the row's largest element into [2^14, 2^15)
       const int be = (int)((__float_as_uint(amax) >> 23) & 0xff);
       float pre = 1.0f, back = 1.0f;
       if (be > 0 && be < 255) {
         pre = __uint_as_float((uint32_t)min(253, 254 + 14 - be) << 23);
         back = 1.0f / pre;   // a power of two
+      } else if (amax != amax) {
+        back = amax;         // (the halves of the operand below are zero for NaN)
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -353,12 +394,7 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
         v.w = pack_f16x2(x[e * 8 + 5] * pre, x[e * 8 + 7] * pre);
         *reinterpret_cast<uint4*>(smem + r * kScoreRowBytes + t * 64 + e * 16) = v;
       }
-      if (t == 0) {
-        float qs = 1.0f;
-        if (p.q_quant_mode == PA_QUANT_PER_TENSOR) qs = __ldg(p.q_scale);
-        if (p.q_quant_mode == PA_QUANT_PER_TOKEN) qs = __ldg(p.q_scale + (int64_t)seq * p.q_scale_stride_seq + grow);
-        factor[r] = back * 256.0f * qs * p.softmax_scale;   // 2^8: the bounds' f16 values are the codes times 2^-8
-      }
+      if (t == 0) factor[r] = back * 256.0f * raw_scale * p.softmax_scale;   // 2^8: the bounds' f16 values are the codes times 2^-8
     }
     tc::named_barrier_sync(1, kScoreWarps * 32);
 
@@ -393,6 +429,9 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       }
     }
     float* out = p.scores + (int64_t)seq * p.out_stride_seq + (int64_t)(head0 + my_head) * p.out_stride_head;
+    a.tile += count;
+    if (a.tile >= tile_off[seq + 1] - tile_off[seq]) next_seq(a);
+    if (kAhead && k + count < n_tiles) fetch_query(a);
 #pragma unroll 1
     while (mine < k + count) {
       if (!dead && !__all_sync(kFullMask, mbar_wait(smem_addr(&bar_full[slot]), phase))) {
@@ -446,11 +485,11 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
           constexpr float kLow = kKeep ? 0x1p-8f : 1.0f;   // converted codes carry their true value
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            best[i] = fmaxf(best[i], fmaxf(fmaf(acc[0][n][2 * i], kLow, acc[1][n][2 * i]) * f.x,
-                                           fmaf(acc[0][n][2 * i + 1], kLow, acc[1][n][2 * i + 1]) * f.y));
+            best[i] = max_or_nan(best[i], max_or_nan(fmaf(acc[0][n][2 * i], kLow, acc[1][n][2 * i]) * f.x,
+                                                     fmaf(acc[0][n][2 * i + 1], kLow, acc[1][n][2 * i + 1]) * f.y));
         }
-        best[0] = quad_max(best[0]);
-        best[1] = quad_max(best[1]);
+        best[0] = quad_max_or_nan(best[0]);
+        best[1] = quad_max_or_nan(best[1]);
         const int in_tile = g + 8 * t, page = (tile_a + mine - k) * kScoreTilePages + in_tile;   // what lanes t = 0, 1 store
         if (t < 2 && page < pages) {
           const float ks = p.k_scale ? __uint_as_float(lds32(tile + kScoreTilePages * pitch + (in_tile * hpc + my_head) * 4)) : 1.0f;
@@ -464,8 +503,6 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       if (slot >= p.slots) slot -= p.slots, phase ^= 1;
     }
     k += count;
-    a.tile += count;
-    if (a.tile >= tile_off[seq + 1] - tile_off[seq]) next_seq(a);
   }
 }
 
