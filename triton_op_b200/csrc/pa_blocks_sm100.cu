@@ -121,7 +121,7 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   }
   const int64_t cap = (int64_t)dev->sm_count * 5;   // what is resident at a time
   // Pages of 64 tokens that get a few rows each (fewer than a run of 16 per sequence, on average), more of them
-  // than four warps apiece could take at once: a warp each (5.3 us against 7.5 for a row of 64 sequences with
+  // than four warps apiece could take at once: a warp each (5.1 us against 7.5 for a row of 64 sequences with
   // eight kv heads; prompts, whose pages have four full runs, would lose: 31 us against 25 for 16 000 rows).
   const bool lone = p->block_size == 64 && p->num_tokens < 16 * (int64_t)p->num_seqs && units > cap;
   const int per_cta = p->block_size == 16 || lone ? 4 : 1;
