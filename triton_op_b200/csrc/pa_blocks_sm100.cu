@@ -109,17 +109,21 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
   if (units > (1 << 30)) return PA_ERR_TOO_LARGE;
   const size_t smem = (size_t)(p->num_seqs + 1) * 4;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Pages of 1024 tokens that get many rows at a time (64 or more per sequence, on average): sixteen warps a
-  // page, or, while all pages find room at once that way, a cluster of eight CTAs.
-  if (p->block_size == 1024 && p->num_tokens >= 64 * (int64_t)p->num_seqs) {
+  const int64_t cap = (int64_t)dev->sm_count * 5;   // CTAs of four warps that are resident at a time
+  // Pages of 1024 tokens.  Four warps a page where a sequence brings a few rows (fewer than 64 on average), and up to
+  // 256 where there are more pages than such CTAs at a time (40 sequences of 100 rows, eight kv heads: 11.5 us against
+  // 13.8 with eight warps and 20.5 with sixteen; of 400 rows 36, 41 and 41, but lengths from 1 to 900 want more:
+  // 84, 78 and 75).  For more rows eight warps (of 1 000 rows: 46 us, with sixteen 49), or, while all pages find
+  // room at once that way, a cluster of eight CTAs.
+  const int64_t few = units > cap ? 256 : 64;
+  if (p->block_size == 1024 && p->num_tokens >= few * p->num_seqs) {
     constexpr int kCluster = 8;
     if (units <= 2 * dev->sm_count / kCluster)   // (two of its CTAs fit an SM)
       return launch(blk ? pa::pa_cache_append_kernel<1024, 64, true, kCluster> : pa::pa_cache_append_kernel<1024, 64, false, kCluster>,
                     dim3((unsigned)(units * kCluster)), 256, smem, st, k, kCluster);
-    const int64_t grid = units < dev->sm_count ? units : dev->sm_count;
-    return launch(blk ? pa::pa_cache_append_kernel<1024, 16, true> : pa::pa_cache_append_kernel<1024, 16, false>, dim3((unsigned)grid), 512, smem, st, k);
+    const int64_t grid = units < 2 * dev->sm_count ? units : 2 * dev->sm_count;
+    return launch(blk ? pa::pa_cache_append_kernel<1024, 8, true> : pa::pa_cache_append_kernel<1024, 8, false>, dim3((unsigned)grid), 256, smem, st, k);
   }
-  const int64_t cap = (int64_t)dev->sm_count * 5;   // what is resident at a time
   // Pages of 64 tokens that get a few rows each (fewer than a run of 16 per sequence, on average), more of them
   // than four warps apiece could take at once: a warp each (5.1 us against 7.5 for a row of 64 sequences with
   // eight kv heads; prompts, whose pages have four full runs, would lose: 31 us against 25 for 16 000 rows).

@@ -18,7 +18,7 @@
 // A unit of work is (page, kv head, key or value), and all of it belongs to one group of warps: the
 // scale is a maximum over every row the page gets, and two writers of one page would race on it.
 // Each warp takes 16 consecutive slots of the page, whose rows stay in registers between the
-// maximum and the store.  A page of 1024 tokens is 64 such runs.  Sixteen warps take four each and read
+// maximum and the store.  A page of 1024 tokens is 64 such runs.  Eight warps take eight each and read
 // the rows twice; where there are fewer pages than could keep the GPU busy that way, a page is shared by
 // a cluster of eight CTAs that find the maximum through each other's shared memory (9 us against 17 for
 // two prompts of 2 200 and 3 300 tokens, one kv head, when that was chosen, 5.9 since; for many pages the clusters'
@@ -27,7 +27,7 @@
 // stored as 16-byte chunks [d/16][token][16], values as 16 tokens of a head dim, 16 bytes too;
 // values of a run that is not whole are merged with the bytes that are there.
 // What bounds it: 512 bytes read and 256 written per (token, kv head).  A prompt is bound by the
-// instructions that quantise it: 16 000 tokens of eight kv heads take 22 us in pages of 16, 25 in pages of 64 and 34 in
+// instructions that quantise it: 16 000 tokens of eight kv heads take 22 us in pages of 16, 25 in pages of 64 and 33 in
 // pages of 1024 (15 at the copy bandwidth).  A row for each of 64 sequences takes 4.3, 5.1 and 9.1 us: launch
 // latency and one chain of loads, which is why whatever a page holds already is asked for at once.
 #pragma once
@@ -169,7 +169,7 @@ static __device__ __noinline__ void rescale_runs(uint8_t* cache, bool is_v, bool
 // BS: tokens per page.  WPU: warps per unit.  PER_BLOCK: scales per (page, kv head), else per tensor.
 // CLUSTER: CTAs that share a unit.
 template <int BS, int WPU, bool PER_BLOCK, int CLUSTER = 1>
-__global__ void __launch_bounds__(WPU / CLUSTER > 4 ? WPU / CLUSTER * 32 : 128, CLUSTER > 1 ? 2 : (WPU > 4 ? 1 : 5))
+__global__ void __launch_bounds__(WPU / CLUSTER > 4 ? WPU / CLUSTER * 32 : 128, WPU > 4 ? 2 : 5)
 pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
   constexpr int kCtaWarps = WPU / CLUSTER;                          // warps of a unit in one CTA
   constexpr int kThreads = kCtaWarps > 4 ? kCtaWarps * 32 : 128;
