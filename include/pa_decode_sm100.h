@@ -40,7 +40,8 @@ typedef enum PaStatus {
 
 typedef enum PaDType {
   PA_DT_BF16 = 0,
-  PA_DT_E4M3FN = 1            /* OCP e4m3fn, max 448 */
+  PA_DT_E4M3FN = 1,           /* OCP e4m3fn, max 448 */
+  PA_DT_F32 = 2               /* tmp_out only */
 } PaDType;
 
 /* Quantisation mode of a scale argument; the first three values are the reference's own
@@ -101,7 +102,7 @@ typedef struct PaDecodeParams {
    * They need not be zeroed: every partition the reduce reads is written by the partition kernel. */
   float* exp_sums;             /* [S, Hkv, P, eqG] fp32 */
   float* max_logits;           /* [S, Hkv, P, eqG] fp32 */
-  void* tmp_out;               /* [S, Hkv, P, eqG, D] out_dtype, already divided by exp_sums */
+  void* tmp_out;               /* [S, Hkv, P, eqG, D] tmp_dtype, already divided by exp_sums */
   int32_t* status;             /* optional device int32, OR-ed with PA_DEV_* bits */
   uint64_t* trace;             /* optional tuning aid: device buffer of PA_TRACE_WORDS uint64 that
                                 * receives SM-clock stamps of CTA 0's pipeline roles; NULL normally.
@@ -167,6 +168,9 @@ typedef struct PaDecodeParams {
   int32_t tune_early;          /* -1: the tcgen05 kernel reads nothing before its dependency wait; 0 (default): it builds
                                 * its partition index from the context lengths before the wait and checks it
                                 * against them after it */
+  int32_t tmp_dtype;           /* PaDType of tmp_out: PA_DT_BF16 (0), the reference's choice, rounds every partition's output
+                                * to 8 bits once more; PA_DT_F32 keeps it whole (kv_quant_mode PA_QUANT_PER_BLOCK, or
+                                * none / per tensor in 256-token partitions of an e4m3fn cache) */
 } PaDecodeParams;
 
 /* Partition kernel followed by the reduce kernel on `stream` (a cudaStream_t); one launch that

@@ -155,8 +155,8 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
 
 def attention_tolerance(out, mass, floor) -> torch.Tensor:
     """What the kernel's roundings can add up to: probabilities as two e4m3 numbers (2^-7 of each, and 2^-18
-    of the largest weighted value scale below the subnormals), bf16 partial outputs (2^-8 of each) and the
-    bf16 result (2^-8), with 2^-12 for everything that is held in 32 bits."""
+    of the largest weighted value scale below the subnormals), bf16 partial outputs (2^-8 of each; only where a
+    caller's workspaces hold them so) and the bf16 result (2^-8), with 2^-12 for everything that is held in 32 bits."""
     return (2.0 ** -7 + 2.0 ** -8 + 2.0 ** -12) * mass + 2.0 ** -8 * out.abs() + 2.0 ** -18 * floor
 
 

@@ -1,0 +1,92 @@
+"""Calls around a cache with scales per (page, kv head) that are easy to get wrong: where a rounding hides, where
+two writers meet, what the host path refuses, host threads, far pages."""
+import math
+
+import pytest
+import torch
+
+import triton_op_b200 as pa
+from oracle import blocks_oracle as bo
+from test_block_cache import D, FP8, SCALE, Cache, cuda, decode, transposed
+from triton_op_b200 import PaArgumentError, _lib
+
+
+# ----------------------------------------------------------------------------- attention: what is rounded, and when
+def cancelling(c):
+    """Values whose means are large in every partition of 256 tokens and cancel between them."""
+    for s, n in enumerate(c.lengths.tolist()):
+        for i in range(-(-n // c.bs)):
+            page = int(c.tables[s, i])
+            v = c.value[page].float().abs() + 64.0                       # [Hkv, D, bs]
+            sign = 1.0 - 2.0 * ((torch.arange(c.bs) + i * c.bs) // 256 % 2)
+            c.value[page] = (v * sign).clamp(-448, 448).to(FP8)
+
+
+def assert_rounded_once(got, want):
+    """Equal logits are exact probabilities (one e4m3 number each, no remainder), so what is left are sums in
+    32 bits -- 256 products a partition, which the tensor core may truncate (2^-23 each), and 16 partitions at most -- and the
+    bf16 result, half a step of its own value."""
+    out, mass, _ = want
+    err = (got.double() - out).abs()
+    assert bool((err <= 2.0 ** -8 * out.abs() + 2.0 ** -14 * mass).all()), float((err / mass).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,group,query_len", [(16, 4, 1), (16, 8, 1), (16, 8, 2), (64, 2, 1), (64, 16, 1), (1024, 6, 1), (1024, 16, 4)])
+def test_partial_outputs_are_not_rounded(bs, group, query_len):
+    c = Cache([2000, 257, 512, 3900], 2, bs, seed=bs + group)
+    cancelling(c)
+    c.vs[:] = 2.0 ** -3
+    q = torch.zeros_like(c.query(group, query_len))
+    got = decode(c, q, query_len=query_len)
+    assert_rounded_once(got, bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, query_len))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scales", ["none", "one value", "per page"])
+@pytest.mark.parametrize("hkv", [1, 3])
+def test_partial_outputs_are_not_rounded_with_a_table_per_head(hkv, scales):
+    c = Cache([2000, 600], hkv, 16, seed=hkv)
+    cancelling(c)
+    c.vs[:] = 0.25
+    q = torch.zeros_like(c.query(4))
+    ks, vs = dict([("none", (None, None)), ("one value", (torch.tensor(0.5), torch.tensor(0.25))), ("per page", (c.ks, c.vs))])[scales]
+    tables = c.tables[:, None].expand(-1, hkv, -1).contiguous()
+    out = torch.full(q.shape, math.nan, dtype=torch.bfloat16, device="cuda")
+    res = pa.paged_attention_decode(out, *cuda(q, c.key, c.value, c.lengths, tables), SCALE, 1, 2000, torch.bfloat16, None, *cuda(ks, vs))
+    assert res["temporary_output"].dtype == torch.float32
+    assert_rounded_once(out.cpu(), bo.attention(q, c.key, c.value, ks, vs, tables, c.lengths, SCALE, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("parts", [40, 140])
+@pytest.mark.parametrize("seqs", [1, 40])
+def test_many_partitions_are_merged_from_whole_outputs(parts, seqs):
+    """Each way of merging: a warp, eight warps or sixteen warps a row."""
+    c = Cache([parts * 256 - 9] + [700] * (seqs - 1), 2, 64, seed=parts)
+    cancelling(c)
+    c.vs[:] = 0.5
+    q = torch.zeros_like(c.query(8))
+    got = decode(c, q)
+    out, mass, _ = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1)
+    err = (got.double() - out).abs()
+    assert bool((err <= 2.0 ** -8 * out.abs() + 2.0 ** -14 * mass).all()), float((err / mass).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_workspaces_of_the_caller(dtype):
+    """A workspace in 32 bits rounds nothing; one in the output's type rounds each partition (2^-8 of it) as it says."""
+    c = Cache([2000, 300], 2, 16, seed=4)
+    cancelling(c)
+    c.vs[:] = 0.5
+    q = torch.zeros_like(c.query(4))
+    shape = (2, 2, 8, 4)
+    kw = dict(exp_sums=torch.empty(shape, device="cuda"), max_logits=torch.empty(shape, device="cuda"),
+              tmp_output=torch.empty(*shape, D, dtype=dtype, device="cuda"))
+    got = decode(c, q, **kw)
+    out, mass, _ = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1)
+    slack = 2.0 ** -14 if dtype == torch.float32 else 2.0 ** -14 + 2.0 ** -8
+    assert bool(((got.double() - out).abs() <= 2.0 ** -8 * out.abs() + slack * mass).all())
+    with pytest.raises(PaArgumentError):
+        decode(c, q, **{**kw, "tmp_output": torch.empty(*shape, D, dtype=torch.float16, device="cuda")})

@@ -17,7 +17,7 @@ from .build import CALLS_PATH, LIB_PATH
 PA_ABI_VERSION = 3
 
 PA_OK = 0
-PA_DT_BF16, PA_DT_E4M3FN = 0, 1
+PA_DT_BF16, PA_DT_E4M3FN, PA_DT_F32 = 0, 1, 2
 PA_QUANT_NONE, PA_QUANT_PER_TENSOR, PA_QUANT_PER_TOKEN, PA_QUANT_PER_BLOCK = -1, 0, 1, 2
 PA_V_NORMAL, PA_V_TRANSPOSED = 0, 1
 PA_DEV_WAIT_TIMEOUT, PA_DEV_BAD_PAGE_ID, PA_DEV_CTX_TOO_LONG, PA_DEV_BAD_RANGE = 1, 2, 4, 8
@@ -53,7 +53,7 @@ class PaDecodeParams(C.Structure):
         + [(n, C.c_int32) for n in (
             "q_dtype", "kv_dtype", "out_dtype", "q_quant_mode", "kv_quant_mode", "v_layout")]
         + [("softmax_scale", C.c_float)]
-        + [(n, C.c_int32) for n in ("tune_warps", "tune_stages", "tune_ctas", "tune_vstages", "tune_fuse", "tune_early")]
+        + [(n, C.c_int32) for n in ("tune_warps", "tune_stages", "tune_ctas", "tune_vstages", "tune_fuse", "tune_early", "tmp_dtype")]
     )
 
 

@@ -161,7 +161,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t parts = longest <= kPartition ? 1 : (longest + kPartition - 1) / kPartition;
     const at::TensorOptions fp32 = out->options().dtype(at::kFloat);
     at::Tensor sums = at::empty({s, h, parts, rows}, fp32), tops = at::empty({s, h, parts, rows}, fp32);
-    at::Tensor tmp = at::empty({s, h, parts, rows, kD}, out->options());
+    at::Tensor tmp = at::empty({s, h, parts, rows, kD}, fp32);   // (bf16 would round every partition once more)
     PaDecodeParams p;
     std::memset(&p, 0, sizeof(p));
     p.struct_size = sizeof(p);
@@ -211,6 +211,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.q_dtype = PA_DT_BF16;
     p.kv_dtype = PA_DT_E4M3FN;
     p.out_dtype = PA_DT_BF16;
+    p.tmp_dtype = PA_DT_F32;
     p.q_quant_mode = PA_QUANT_NONE;
     p.kv_quant_mode = mode;
     p.v_layout = transposed ? PA_V_TRANSPOSED : PA_V_NORMAL;

@@ -129,6 +129,7 @@ int validate(const PaDecodeParams* p, bool need_partition_inputs, bool need_out)
   if (p->head_size != pa::kD) return PA_ERR_UNSUPPORTED;
   if (p->query_len > 4) return PA_ERR_UNSUPPORTED;  // reference: QUERY_SEQ_LEN <= 4
   if (p->out_dtype != PA_DT_BF16) return PA_ERR_UNSUPPORTED;
+  if (p->tmp_dtype != PA_DT_BF16 && p->tmp_dtype != PA_DT_F32) return PA_ERR_UNSUPPORTED;
   if (!p->context_lens || !p->exp_sums || !p->max_logits || !p->tmp_out) return PA_ERR_NULL_POINTER;
   if (need_out && !p->out) return PA_ERR_NULL_POINTER;
   if (p->partition_size % p->block_size != 0 && p->block_size % p->partition_size != 0)
@@ -166,8 +167,9 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   const int kv_item = bf16_kv ? 2 : 1;  // bytes per cache element
   if (bf16_kv && p->kv_quant_mode == PA_QUANT_PER_TOKEN) return PA_ERR_UNSUPPORTED;
   if (p->kv_quant_mode < PA_QUANT_NONE || p->kv_quant_mode > PA_QUANT_PER_BLOCK) return PA_ERR_UNSUPPORTED;
-  // Scales per (page, kv head), or tables per kv head: the tcgen05 kernel's BLK form, 256-token partitions.
-  const bool blk = p->kv_quant_mode == PA_QUANT_PER_BLOCK || bt_stride_head != 0;
+  // Scales per (page, kv head), tables per kv head, or partial outputs in fp32: the tcgen05 kernel's BLK form,
+  // 256-token partitions.
+  const bool blk = p->kv_quant_mode == PA_QUANT_PER_BLOCK || bt_stride_head != 0 || p->tmp_dtype == PA_DT_F32;
   if (blk) {
     if (bf16_kv || p->partition_size != pa::tc::kItemTokens || p->tune_warps != 0) return PA_ERR_UNSUPPORTED;
     if (p->kv_quant_mode == PA_QUANT_PER_TOKEN) return PA_ERR_UNSUPPORTED;
@@ -256,6 +258,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   k.tmp_stride_head = p->tmp_stride_head;
   k.tmp_stride_part = p->tmp_stride_part;
   k.tmp_stride_row = p->tmp_stride_row;
+  k.tmp_f32 = p->tmp_dtype == PA_DT_F32;
   k.q_quant_mode = p->q_quant_mode;
   k.kv_quant_mode = p->kv_quant_mode;
   plan->blk = blk;
@@ -618,9 +621,11 @@ int launch_reduce(const PaDecodeParams* p, float* tri_m, float* tri_l, float* tr
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = wpr == 1   ? cudaLaunchKernelEx(&cfg, pa::pa_reduce_kernel<1>, r)
-                  : wpr == 4 ? cudaLaunchKernelEx(&cfg, pa::pa_reduce_mid_kernel, r)
-                             : cudaLaunchKernelEx(&cfg, pa::pa_reduce_kernel<16>, r);
+  const bool f32 = p->tmp_dtype == PA_DT_F32;
+  void (*kernel)(pa::ReduceParams) = wpr == 1   ? (f32 ? pa::pa_reduce_kernel<1, true> : pa::pa_reduce_kernel<1, false>)
+                                     : wpr == 4 ? (f32 ? pa::pa_reduce_mid_kernel<true> : pa::pa_reduce_mid_kernel<false>)
+                                                : (f32 ? pa::pa_reduce_kernel<16, true> : pa::pa_reduce_kernel<16, false>);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, r);
   if (e != cudaSuccess) return cuda_fail(e);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e);
@@ -726,6 +731,7 @@ int pa_decode_noalloc_sm100(const PaDecodeParams* params, void* stream) {
   q.exp_sums = reinterpret_cast<float*>(base);
   q.max_logits = reinterpret_cast<float*>(base + f32_bytes);
   q.tmp_out = base + 2 * f32_bytes;
+  q.tmp_dtype = PA_DT_BF16;   // (what the array was sized for)
   q.ws_stride_part = eqG;
   q.ws_stride_head = eqG * params->max_partitions;
   q.ws_stride_seq = q.ws_stride_head * params->num_kv_heads;

@@ -21,7 +21,7 @@ struct KernelParams {
   const float* alibi;          // [Hkv * G] slopes or null
   float* exp_sums;
   float* max_logits;
-  uint8_t* tmp_out;            // bf16
+  uint8_t* tmp_out;            // bf16, or fp32 (tmp_f32)
   int32_t* status;             // may be null
   unsigned long long* trace;   // tuning aid: per-role clock stamps of CTA 0; null in normal operation
   // single-launch decode (the partition kernel also merges the partitions): the final output, the
@@ -67,6 +67,7 @@ struct KernelParams {
   int32_t early_start;         // build the partition index before the dependency wait (checked after it)
   int32_t team_size;           // single-launch form: CTAs per team (divides Hkv and the grid)
   int32_t off_stash;           // PAIR form of the tcgen05 kernel: where a partition's first half waits for its second
+  int32_t tmp_f32;             // partial outputs are stored as fp32 (BLK form of the tcgen05 kernel only)
 };
 
 // Fixed head of the shared-memory carve: mbarriers and the scan scratch.

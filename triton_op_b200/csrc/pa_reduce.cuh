@@ -40,7 +40,7 @@ struct ReduceParams {
   uint8_t* out;                 // bf16 [S, Hkv*eqG, D]; may be null when triples are stored
   const float* exp_sums;
   const float* max_logits;
-  const uint8_t* tmp_out;       // bf16
+  const uint8_t* tmp_out;       // bf16 or fp32 (F32 of the kernels)
   const int32_t* context_lens;
   const float* sink;            // optional [Hkv*G]: sink logit per query head, added to the row's weight sum
   float* tri_m;                 // optional fp32 triples
@@ -58,7 +58,7 @@ struct ReduceParams {
 };
 
 // One output row whose partitions (at most 32) all lie in one chunk, merged by one warp: the
-// arithmetic of pa_reduce_kernel<1> below, operation for operation, so that a decode call gives
+// arithmetic of pa_reduce_kernel<1, false> below, operation for operation, so that a decode call gives
 // the same bits whether its partitions are merged by that kernel or, in the single-launch form,
 // by a warp of the partition kernel itself.  Loads go to L2 (ld.global.cg): the partitions were
 // written by other SMs during the same launch.  lane owns head dims 4*lane..4*lane+3.
@@ -145,18 +145,53 @@ __device__ __forceinline__ uint2 ld_global_u2(const void* ptr) {
   asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(ptr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint4 ld_global_u4(const void* ptr) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float ld_global_f32(const void* ptr) {
   float v;
   asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(ptr) : "memory");
   return v;
 }
 
+// A lane's four head dims of one partial output, as bf16 or as fp32.
+template <bool F32>
+struct PartialRow;
+template <>
+struct PartialRow<false> {
+  static constexpr int kItem = 2;
+  uint2 raw;
+  __device__ __forceinline__ void clear() { raw = make_uint2(0u, 0u); }
+  __device__ __forceinline__ void load(const void* ptr) { raw = ld_global_u2(ptr); }
+  __device__ __forceinline__ void add(float w, float (&acc)[4]) const {
+    acc[0] = fmaf(w, bf16_lo_to_f32(raw.x), acc[0]);
+    acc[1] = fmaf(w, bf16_hi_to_f32(raw.x), acc[1]);
+    acc[2] = fmaf(w, bf16_lo_to_f32(raw.y), acc[2]);
+    acc[3] = fmaf(w, bf16_hi_to_f32(raw.y), acc[3]);
+  }
+};
+template <>
+struct PartialRow<true> {
+  static constexpr int kItem = 4;
+  uint4 raw;
+  __device__ __forceinline__ void clear() { raw = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const void* ptr) { raw = ld_global_u4(ptr); }
+  __device__ __forceinline__ void add(float w, float (&acc)[4]) const {
+    acc[0] = fmaf(w, __uint_as_float(raw.x), acc[0]);
+    acc[1] = fmaf(w, __uint_as_float(raw.y), acc[1]);
+    acc[2] = fmaf(w, __uint_as_float(raw.z), acc[2]);
+    acc[3] = fmaf(w, __uint_as_float(raw.w), acc[3]);
+  }
+};
+
 // One warp's share of a row: the 32-partition chunks `first`, `first + step`, ... folded into a
 // running (maximum M, weight sum W, weighted output acc).  Partitions are taken 32 at a time
 // (lane = partition for the max / weight, then FLIGHT partial-output rows in flight per step).
 // The first FLIGHT rows of a chunk are requested together with the maxima and sums, so the usual
 // row (at most 16 partitions) costs one memory round trip.
-template <int FLIGHT>
+template <int FLIGHT, bool F32>
 __device__ __forceinline__ void reduce_chunks(const ReduceParams& p, const RowRef& a, int first, int step, int lane,
                                               float& M, float& W, float (&acc)[4]) {
   for (int p0 = first * 32; p0 < a.np; p0 += 32 * step) {
@@ -167,11 +202,18 @@ __device__ __forceinline__ void reduce_chunks(const ReduceParams& p, const RowRe
       m = ld_global_f32(p.max_logits + a.ws_base + (int64_t)pi * p.ws_stride_part);
       l = ld_global_f32(p.exp_sums + a.ws_base + (int64_t)pi * p.ws_stride_part);
     }
-    const uint8_t* part0 = p.tmp_out + 2 * (a.tmp_base + (int64_t)p0 * p.tmp_stride_part);   // this lane's bytes of partition p0
-    const int64_t part_bytes = 2 * p.tmp_stride_part;
-    uint2 raw[FLIGHT];  // requested before the maximum is known
+    constexpr int kItem = PartialRow<F32>::kItem;
+    const uint8_t* part0 = p.tmp_out + kItem * (a.tmp_base + (int64_t)p0 * p.tmp_stride_part);   // this lane's bytes of partition p0
+    const int64_t part_bytes = kItem * p.tmp_stride_part;
+    PartialRow<F32> row[FLIGHT];  // requested before the maximum is known
+    auto request = [&](int j0) {
 #pragma unroll
-    for (int j = 0; j < FLIGHT; ++j) raw[j] = j < cnt ? ld_global_u2(part0 + j * part_bytes) : make_uint2(0u, 0u);
+      for (int j = 0; j < FLIGHT; ++j) {
+        if (j0 + j < cnt) row[j].load(part0 + (j0 + j) * part_bytes);
+        else row[j].clear();
+      }
+    };
+    request(0);
     float cm = (l > 0.f) ? m : -INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(kFullMask, cm, o));
@@ -185,20 +227,13 @@ __device__ __forceinline__ void reduce_chunks(const ReduceParams& p, const RowRe
     }
     const float w = (l > 0.f && m > -INFINITY) ? l * expf(m - M) : 0.f;
     for (int j0 = 0; j0 < cnt; j0 += FLIGHT) {
-      if (j0 > 0) {
-#pragma unroll
-        for (int j = 0; j < FLIGHT; ++j)
-          raw[j] = (j0 + j) < cnt ? ld_global_u2(part0 + (j0 + j) * part_bytes) : make_uint2(0u, 0u);
-      }
+      if (j0 > 0) request(j0);
 #pragma unroll
       for (int j = 0; j < FLIGHT; ++j) {
         const float wj = __shfl_sync(kFullMask, w, (j0 + j) & 31);
         if ((j0 + j) < cnt && wj != 0.f) {  // a zero-weight partition may hold anything
           W += wj;
-          acc[0] = fmaf(wj, bf16_lo_to_f32(raw[j].x), acc[0]);
-          acc[1] = fmaf(wj, bf16_hi_to_f32(raw[j].x), acc[1]);
-          acc[2] = fmaf(wj, bf16_lo_to_f32(raw[j].y), acc[2]);
-          acc[3] = fmaf(wj, bf16_hi_to_f32(raw[j].y), acc[3]);
+          row[j].add(wj, acc);
         }
       }
     }
@@ -264,7 +299,8 @@ __device__ __forceinline__ void finish_row(const ReduceParams& p, const RowRef& 
 // after the other; with WPR = 16 the warps of a CTA take the 32-partition chunks of ONE row
 // round-robin and combine their running (max, sum, weighted output) through shared memory.
 // (Rows of up to 128 partitions have a kernel of their own below.)
-template <int WPR>
+// F32: the partial outputs are fp32 (twice the registers for a row in flight, so fewer rows).
+template <int WPR, bool F32>
 __global__ void __launch_bounds__(WPR == 1 ? 128 : 512) pa_reduce_kernel(const __grid_constant__ ReduceParams p) {
   static_assert(WPR == 1 || WPR == 16, "one warp per row (four rows per CTA) or sixteen");
   constexpr int kWarps = WPR == 1 ? 4 : 16;
@@ -288,7 +324,7 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 512) pa_reduce_kernel(const _
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   float W = 0.f;
   // rows in flight: a 16-warp row has one 32-partition chunk per warp, taken in one round trip
-  reduce_chunks<WPR == 16 ? 32 : 16>(p, a, slice, WPR, lane, M, W, acc);
+  reduce_chunks<WPR == 16 ? (F32 ? 16 : 32) : 16, F32>(p, a, slice, WPR, lane, M, W, acc);
   if (WPR > 1) {
     // combine the warps' partial results: warp `slice` holds (M, W, acc) of its chunks
     __shared__ float s_m[kWarps], s_w[kWarps];
@@ -322,15 +358,17 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 512) pa_reduce_kernel(const _
 constexpr int kMidRows = 8;           // rows (= warps) per CTA
 constexpr int kMidChunks = 4;         // chunks per row at most (128 partitions)
 // one chunk of one row
+template <bool F32>
 __device__ __forceinline__ void reduce_one_chunk(const ReduceParams& p, const RowRef& a, int chunk, int lane,
                                                  float* M, float* W, float* acc) {
   float m = -INFINITY, w = 0.f;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  reduce_chunks<16>(p, a, chunk, kMidChunks, lane, m, w, v);
+  reduce_chunks<F32 ? 8 : 16, F32>(p, a, chunk, kMidChunks, lane, m, w, v);
   *M = m;
   *W = w;
   acc[0] = v[0], acc[1] = v[1], acc[2] = v[2], acc[3] = v[3];
 }
+template <bool F32>
 __global__ void __launch_bounds__(kMidRows * 32, 3) pa_reduce_mid_kernel(const __grid_constant__ ReduceParams p) {
   __shared__ int s_extra[kMidRows];                                   // further chunks of each row
   __shared__ float s_m[kMidRows * (kMidChunks - 1)], s_w[kMidRows * (kMidChunks - 1)];
@@ -349,7 +387,7 @@ __global__ void __launch_bounds__(kMidRows * 32, 3) pa_reduce_mid_kernel(const _
 
   // the row's first chunk
   float M, W, acc[4];
-  reduce_one_chunk(p, a, 0, lane, &M, &W, acc);
+  reduce_one_chunk<F32>(p, a, 0, lane, &M, &W, acc);
   __syncthreads();
   // further chunks of the CTA's rows, numbered row by row: task t = chunk 1 + (t - first task of its row)
   int first_task = 0, total = 0;
@@ -372,7 +410,7 @@ __global__ void __launch_bounds__(kMidRows * 32, 3) pa_reduce_mid_kernel(const _
     }
     const RowRef b = row_ref(p, row0 + owner, true, lane);
     float m2, w2, a2[4];
-    reduce_one_chunk(p, b, 1 + (t - before), lane, &m2, &w2, a2);
+    reduce_one_chunk<F32>(p, b, 1 + (t - before), lane, &m2, &w2, a2);
     if (lane == 0) {
       s_m[t] = m2;
       s_w[t] = w2;

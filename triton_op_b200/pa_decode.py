@@ -344,8 +344,10 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     if kv_mode == _lib.PA_QUANT_PER_BLOCK and (partition_size != SEQUENCE_PARTITION_SIZE or (tune and tune.get("warps"))):
         _fail(f"block kv scales run in partitions of {SEQUENCE_PARTITION_SIZE} tokens, but got partition_size {partition_size}")
     max_partitions = max(1, (int(max_sequence_length) + partition_size - 1) // partition_size)
+    # (with block scales the partial outputs keep 32 bits unless the caller's workspace holds fewer)
+    tmp_dtypes = (torch.float32, output.dtype) if kv_mode == _lib.PA_QUANT_PER_BLOCK else (output.dtype,)
     if exp_sums is None or max_logits is None or tmp_output is None:
-        ws = get_workspaces(num_seqs, num_kv_heads, max_partitions, eq_group, head_size, output.dtype, dev)
+        ws = get_workspaces(num_seqs, num_kv_heads, max_partitions, eq_group, head_size, tmp_dtypes[0], dev)
         exp_sums = ws[0] if exp_sums is None else exp_sums
         max_logits = ws[1] if max_logits is None else max_logits
         tmp_output = ws[2] if tmp_output is None else tmp_output
@@ -355,8 +357,8 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
             _fail(f"{name} must be fp32 [num_seqs, num_kv_heads, >=max_partitions, eq_group] = {ws_shape}")
     if not (exp_sums.stride() == max_logits.stride()):
         _fail("exp_sums and max_logits must share strides")
-    if not (tmp_output.dtype == output.dtype and tmp_output.dim() == 5 and tuple(tmp_output.shape[:2]) == ws_shape[:2] and tmp_output.shape[2] >= max_partitions and tuple(tmp_output.shape[3:]) == (eq_group, head_size) and tmp_output.stride(4) == 1 and tmp_output.device == dev):
-        _fail(f"tmp_output must be {output.dtype} {ws_shape + (head_size,)}")
+    if not (tmp_output.dtype in tmp_dtypes and tmp_output.dim() == 5 and tuple(tmp_output.shape[:2]) == ws_shape[:2] and tmp_output.shape[2] >= max_partitions and tuple(tmp_output.shape[3:]) == (eq_group, head_size) and tmp_output.stride(4) == 1 and tmp_output.device == dev):
+        _fail(f"tmp_output must be {' or '.join(map(str, tmp_dtypes))} {ws_shape + (head_size,)}")
 
     p = PaDecodeParams()
     p.struct_size = C.sizeof(PaDecodeParams)
@@ -402,6 +404,7 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     p.q_dtype, p.kv_dtype, p.out_dtype = q_dtype, kv_dtype, _lib.PA_DT_BF16
     p.q_quant_mode, p.kv_quant_mode, p.v_layout = q_mode, kv_mode, v_layout
     p.softmax_scale = float(softmax_scale)
+    p.tmp_dtype = _lib.PA_DT_F32 if tmp_output.dtype == torch.float32 else _lib.PA_DT_BF16
     if tune:
         p.tune_warps = int(tune.get("warps", 0))
         p.tune_stages = int(tune.get("stages", 0))
@@ -433,7 +436,7 @@ def _check_block_scales(k_scale, v_scale, key_cache) -> Tuple[int, int]:
 
 # PaDecodeParams as one packed record: filling the block field by field costs more host time than a
 # small call takes on the GPU.
-_PACK = struct.Struct("=2I17Q10i19q6if6i4x")
+_PACK = struct.Struct("=2I17Q10i19q6if7i")
 assert _PACK.size == C.sizeof(PaDecodeParams)
 
 
@@ -583,7 +586,7 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
     exp_sums = torch.empty_strided(ws_shape, ws_stride, dtype=torch.float32, device=dev)
     max_logits = torch.empty_strided(ws_shape, ws_stride, dtype=torch.float32, device=dev)
     tmp = torch.empty_strided(ws_shape + (head_size,), (num_kv_heads * w_head * head_size, w_head * head_size,
-                                                        rows * head_size, head_size, 1), dtype=torch.bfloat16, device=dev)
+                                                        rows * head_size, head_size, 1), dtype=torch.float32, device=dev)
     p = PaDecodeParams.from_buffer_copy(_PACK.pack(
         _PACK.size, _lib.PA_ABI_VERSION,
         output.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
@@ -595,7 +598,7 @@ def _build_by_block(output, query, key_cache, value_cache, sequence_lengths, blo
         num_kv_heads * w_head, w_head, rows, num_kv_heads * w_head * head_size, w_head * head_size,
         rows * head_size, head_size,
         q_dtype, _lib.PA_DT_E4M3FN, _lib.PA_DT_BF16, q_mode, kv_mode, v_layout, float(softmax_scale),
-        0, 0, 0, 0, 0, 0))
+        0, 0, 0, 0, 0, 0, _lib.PA_DT_F32))
     keep = (query, sequence_lengths, block_tables, query_scale, key_scale, value_scale)
     head_stride = t_stride[1] if per_head and num_kv_heads > 1 else 0
     return p, head_stride, keep, (exp_sums, max_logits, tmp)
@@ -645,11 +648,13 @@ def paged_attention_decode(
 
     With per-page scales or tables per kv head the call allocates its workspaces from torch's
     allocator (its own stream's, or the graph's under capture) and keeps nothing for the next call.
-    ``maximum_logits`` / ``exponential_sums`` then refer to logit + log(value scale) of the token.
+    ``maximum_logits`` / ``exponential_sums`` then refer to logit + log(value scale) of the token, and
+    ``temporary_output`` is fp32 (a ``tmp_output`` in the output dtype, which is taken with per-page
+    scales, rounds each partition's output once more).  Value scales below 2**-100 count as 2**-100.
 
     Keyword-only additions: ``partition_size`` (reference constant 256); ``exp_sums`` /
     ``max_logits`` ``[num_seqs, num_kv_heads, P, eq_group]`` fp32 and ``tmp_output``
-    ``[..., eq_group, head_size]`` in the output dtype, with ``P >= ceil(max_sequence_length /
+    ``[..., eq_group, head_size]`` in the output dtype (fp32 too with per-page scales), with ``P >= ceil(max_sequence_length /
     partition_size)`` -- when omitted they come from a per-shape cache, so the tensors in the
     returned dictionary are overwritten by the next call of the same shape; ``status``: optional
     int32 CUDA scalar the kernels OR ``PA_DEV_*`` bits into; ``time_kernels``: measure the two
