@@ -90,3 +90,33 @@ def test_workspaces_of_the_caller(dtype):
     assert bool(((got.double() - out).abs() <= 2.0 ** -8 * out.abs() + slack * mass).all())
     with pytest.raises(PaArgumentError):
         decode(c, q, **{**kw, "tmp_output": torch.empty(*shape, D, dtype=torch.float16, device="cuda")})
+
+
+# ----------------------------------------------------------------------------- scores
+def scores_of(q, bounds, lengths, tables, bs, ks, query_len=1, **kw):
+    return pa.score_blocks(*cuda(q, bounds, lengths, tables), SCALE, query_len, bs, key_scale=cuda(ks), **kw).cpu()
+
+
+def assert_scores(got, want, terms):
+    """256 products added in 32 bits, whose additions may truncate (2^-23 each), and three more roundings."""
+    live = want > -math.inf
+    assert torch.equal(got > -math.inf, live)
+    assert bool(((got.double() - want).abs()[live] <= (260 * 2.0 ** -23) * terms[live]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hkv,group", [(1, 2), (2, 3), (8, 1), (2, 12), (1, 40)])
+def test_scores_through_every_slot_of_the_ring(hkv, group):
+    """Launches that each set the ring's barriers up anew and use all of them at once, with other inputs every time."""
+    c = Cache([16 * 16 * 148 * 3 + 5, 90], hkv, 16, seed=hkv + group, spare=1)
+    for _ in range(3):
+        q = c.query(group)
+        got = scores_of(q, c.bounds(), c.lengths, c.tables, 16, c.ks)
+        ids = c.tables[0].long()
+        lo, hi = bo.codes(c.bounds()[ids]).permute(2, 1, 0, 3)                 # [Hkv, pages, D]
+        rows = q[0].double().view(hkv, group, D)
+        terms = rows.clamp_min(0) @ hi.abs().transpose(1, 2) + (-rows.clamp_max(0)) @ lo.abs().transpose(1, 2)
+        want = rows.clamp_min(0) @ hi.transpose(1, 2) + rows.clamp_max(0) @ lo.transpose(1, 2)
+        factor = SCALE * c.ks[ids, :, 0, 0].double().T
+        assert_scores(got[0], want.amax(1) * factor, terms.amax(1) * factor)
+        assert bool((got[1, :, 6:] == -math.inf).all()) and not bool((got[1, :, :6] == -math.inf).any())

@@ -143,8 +143,7 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
   if (tid < p.slots) {
     mbar_init(smem_addr(&bar_full[tid]), 33);     // the producer's arrival, and its lanes' key scale copies
     mbar_init(smem_addr(&bar_empty[tid]), hpc);   // the warps that multiply the tile
-  }
-  if (tid == 0) {
+    // (a fence orders what its own thread has done: every thread that has initialised a barrier, not one for all)
     mbar_fence_init();
     fence_proxy_async();
   }
