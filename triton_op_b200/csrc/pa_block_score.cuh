@@ -244,9 +244,9 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
     int g0, v0, id0, g1, v1, id1;
     fetch(first, g0, v0, id0);
     fetch(first + producers, g1, v1, id1);
-    int slot = first;
+    int slot = first, k = first;
     uint32_t phase = 1;
-    for (int k = first; k < n_tiles; k += producers) {
+    for (; k < n_tiles; k += producers) {
       const int group = g0, valid = v0;
       int id = id0;
       g0 = g1, v0 = v1, id0 = id1;
@@ -289,6 +289,15 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       cp_async_arrive(full);
       slot += producers;
       if (slot >= p.slots) slot -= p.slots, phase ^= 1;
+    }
+    // Nobody leaves with a copy in flight.  The multiplying warps wait for every tile, but not after a wait of theirs
+    // has run out; so each producer waits, bounded again, for its tiles that are the last in their slots (k: the
+    // first one that it has not requested).
+    for (int last = k - producers; last >= first && last + p.slots >= min(k, n_tiles); last -= producers) {
+      if (!__all_sync(kFullMask, mbar_wait(smem_addr(&bar_full[last % p.slots]), (uint32_t)(last / p.slots) & 1))) {
+        if (lane == 0 && p.status) atomicOr(p.status, PA_DEV_WAIT_TIMEOUT);
+        break;
+      }
     }
     return;
   }
