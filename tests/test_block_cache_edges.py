@@ -1,5 +1,6 @@
 """Calls around a cache with scales per (page, kv head) that are easy to get wrong: where a rounding hides, where
 two writers meet, what the host path refuses, host threads, far pages."""
+import ctypes as C
 import math
 
 import pytest
@@ -9,6 +10,7 @@ import triton_op_b200 as pa
 from oracle import blocks_oracle as bo
 from test_block_cache import D, FP8, SCALE, Cache, cuda, decode, transposed
 from triton_op_b200 import PaArgumentError, _lib
+from triton_op_b200.pa_decode import build_params
 
 
 # ----------------------------------------------------------------------------- attention: what is rounded, and when
@@ -120,3 +122,79 @@ def test_scores_through_every_slot_of_the_ring(hkv, group):
         factor = SCALE * c.ks[ids, :, 0, 0].double().T
         assert_scores(got[0], want.amax(1) * factor, terms.amax(1) * factor)
         assert bool((got[1, :, 6:] == -math.inf).all()) and not bool((got[1, :, :6] == -math.inf).any())
+
+
+# ----------------------------------------------------------------------------- host threads
+def launches_of(monkeypatch, call):
+    """The library calls that `call` makes, as functions that make them again on a stream: () -> status."""
+    made = []
+
+    def record(index, fn, where, *args):
+        made.append((fn, args))
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "launch", record)
+        call()
+    stream = torch.cuda.Stream()
+    return [lambda fn=fn, args=args: fn(*args, stream.cuda_stream) for fn, args in made]
+
+
+def in_two_threads(a, b, rounds):
+    """Library calls a and b over and over, each from a thread of its own (a call into the library leaves the other
+    thread its turn): the statuses that are not 0."""
+    import threading
+    bad = []
+    go = threading.Barrier(2)
+
+    def run(call):
+        go.wait()
+        for _ in range(rounds):
+            status = call()
+            if status:
+                bad.append(status)
+            if bad:
+                return
+
+    threads = [threading.Thread(target=run, args=(call,)) for call in (a, b)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["scores", "attention", "attention, scales per token"])
+def test_two_threads_call_with_batches_of_different_sizes(monkeypatch, what):
+    """The index of a large batch lies in shared memory: its launch asks for more of it than a small one's."""
+    calls, outs, kept = [], [], []
+    for seqs in (4000, 3):
+        c = Cache([5] * seqs, 2, 16, seed=seqs)
+        q, bounds, lengths, tables, ks, vs, kc, vc = cuda(c.query(1), c.bounds(), c.lengths, c.tables, c.ks, c.vs, c.key, c.value)
+        if what == "scores":
+            out = torch.full((seqs, 2, 1), math.nan, device="cuda")
+            made = launches_of(monkeypatch, lambda: pa.score_blocks(q, bounds, lengths, tables, SCALE, 1, 16, key_scale=ks, scores=out))
+        elif what == "attention":
+            out = torch.full_like(q, math.nan)
+            sink = torch.zeros(2, device="cuda")
+            def call():
+                kept.append(pa.paged_attention_decode(out, q, kc, vc, lengths, tables, SCALE, 1, 5, torch.bfloat16, None, ks, vs, sink_tokens=sink))
+            made = launches_of(monkeypatch, call)
+            kept.append(sink)
+        else:
+            out = torch.full_like(q, math.nan)
+            tok = ks.expand(-1, -1, 16, -1).contiguous()
+            p, keep = build_params(out, q, kc, vc, lengths, tables, SCALE, 1, 5, None, None, tok, tok, None, 256, None, None, None, None, None)
+            stream = torch.cuda.Stream()
+            made = [lambda p=p, stream=stream: _lib.lib().pa_decode_sm100(C.byref(p), stream.cuda_stream)]
+            kept.append((keep, tok))
+        assert len(made) == 1
+        torch.cuda.synchronize()
+        assert made[0]() == 0
+        torch.cuda.synchronize()
+        calls.append(made[0])
+        outs.append((out, out.clone()))
+        kept.append((q, bounds, lengths, tables, ks, vs, kc, vc))
+    assert in_two_threads(*calls, 10000) == []
+    for out, want in outs:
+        assert not want.isnan().any() and torch.equal(out, want)

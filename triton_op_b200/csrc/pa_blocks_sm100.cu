@@ -206,7 +206,8 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
   k.off_index = (heads * nb8 * 8 * (pa::kScoreRowBytes + 4) + 15) & ~15;
   const int64_t off_ring = (k.off_index + ((int64_t)2 * p->num_seqs + 1) * 4 + 127) & ~(int64_t)127;
   const int slot = pa::score_slot_bytes(heads);
-  int64_t slots = ((int64_t)dev->max_smem_optin - 1024 - off_ring) / slot;   // (1 KB: the kernel's barriers)
+  constexpr int kDeclared = 1024;   // the kernel's barriers and scan buffer
+  int64_t slots = ((int64_t)dev->max_smem_optin - kDeclared - off_ring) / slot;
   if (slots > pa::kScoreRingBytes / slot) slots = pa::kScoreRingBytes / slot;
   if (slots > pa::kScoreMaxSlots) slots = pa::kScoreMaxSlots;
   const int warps = pa::score_warps(nb8), step = warps / heads;
@@ -221,7 +222,7 @@ int pa_block_scores_sm100(const PaBlockScoreParams* p, void* stream) {
                                          : nb8 == 2 ? pa::pa_block_score_kernel<2, 4>
                                          : nb8 == 4 ? pa::pa_block_score_kernel<4, 4>
                                                     : pa::pa_block_score_kernel<8, 4>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = pa_host::raise_dynamic_smem(kernel, *dev, kDeclared);
   if (e != cudaSuccess) return cuda_fail(e);
   return launch(kernel, dim3((unsigned)grid), (warps + producers) * 32, (size_t)smem, st, k);
 }

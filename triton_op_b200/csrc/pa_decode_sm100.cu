@@ -116,6 +116,7 @@ struct LaunchPlan {
   int rows = 0;              // query rows per work item (tcgen05 kernel)
   int grid = 0;
   int smem = 0;
+  const DeviceInfo* dev = nullptr;
 };
 
 // Validation common to every entry point that reads PaDecodeParams.
@@ -158,6 +159,7 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
   DeviceInfo* dev = nullptr;
   rc = device_info(&dev);
   if (rc != PA_OK) return rc;
+  plan->dev = dev;
 
   const int eqG = p->query_group_size * p->query_len;
   if (p->q_dtype != PA_DT_BF16 && p->q_dtype != PA_DT_E4M3FN) return PA_ERR_UNSUPPORTED;
@@ -414,9 +416,8 @@ int make_plan(const PaDecodeParams* p, LaunchPlan* plan, bool allow_fuse = false
 template <int NW, int MT, bool PT>
 int launch_partition_t(const LaunchPlan& plan, cudaStream_t stream) {
   auto kern = pa::pa_partition_fp8_p16_kernel<NW, MT, PT>;
-  // Raising the dynamic shared-memory limit is per function and per device; repeating the
-  // call is cheap and keeps the library free of per-device mutable state.
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
+  // (repeating the call is cheap and keeps the library free of per-device mutable state)
+  cudaError_t e = pa_host::raise_dynamic_smem(kern, *plan.dev);
   if (e != cudaSuccess) return cuda_fail(e);
   kern<<<plan.grid, NW * 32, plan.smem, stream>>>(plan.kp);
   e = cudaGetLastError();
@@ -428,7 +429,7 @@ template <int BS, int QR, bool PT, bool TRACE, bool ALIBI = false, bool FUSE = f
           bool BLK = false>
 int launch_tensor_t(const LaunchPlan& plan, cudaStream_t stream) {
   auto kern = pa::tc::pa_partition_fp8_tc_kernel<BS, QR, PT, TRACE, ALIBI, FUSE, PAIR, STAGE, BLK>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
+  cudaError_t e = pa_host::raise_dynamic_smem(kern, *plan.dev);
   if (e != cudaSuccess) return cuda_fail(e);
   // Programmatic dependent launch: in a decode loop the CTAs may become resident and set up their
   // barriers and tensor memory while the kernel before this one in the stream (the previous step's
@@ -530,7 +531,7 @@ int launch_partition(const LaunchPlan& plan, cudaStream_t stream) {
   }
   if (plan.bf16_kv) {
     auto kern = pa::pa_partition_bf16_p16_kernel<8>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
+    cudaError_t e = pa_host::raise_dynamic_smem(kern, *plan.dev);
     if (e != cudaSuccess) return cuda_fail(e);
     kern<<<plan.grid, 8 * 32, plan.smem, stream>>>(plan.kp);
     e = cudaGetLastError();
