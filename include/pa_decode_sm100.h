@@ -323,6 +323,8 @@ int pa_cache_write_sm100(const PaCacheWriteParams* params, void* stream);
  * and key_bounds (optional) the smallest and the largest key code of every head dim over the page's
  * tokens.  Scales of pages that hold tokens must be positive.  Pages that receive no row, and, where
  * no scale grows, slots that receive no row, are left as they are.  No page may receive rows of two sequences.
+ * What is written may not share memory: strides of zero over several pages or heads, and key and value scales
+ * that meet, are refused (PA_ERR_BAD_SHAPE).
  *   kv_quant_mode PA_QUANT_PER_BLOCK   key_scale / value_scale [NB, Hkv] are read and written
  *                 PA_QUANT_PER_TENSOR  key_scale / value_scale point to one value, read only
  * Rows without a place (a table too narrow, a page id outside the pool, more rows than tokens) are

@@ -8,7 +8,7 @@ import torch
 
 import triton_op_b200 as pa
 from oracle import blocks_oracle as bo
-from test_block_cache import D, FP8, SCALE, Cache, cuda, decode, transposed
+from test_block_cache import D, FP8, SCALE, Cache, assert_same, cuda, decode
 from triton_op_b200 import PaArgumentError, _lib
 from triton_op_b200.pa_decode import build_params
 
@@ -122,6 +122,97 @@ def test_scores_through_every_slot_of_the_ring(hkv, group):
         factor = SCALE * c.ks[ids, :, 0, 0].double().T
         assert_scores(got[0], want.amax(1) * factor, terms.amax(1) * factor)
         assert bool((got[1, :, 6:] == -math.inf).all()) and not bool((got[1, :, :6] == -math.inf).any())
+
+
+# ----------------------------------------------------------------------------- append: two writers of one place
+def append_args(device="cpu"):
+    c = Cache([40, 7], 2, 16)
+    kv = torch.randn(5, 2, D, generator=c.g).bfloat16()
+    args = dict(key=kv, value=kv, key_cache=c.key, value_cache=c.value, key_scale=c.ks, value_scale=c.vs, block_tables=c.tables,
+                sequence_lengths=c.lengths, query_start_loc=torch.tensor([0, 3, 5], dtype=torch.int32), key_bounds=c.bounds())
+    return {k: v.to(device) for k, v in args.items()}
+
+
+def shared_places(a):
+    """Changes of append_args whose pages, heads or scales share memory, and ones that only look so."""
+    nb, dev = a["key_scale"].shape[0], a["key_scale"].device
+    pool = torch.ones(2 * nb + 1, 2, 1, 1, device=dev)
+    side = torch.ones(nb, 2, 2, 1, device=dev)
+    bad = [dict(value_scale=a["key_scale"]),
+           dict(key_scale=pool[:nb], value_scale=pool[nb - 1:2 * nb - 1]),                    # one page of both
+           dict(key_scale=pool[1:nb + 1], value_scale=pool[:nb]),
+           dict(key_scale=pool.view(-1)[:2 * nb].view(nb, 2, 1, 1), value_scale=pool.view(-1)[1:2 * nb + 1].view(nb, 2, 1, 1)),
+           dict(key_bounds=a["key_bounds"][:1].expand(nb, -1, -1, -1)),
+           dict(key_bounds=a["key_bounds"][:, :1].expand(-1, 2, -1, -1)),
+           dict(key_cache=a["key_cache"][:1].expand(nb, -1, -1, -1, -1)),
+           dict(value_cache=a["value_cache"][:, :1].expand(-1, 2, -1, -1))]
+    good = [dict(key_scale=pool[:nb], value_scale=pool[nb:2 * nb]),
+            dict(key_scale=side[:, :, :1], value_scale=side[:, :, 1:]),                       # side by side, never met
+            dict(key_scale=pool[:2 * nb:2], value_scale=pool[1:2 * nb:2])]
+    return bad, good
+
+
+def test_append_refuses_places_that_are_shared():
+    a = append_args()
+    bad, good = shared_places(a)
+    for over in bad:
+        with pytest.raises(PaArgumentError, match="place of its own"):
+            pa.append_kv_cache(**{**a, **over})
+    for over in good:
+        with pytest.raises(RuntimeError, match="CUDA"):            # refused for being on the CPU only
+            pa.append_kv_cache(**{**a, **over})
+    one = torch.tensor(0.5)
+    with pytest.raises(RuntimeError, match="CUDA"):                # read only: the same value twice is fine
+        pa.append_kv_cache(**{**a, "key_scale": one, "value_scale": one})
+
+
+def test_the_library_refuses_places_that_are_shared():
+    lib = _lib.lib()
+    p = _lib.PaCacheAppendParams()
+    p.struct_size, p.abi_version = C.sizeof(p), _lib.PA_ABI_VERSION
+    room = (C.c_float * 64)()
+    at = (C.addressof(room) + 15) & ~15
+    p.num_tokens, p.num_seqs, p.num_kv_heads, p.head_size, p.block_size, p.num_blocks, p.max_blocks_per_seq = 1, 1, 2, D, 16, 4, 1
+    p.kv_quant_mode, p.v_layout = _lib.PA_QUANT_PER_BLOCK, _lib.PA_V_NORMAL
+    for name in ("key", "value", "key_cache", "value_cache", "block_tables", "context_lens", "row_start", "key_bounds"):
+        setattr(p, name, at)                                       # (nothing is read before the refusal)
+    p.key_stride_token = p.value_stride_token = 2 * D
+    p.key_stride_head = p.value_stride_head = D
+    p.k_stride_block = p.v_stride_block = 2 * 16 * D
+    p.k_stride_head = p.v_stride_head = 16 * D
+    p.bounds_stride_block, p.bounds_stride_head = 4 * D, 2 * D
+    p.kv_scale_stride_block, p.kv_scale_stride_head = 2, 1
+    for apart in (0, 1, -1, 6, 7, -7):
+        p.key_scale, p.value_scale = at + 64, at + 64 + 4 * apart
+        assert lib.pa_cache_append_sm100(C.byref(p), None) == -2, apart
+    p.key_scale, p.value_scale = at, at + 4 * 16
+    for name in ("k_stride_block", "v_stride_head", "bounds_stride_block", "bounds_stride_head", "kv_scale_stride_block"):
+        was = getattr(p, name)
+        setattr(p, name, 0)
+        assert lib.pa_cache_append_sm100(C.byref(p), None) == -2, name
+        setattr(p, name, was)
+
+
+@pytest.mark.gpu
+def test_append_refuses_shared_places_on_the_gpu_and_takes_neighbours():
+    a = append_args("cuda")
+    bad, good = shared_places(a)
+    before = {k: v.clone() for k, v in a.items()}
+    for over in bad:
+        with pytest.raises(PaArgumentError, match="place of its own"):
+            pa.append_kv_cache(**{**a, **over})
+    torch.cuda.synchronize()
+    assert all(torch.equal(a[k].view(torch.uint8), before[k].view(torch.uint8)) for k in a if a[k].dtype == FP8)
+    state = ("key_cache", "value_cache", "key_scale", "value_scale", "key_bounds")
+    for over in good:
+        mine = {k: v.clone() for k, v in a.items()}
+        views = {k: v.copy_(a[k]) for k, v in over.items()}
+        pa.append_kv_cache(**{**mine, **views})
+        ref = {k: v.cpu().clone() for k, v in a.items()}
+        bo.append(ref["key"], ref["value"], ref["key_cache"], ref["value_cache"], ref["key_scale"], ref["value_scale"],
+                  ref["block_tables"], ref["sequence_lengths"], ref["query_start_loc"], ref["key_bounds"])
+        got = {**mine, **views}
+        assert_same([got[k].cpu() for k in state], [ref[k] for k in state])
 
 
 # ----------------------------------------------------------------------------- host threads

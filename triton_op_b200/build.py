@@ -24,8 +24,8 @@ SOURCES = {
     "pa_decode_sm100.cu": _COMMON + [
         "pa_partition_fp8.cuh", "pa_partition_bf16.cuh", "pa_partition_tc.cuh", "pa_tcgen05.cuh", "pa_reduce.cuh",
         "pa_cache_write.cuh", "pa_exchange.cuh", "pa_stream_probe.cuh"],
-    CALLS_SOURCE: [os.path.join("..", "..", "include", "pa_decode_sm100.h")],
-    "pa_blocks_sm100.cu": _COMMON + ["pa_block_score.cuh", "pa_block_select.cuh", "pa_cache_append.cuh", "pa_tcgen05.cuh"],
+    CALLS_SOURCE: ["pa_places.h", os.path.join("..", "..", "include", "pa_decode_sm100.h")],
+    "pa_blocks_sm100.cu": _COMMON + ["pa_places.h", "pa_block_score.cuh", "pa_block_select.cuh", "pa_cache_append.cuh", "pa_tcgen05.cuh"],
 }
 
 NVCC_FLAGS = [

@@ -119,6 +119,21 @@ def _rows(t: torch.Tensor):
     return t, stride
 
 
+def _distinct(stride, shape) -> bool:
+    """Every page and kv head has a place of its own (no stride of zero)."""
+    return not ((shape[0] > 1 and stride[0] == 0) or (shape[1] > 1 and stride[1] == 0))
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """An entry [page, kv head] of one is an entry of the other (both with the same strides)."""
+    (n0, n1), (s0, s1) = a.shape[:2], a.stride()[:2]
+    apart, left = divmod(b.data_ptr() - a.data_ptr(), 4)
+    if left or abs(apart) > (n0 - 1) * s0 + (n1 - 1) * s1:
+        return False
+    rests = (apart - j * s1 for j in range(1 - n1, n1))
+    return any(r == 0 if s0 == 0 else r % s0 == 0 and abs(r // s0) < n0 for r in rests)
+
+
 def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                     key_scale: torch.Tensor, value_scale: torch.Tensor, block_tables: torch.Tensor,
                     sequence_lengths: torch.Tensor, query_start_loc: torch.Tensor, *,
@@ -136,7 +151,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     ``key_bounds``: e4m3fn ``[num_blocks, num_kv_heads, 2, head_size]``, the smallest and largest key
     code of every head dim over the page's tokens, kept up to date for
     :func:`triton_op_b200.score_blocks`.  ``status`` (int32 scalar) receives ``PA_DEV_*`` bits for rows
-    that have no place; they are skipped.  No page may get rows of two sequences in a call.  Runs on
+    that have no place; they are skipped.  No page may get rows of two sequences in a call; what is
+    written (scales, codes and bounds of each page and kv head) may not share memory.  Runs on
     the current stream; there is no CPU fallback.
     """
     done = _lib.calls().append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables, sequence_lengths,
@@ -166,6 +182,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     if not ((kc_stride[4] == 1 and kc_stride[3] == 16 and kc_stride[2] == 16 * bs) or _inner_contiguous(key_cache, 2)) or not (
             (not trans and vc_stride[3] == 1 and vc_stride[2] == bs) or _inner_contiguous(value_cache, 2)):
         raise PaArgumentError("the per-(block, head) slabs of the KV caches must be contiguous")
+    if not (_distinct(kc_stride, c_shape) and _distinct(vc_stride, c_shape)):
+        raise PaArgumentError("the caches are written: every page and kv head needs a place of its own")
     if not (isinstance(key_scale, torch.Tensor) and isinstance(value_scale, torch.Tensor)
             and key_scale.dtype == torch.float32 and value_scale.dtype == torch.float32):
         raise PaArgumentError("key_scale and value_scale must be float32 tensors")
@@ -173,8 +191,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
         mode, s_block, s_head = _lib.PA_QUANT_PER_TENSOR, 0, 0
     else:
         s_block, s_head = _check_block_scales(key_scale, value_scale, key_cache)
-        if (num_blocks > 1 and s_block == 0) or (num_kv_heads > 1 and s_head == 0):
-            raise PaArgumentError("block kv scales are written: every page and kv head needs a place of its own")
+        if not _distinct((s_block, s_head), c_shape) or _meet(key_scale, value_scale):
+            raise PaArgumentError("block kv scales are written: every page and kv head needs a place of its own, for its keys and for its values")
         mode = _lib.PA_QUANT_PER_BLOCK
     b_block = b_head = b_ptr = st_ptr = 0
     if key_bounds is not None:
@@ -182,6 +200,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
         if not (key_bounds.dtype == FP8_DTYPE and key_bounds.shape == (num_blocks, num_kv_heads, 2, head_size)
                 and b_stride[3] == 1 and b_stride[2] == head_size and key_bounds.get_device() == on):
             raise PaArgumentError(f"key_bounds must be {FP8_DTYPE} {(num_blocks, num_kv_heads, 2, head_size)} on {dev}, its last two dims contiguous")
+        if not _distinct(b_stride, c_shape):
+            raise PaArgumentError("key_bounds are written: every page and kv head needs a place of its own")
         b_block, b_head, b_ptr = b_stride[0], b_stride[1], key_bounds.data_ptr()
     t_shape = block_tables.shape
     num_seqs = t_shape[0]

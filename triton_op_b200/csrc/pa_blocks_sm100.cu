@@ -7,6 +7,7 @@
 
 #include "../../include/pa_decode_sm100.h"
 #include "pa_host.h"
+#include "pa_places.h"
 #include "pa_block_score.cuh"
 #include "pa_block_select.cuh"
 #include "pa_cache_append.cuh"
@@ -66,6 +67,15 @@ int pa_cache_append_sm100(const PaCacheAppendParams* p, void* stream) {
       (p->k_stride_block & 15) || (p->k_stride_head & 15) || (p->v_stride_block & 15) || (p->v_stride_head & 15) ||
       (p->bounds_stride_block & 15) || (p->bounds_stride_head & 15))
     return PA_ERR_ALIGNMENT;
+  // what is written by units that know nothing of each other: every page and kv head needs a place of its own
+  if (!pa_places::distinct(p->num_blocks, p->num_kv_heads, p->k_stride_block, p->k_stride_head) ||
+      !pa_places::distinct(p->num_blocks, p->num_kv_heads, p->v_stride_block, p->v_stride_head) ||
+      (p->key_bounds && !pa_places::distinct(p->num_blocks, p->num_kv_heads, p->bounds_stride_block, p->bounds_stride_head)))
+    return PA_ERR_BAD_SHAPE;
+  if (p->kv_quant_mode == PA_QUANT_PER_BLOCK &&
+      (!pa_places::distinct(p->num_blocks, p->num_kv_heads, p->kv_scale_stride_block, p->kv_scale_stride_head) ||
+       pa_places::meet(p->value_scale - p->key_scale, p->num_blocks, p->num_kv_heads, p->kv_scale_stride_block, p->kv_scale_stride_head)))
+    return PA_ERR_BAD_SHAPE;
   DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc != PA_OK) return rc;

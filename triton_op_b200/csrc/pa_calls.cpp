@@ -20,6 +20,7 @@
 #include <cstring>
 
 #include "../../include/pa_decode_sm100.h"
+#include "pa_places.h"
 
 namespace {
 
@@ -236,14 +237,18 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (x->stride(2) != 1 || (x->stride(0) & 7) || (x->stride(1) & 7) || !aligned16(*x)) return nullptr;
     const int mode = scale_mode(*ks, *vs, nb, h);
     if (mode < 0) return nullptr;
-    if (mode == PA_QUANT_PER_BLOCK && ((nb > 1 && ks->stride(0) == 0) || (h > 1 && ks->stride(1) == 0))) return nullptr;
+    auto distinct = [&](const at::Tensor& x) { return pa_places::distinct(nb, h, x.stride(0), x.stride(1)); };
+    if (!distinct(*k) || !distinct(*v)) return nullptr;
+    if (mode == PA_QUANT_PER_BLOCK &&
+        (!distinct(*ks) || pa_places::meet(vs->data_ptr<float>() - ks->data_ptr<float>(), nb, h, ks->stride(0), ks->stride(1))))
+      return nullptr;
     if (!is(*bt, at::kInt, 2) || bt->size(1) < 1 || bt->stride(1) != 1) return nullptr;
     const int64_t s = bt->size(0);
     if (!is(*len, at::kInt, 1) || len->size(0) != s || !is(*start, at::kInt, 1) || start->size(0) != s + 1 ||
         (s > 1 && len->stride(0) != 1) || start->stride(0) != 1)
       return nullptr;
     if (bounds && (bounds->scalar_type() != at::kFloat8_e4m3fn || !sized(*bounds, {nb, h, 2, kD}) || bounds->stride(3) != 1 ||
-                   bounds->stride(2) != kD))
+                   bounds->stride(2) != kD || !distinct(*bounds)))
       return nullptr;
     const int device = common_device({key, val, k, v, ks, vs, bt, len, start, bounds ? bounds : key});
     int32_t* status;
