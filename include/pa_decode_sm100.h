@@ -400,6 +400,8 @@ int pa_block_scores_sm100(const PaBlockScoreParams* params, void* stream);
  * as -inf, ties to the lower place), top_k in all, as a block table in the order of the context.
  * A sequence of at most top_k pages keeps them all.  Unused entries become 0.
  *   lengths[s] = tokens in the pages of one such table (the same for every kv head)
+ * tables and lengths may not share memory with what is read (tables or lengths that begin where the ones that
+ * are read do: PA_ERR_BAD_SHAPE).
  */
 typedef struct PaBlockSelectParams {
   uint32_t struct_size, abi_version;

@@ -215,6 +215,23 @@ def test_append_refuses_shared_places_on_the_gpu_and_takes_neighbours():
         assert_same([got[k].cpu() for k in state], [ref[k] for k in state])
 
 
+# ----------------------------------------------------------------------------- outputs that are read, or shared
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_outputs_need_places_of_their_own(device):
+    c = Cache([40, 7], 2, 16)
+    lengths, tables = c.lengths.to(device), c.tables.to(device)
+    score = torch.zeros(2, 2, 3, device=device)
+    one = torch.zeros(2, 1, 3, dtype=torch.int32, device=device)
+    for over in (dict(lengths=lengths), dict(tables=one.expand(-1, 2, -1)[:, :, :2]), dict(tables=one[:1].expand(2, 2, -1)[:, :, :2])):
+        with pytest.raises(PaArgumentError):
+            pa.select_blocks(score, lengths, tables, 16, 2, **over)
+    with pytest.raises(PaArgumentError):                               # one kv head: its tables could be the sequences'
+        pa.select_blocks(score[:, :1], lengths, tables, 16, 3, tables=tables[:, None])
+    for out in (score[:, :1].expand(-1, 2, -1), score[:1].expand(2, -1, -1)):
+        with pytest.raises(PaArgumentError):
+            pa.score_blocks(c.query(3).to(device), c.bounds().to(device), lengths, tables, SCALE, 1, 16, scores=out)
+
+
 # ----------------------------------------------------------------------------- host threads
 def launches_of(monkeypatch, call):
     """The library calls that `call` makes, as functions that make them again on a stream: () -> status."""

@@ -245,6 +245,8 @@ int pa_block_select_sm100(const PaBlockSelectParams* p, void* stream) {
     return PA_ERR_BAD_SHAPE;
   if (p->num_seqs == 0) return PA_OK;
   if (!p->scores || !p->block_tables || !p->context_lens || !p->tables || !p->lengths) return PA_ERR_NULL_POINTER;
+  // outputs that other CTAs still read
+  if (p->lengths == p->context_lens || p->tables == p->block_tables) return PA_ERR_BAD_SHAPE;
   const int64_t grid = (int64_t)p->num_seqs * p->num_kv_heads;
   if (grid > 0x7fffffff || (int64_t)p->max_blocks_per_seq > 0x7fffffff - pa::kSelectLarge) return PA_ERR_TOO_LARGE;
   pa::BlockSelectParams k;

@@ -56,6 +56,12 @@ def _tables_and_lengths(sequence_lengths, block_tables, on: int):
     return sequence_lengths, block_tables, shape[0], shape[1], stride[0]
 
 
+def _own_rows(t: torch.Tensor, name: str) -> None:
+    """Refuses an output [num_seqs, num_kv_heads, ..] whose rows share memory by a stride of zero."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape[:2], t.stride()[:2])):
+        _fail(f"{name} is written: every sequence and kv head needs a row of its own")
+
+
 def _status_ptr(status, dev) -> int:
     if status is None:
         return 0
@@ -151,6 +157,8 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
     elif not (scores.dtype == torch.float32 and scores.device == dev and scores.shape == (num_seqs, num_kv_heads, width)
               and scores.stride(2) == 1):
         _fail(f"scores must be fp32 {(num_seqs, num_kv_heads, width)} on {dev}, its last dim contiguous")
+    else:
+        _own_rows(scores, "scores")
     s_stride = scores.stride()
     status_ptr = _status_ptr(status, dev)
     if on < 0:
@@ -177,7 +185,8 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     such table -- what ``paged_attention_decode`` takes as ``block_tables`` and ``sequence_lengths``.
     The first ``keep_first`` and the last ``keep_last`` pages are always among them; the others go by
     ``scores`` (fp32 ``[num_seqs, num_kv_heads, max_blocks]``), NaN as -inf, ties to the lower place.
-    With several query tokens ``keep_last`` has to cover the last ``query_len`` tokens: 2.
+    With several query tokens ``keep_last`` has to cover the last ``query_len`` tokens: 2.  ``tables`` and
+    ``lengths``: output tensors to use, not the ones that are read.
     """
     if tables is None and lengths is None:
         done = _lib.calls().select(scores, sequence_lengths, block_tables, block_size, top_k, keep_first, keep_last, status)
@@ -206,10 +215,16 @@ def select_blocks(scores: torch.Tensor, sequence_lengths: torch.Tensor, block_ta
     elif not (tables.dtype == torch.int32 and tables.device == dev and tables.shape == (num_seqs, num_kv_heads, top_k)
               and tables.stride(2) == 1):
         _fail(f"tables must be int32 {(num_seqs, num_kv_heads, top_k)} on {dev}, its last dim contiguous")
+    else:
+        _own_rows(tables, "tables")
+        if tables.numel() > 0 and tables.data_ptr() == block_tables.data_ptr():
+            _fail("tables must not be block_tables, which are read")
     if lengths is None:
         lengths = torch.empty_strided((num_seqs,), (1,), dtype=torch.int32, device=dev)
     elif not (lengths.dtype == torch.int32 and lengths.device == dev and lengths.shape == (num_seqs,) and lengths.is_contiguous()):
         _fail(f"lengths must be a contiguous int32 tensor of {num_seqs} on {dev}")
+    elif num_seqs > 0 and abs(lengths.data_ptr() - sequence_lengths.data_ptr()) < 4 * num_seqs:
+        _fail("lengths must not be sequence_lengths, which every kv head reads")
     t_stride = tables.stride()
     status_ptr = _status_ptr(status, dev)
     if on < 0:
