@@ -367,7 +367,9 @@ int pa_cache_append_sm100(const PaCacheAppendParams* params, void* stream);
  *   scores[s, h, i] = key_scale[page, h] * max_r softmax_scale * qs_r * sum_d max(q_rd lo_d, q_rd hi_d)
  * over the query rows r of kv head h, where (lo, hi) = key_bounds[page, h]: no logit of the group
  * with a key of the page is larger.  Entries past the last such page become -inf; a query row that
- * holds a NaN makes the scores of its kv head NaN.
+ * holds a NaN makes the scores of its kv head NaN.  The sum is taken as q+ . hi + q- . lo (the positive and the
+ * negative part of the row): an infinite element makes it infinite, or NaN where it meets a bound of zero or an
+ * infinity of the other sign.
  */
 typedef struct PaBlockScoreParams {
   uint32_t struct_size, abi_version;

@@ -124,6 +124,40 @@ def test_scores_through_every_slot_of_the_ring(hkv, group):
         assert bool((got[1, :, 6:] == -math.inf).all()) and not bool((got[1, :, :6] == -math.inf).any())
 
 
+def split_scores(q, c, bounds, group):
+    """q+ . hi + q- . lo in 64 bits, and the finite terms' absolute sum: [Hkv, group, pages] of sequence 0 each, unscaled by head."""
+    ids = c.tables[0, :-(-int(c.lengths[0]) // c.bs)].long()
+    lo, hi = bo.codes(bounds[ids]).permute(2, 1, 0, 3)
+    rows = q[0].double().view(c.hkv, group, D)
+    up, down = rows.clamp_min(0), rows.clamp_max(0)
+    terms = (up.nan_to_num(posinf=0) @ hi.abs().transpose(1, 2)) + (-down.nan_to_num(neginf=0)) @ lo.abs().transpose(1, 2)
+    return up @ hi.transpose(1, 2) + down @ lo.transpose(1, 2), terms, c.ks[ids, :, 0, 0].double().T
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [1, 3, 12, 20, 50])
+def test_scores_of_infinite_query_elements(group):
+    c = Cache([400], 2, 16, seed=group)
+    bounds = c.bounds()
+    bounds.view(torch.uint8)[c.tables[0, 2].long(), :, 1, 9] = 0           # one page's largest code of dim 9 is zero
+    q = c.query(group)
+    q[0, 0, 9] = math.inf                       # head 0: one infinity beside elements far below and above f16's largest
+    q[0, 0, 10], q[0, 0, 11] = 2.0 ** 70, 2.0 ** 55
+    q[0, group, 5], q[0, group, 6] = -math.inf, 2.0 ** 100                  # head 1
+    got = scores_of(q, bounds, c.lengths, c.tables, 16, c.ks)[0]
+    sums, terms, ks = split_scores(q, c, bounds, group)
+    nan = sums.isnan().any(1)
+    want = sums.nan_to_num(nan=0.0, posinf=math.inf, neginf=-math.inf).amax(1) * SCALE * ks
+    assert bool(nan.any()) and bool((want == math.inf).any())
+    assert torch.equal(got.isnan(), nan)
+    fine = ~nan
+    assert torch.equal(got.isinf() & fine, want.isinf() & fine)
+    assert torch.equal(got[want.isinf() & fine].double(), want[want.isinf() & fine])
+    fine &= ~want.isinf()
+    slack = 260 * 2.0 ** -23 * terms.amax(1) * SCALE * ks
+    assert bool(((got.double() - want).abs()[fine] <= slack[fine]).all())
+
+
 # ----------------------------------------------------------------------------- append: two writers of one place
 def append_args(device="cpu"):
     c = Cache([40, 7], 2, 16)

@@ -384,6 +384,13 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) amax = max_or_nan(amax, fabsf(x[e]));
       amax = quad_max_or_nan(amax);
+      if (__any_sync(kFullMask, amax == INFINITY)) {   // (rare) the finite elements beside an infinite one keep their digits
+        float finite = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) finite = fmaxf(finite, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+        finite = quad_max_or_nan(finite);
+        if (amax == INFINITY) amax = finite;
+      }
       // power of two that brings the row's largest element into [2^14, 2^15)
       const int be = (int)((__float_as_uint(amax) >> 23) & 0xff);
       float pre = 1.0f, back = 1.0f;
