@@ -140,6 +140,9 @@ def test_scores_of_infinite_query_elements(group):
     c = Cache([400], 2, 16, seed=group)
     bounds = c.bounds()
     bounds.view(torch.uint8)[c.tables[0, 2].long(), :, 1, 9] = 0           # one page's largest code of dim 9 is zero
+    for dim in (6, 10, 11):                     # pages on which large finite elements give zero, or less
+        bounds.view(torch.uint8)[c.tables[0, 4].long(), :, :, dim] = 0
+        bounds[c.tables[0, 3].long(), :, :, dim] = torch.tensor([-20.0, -5.0]).to(FP8)
     q = c.query(group)
     q[0, 0, 9] = math.inf                       # head 0: one infinity beside elements far below and above f16's largest
     q[0, 0, 10], q[0, 0, 11] = 2.0 ** 70, 2.0 ** 55
@@ -156,6 +159,22 @@ def test_scores_of_infinite_query_elements(group):
     fine &= ~want.isinf()
     slack = 260 * 2.0 ** -23 * terms.amax(1) * SCALE * ks
     assert bool(((got.double() - want).abs()[fine] <= slack[fine]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [2, 12])
+def test_scores_of_subnormal_query_rows(group):
+    """Rows whose largest element is below bf16's smallest normal number (2^-126) beside rows that are not."""
+    c = Cache([400], 2, 16, seed=group)
+    bounds = c.bounds()
+    q = c.query(group)
+    steps = torch.randint(-127, 128, (2, D), generator=c.g).float()
+    q[0, 0], q[0, group] = (steps * 2.0 ** -133).bfloat16()
+    q[0, 1:group] = 0                                   # head 0 has nothing larger
+    got = scores_of(q, bounds, c.lengths, c.tables, 16, c.ks)[0]
+    sums, terms, ks = split_scores(q, c, bounds, group)
+    # (no product, sum or factor of head 0 is subnormal in 32 bits: terms of 2^-133 * SCALE * 2^-8 at least are summed scaled up)
+    assert bool(((got.double() - sums.amax(1) * SCALE * ks).abs() <= 260 * 2.0 ** -23 * terms.amax(1) * SCALE * ks).all())
 
 
 # ----------------------------------------------------------------------------- append: two writers of one place

@@ -394,7 +394,7 @@ pa_block_score_kernel(const __grid_constant__ BlockScoreParams p) {
       // power of two that brings the row's largest element into [2^14, 2^15)
       const int be = (int)((__float_as_uint(amax) >> 23) & 0xff);
       float pre = 1.0f, back = 1.0f;
-      if (be > 0 && be < 255) {
+      if (be < 255) {        // (zeros and subnormal rows: the largest power there is room for)
         pre = __uint_as_float((uint32_t)min(253, 254 + 14 - be) << 23);
         back = 1.0f / pre;   // a power of two
       } else if (amax != amax) {
