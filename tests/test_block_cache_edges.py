@@ -94,6 +94,32 @@ def test_workspaces_of_the_caller(dtype):
         decode(c, q, **{**kw, "tmp_output": torch.empty(*shape, D, dtype=torch.float16, device="cuda")})
 
 
+@pytest.mark.parametrize("given", [(), ("exp_sums", "max_logits"), ("tmp_output",)])
+def test_block_scales_never_share_workspaces(given):
+    """Two calls of one shape, as two streams or two captured graphs make them, whatever their options."""
+    c = Cache([600, 40], 2, 16)
+    q = c.query(3)
+    shape = (2, 2, 3, 3)
+    mine = dict(exp_sums=torch.empty(shape), max_logits=torch.empty(shape), tmp_output=torch.empty(*shape, D))
+    blocks = [build_params(torch.empty_like(q), q, c.key, c.value, c.lengths, c.tables, SCALE, 1, 600, None, None, c.ks, c.vs, None, 256,
+                           *(mine[n] if n in given else None for n in mine), None, dict(fuse=1)) for _ in range(2)]
+    for name, field in (("exp_sums", "exp_sums"), ("max_logits", "max_logits"), ("tmp_output", "tmp_out")):
+        a, b = (getattr(p, field) for p, _ in blocks)
+        assert (a == b == mine[name].data_ptr()) if name in given else (a != b), name
+
+
+@pytest.mark.gpu
+def test_timed_calls_keep_their_workspaces():
+    c = Cache([600, 40], 2, 16, seed=8)
+    q = cuda(c.query(3))
+    res = [pa.paged_attention_decode(torch.empty_like(q), q * k, *cuda(c.key, c.value, c.lengths, c.tables), SCALE, 1, 600, torch.bfloat16, None,
+                                     *cuda(c.ks, c.vs), time_kernels=True) for k in (1, 3)]
+    assert not torch.equal(res[0]["maximum_logits"], res[1]["maximum_logits"])
+    plain = pa.paged_attention_decode(torch.empty_like(q), q, *cuda(c.key, c.value, c.lengths, c.tables), SCALE, 1, 600, torch.bfloat16, None, *cuda(c.ks, c.vs))
+    assert torch.equal(plain["final_output"], res[0]["final_output"])
+    assert torch.equal(plain["maximum_logits"][0], res[0]["maximum_logits"][0])
+
+
 # ----------------------------------------------------------------------------- scores
 def scores_of(q, bounds, lengths, tables, bs, ks, query_len=1, **kw):
     return pa.score_blocks(*cuda(q, bounds, lengths, tables), SCALE, query_len, bs, key_scale=cuda(ks), **kw).cpu()

@@ -347,7 +347,12 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     # (with block scales the partial outputs keep 32 bits unless the caller's workspace holds fewer)
     tmp_dtypes = (torch.float32, output.dtype) if kv_mode == _lib.PA_QUANT_PER_BLOCK else (output.dtype,)
     if exp_sums is None or max_logits is None or tmp_output is None:
-        ws = get_workspaces(num_seqs, num_kv_heads, max_partitions, eq_group, head_size, tmp_dtypes[0], dev)
+        if kv_mode == _lib.PA_QUANT_PER_BLOCK:      # the call's own, whatever its options: nothing is kept for the next one
+            shape = (num_seqs, num_kv_heads, max_partitions, eq_group)
+            ws = (torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev),
+                  torch.empty(*shape, head_size, dtype=tmp_dtypes[0], device=dev))
+        else:
+            ws = get_workspaces(num_seqs, num_kv_heads, max_partitions, eq_group, head_size, tmp_dtypes[0], dev)
         exp_sums = ws[0] if exp_sums is None else exp_sums
         max_logits = ws[1] if max_logits is None else max_logits
         tmp_output = ws[2] if tmp_output is None else tmp_output
@@ -382,7 +387,7 @@ def _build_params(output, query, key_cache, value_cache, sequence_lengths, block
     p.exp_sums, p.max_logits, p.tmp_out = exp_sums.data_ptr(), max_logits.data_ptr(), tmp_output.data_ptr()
     p.status = status.data_ptr() if status is not None else None
     counters = None
-    if tune and tune.get("fuse", 0) > 0 and num_seqs > 0:
+    if tune and tune.get("fuse", 0) > 0 and num_seqs > 0 and kv_mode != _lib.PA_QUANT_PER_BLOCK:
         counters = get_merge_counters(tmp_output, num_seqs, num_kv_heads)
         p.merge_counters = counters.data_ptr()
     p.trace = tune["trace"].data_ptr() if tune and tune.get("trace") is not None else None
