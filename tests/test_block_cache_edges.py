@@ -8,9 +8,10 @@ import torch
 
 import triton_op_b200 as pa
 from oracle import blocks_oracle as bo
-from test_block_cache import D, FP8, SCALE, Cache, assert_same, cuda, decode
+from test_block_cache import D, FP8, SCALE, Cache, assert_attention, assert_same, cuda, decode, serve
 from triton_op_b200 import PaArgumentError, _lib
 from triton_op_b200.pa_decode import build_params
+from triton_op_b200.sharding import KvShardedDecoder, decode_kv_shard, local_block_table, merge_triples_cuda, plan_kv_shards
 
 
 # ----------------------------------------------------------------------------- attention: what is rounded, and when
@@ -309,6 +310,159 @@ def test_outputs_need_places_of_their_own(device):
     for out in (score[:, :1].expand(-1, 2, -1), score[:1].expand(2, -1, -1)):
         with pytest.raises(PaArgumentError):
             pa.score_blocks(c.query(3).to(device), c.bounds().to(device), lengths, tables, SCALE, 1, 16, scores=out)
+
+
+# ----------------------------------------------------------------------------- refusals, whichever way a call takes
+def calls_and_mistakes(device):
+    """(function, an ordinary call, changes that make it a mistake) of each operator."""
+    c = Cache([40, 7], 2, 16)
+    t = {k: v.to(device) for k, v in dict(kc=c.key, vc=c.value, ks=c.ks, vs=c.vs, bt=c.tables, len=c.lengths, b=c.bounds(), q=c.query(3),
+                                          wide=c.query(65)).items()}
+    nb, ones = c.nb, lambda *shape, **kw: torch.ones(*shape, device=device, **kw)
+    kv = torch.zeros(5, 2, D, dtype=torch.bfloat16, device=device)
+    start = torch.tensor([0, 3, 5], dtype=torch.int32, device=device)
+    heads = t["bt"][:, None].expand(-1, 2, -1).contiguous()
+    half_pages = t["kc"].view(torch.uint8)[:, :, :, ::2].view(FP8)
+    yield pa.append_kv_cache, dict(
+        key=kv, value=kv, key_cache=t["kc"], value_cache=t["vc"], key_scale=t["ks"], value_scale=t["vs"], block_tables=t["bt"],
+        sequence_lengths=t["len"], query_start_loc=start), [
+        dict(key=kv.float()), dict(value=kv[:4]), dict(key=kv[0]), dict(key_cache=t["kc"].float().bfloat16()), dict(key_cache=t["kc"][:, :1]),
+        dict(value_cache=t["vc"][:, :, :, :8]), dict(key_scale=ones(())), dict(key_scale=1.0), dict(value_scale=t["vs"].double()),
+        dict(key_bounds=t["b"].float()), dict(key_bounds=t["b"][..., :64]), dict(key_bounds=t["b"][:1]), dict(block_tables=t["bt"].long()),
+        dict(block_tables=t["bt"][:, :0]), dict(sequence_lengths=t["len"][:1]), dict(query_start_loc=start[:2]), dict(query_start_loc=start.long()),
+        dict(status=ones(())), dict(key_cache=half_pages), dict(key_scale=ones(nb + 1, 2, 1, 1), value_scale=ones(nb + 1, 2, 1, 1))]
+    yield pa.paged_attention_decode, dict(
+        output=torch.empty_like(t["q"]), query=t["q"], key_cache=t["kc"], value_cache=t["vc"], sequence_lengths=t["len"], block_tables=t["bt"],
+        softmax_scale=SCALE, query_sequence_length=1, max_sequence_length=40, compute_type=torch.bfloat16, query_scale=None,
+        key_scale=t["ks"], value_scale=t["vs"]), [
+        dict(value_scale=ones(())), dict(value_scale=None), dict(key_scale=ones(nb, 1, 1, 1), value_scale=ones(nb, 1, 1, 1)),
+        dict(key_scale=ones(nb + 1, 2, 1, 1), value_scale=ones(nb + 1, 2, 1, 1)), dict(key_scale=t["ks"].double(), value_scale=t["vs"].double()),
+        dict(key_scale=ones(2, nb, 1, 1).transpose(0, 1)), dict(block_tables=heads[:, :1]), dict(block_tables=heads.long()), dict(block_tables=heads[:1]),
+        dict(block_tables=heads, key_scale=ones(nb, 2, 16, 1), value_scale=ones(nb, 2, 16, 1)), dict(query_sequence_length=5),
+        dict(query_sequence_length=2), dict(query_sequence_length=0), dict(output=torch.empty(2, 6, D, device=device)),
+        dict(output=torch.empty_like(t["q"])[:1]), dict(query=t["q"].half()), dict(key_cache=t["kc"].float().bfloat16()), dict(key_cache=half_pages),
+        dict(value_cache=t["vc"][:, :, :64]), dict(sequence_lengths=t["len"].long()), dict(sequence_lengths=t["len"][:1]),
+        dict(status=torch.zeros((), dtype=torch.int64, device=device)), dict(query=t["wide"], output=torch.empty_like(t["wide"]))]
+    yield pa.score_blocks, dict(
+        query=t["q"], key_bounds=t["b"], sequence_lengths=t["len"], block_tables=t["bt"], softmax_scale=SCALE, query_sequence_length=1,
+        block_size=16, key_scale=t["ks"]), [
+        dict(query=t["q"].half()), dict(query=t["q"][0]), dict(query=t["q"][..., :64]), dict(query=t["wide"]), dict(key_bounds=t["b"].float()),
+        dict(key_bounds=t["b"][..., :64]), dict(key_bounds=t["b"][:, :, :1]), dict(softmax_scale=0.0), dict(softmax_scale=-1.0),
+        dict(softmax_scale=math.nan), dict(query_sequence_length=2), dict(query_sequence_length=0), dict(query_sequence_length=5), dict(block_size=32),
+        dict(key_scale=ones(nb, 2, 16, 1)), dict(key_scale=ones(nb, 1, 1, 1)), dict(key_scale=ones(nb + 1, 2, 1, 1)), dict(block_tables=t["bt"][:1]),
+        dict(block_tables=t["bt"].long()), dict(sequence_lengths=t["len"].long()), dict(sequence_lengths=t["len"][:1]), dict(status=ones(()))]
+    score = torch.zeros(2, 2, 3, device=device)
+    yield pa.select_blocks, dict(scores=score, sequence_lengths=t["len"], block_tables=t["bt"], block_size=16, top_k=2), [
+        dict(scores=score[:, :, :2]), dict(scores=score.double()), dict(scores=score[0]), dict(scores=score[:1]), dict(top_k=1), dict(top_k=0),
+        dict(keep_first=-1), dict(keep_last=0), dict(keep_first=2), dict(block_size=48), dict(block_tables=t["bt"].long()),
+        dict(sequence_lengths=t["len"].long()), dict(sequence_lengths=t["len"][:1]), dict(status=ones(()))]
+
+
+@pytest.mark.gpu
+def test_mistakes_on_the_gpu_are_refused(monkeypatch):
+    """The host calls check for themselves what the Python functions check: nothing that those refuse is taken."""
+    taken = []
+
+    class Watched:
+        def __getattr__(self, name):
+            def call(*args):
+                done = getattr(real, name)(*args)
+                taken.append(done is not None)
+                return done
+            return call
+    real = _lib.calls()
+    monkeypatch.setattr(_lib, "_CALLS", Watched())
+    for fn, good, mistakes in calls_and_mistakes("cuda"):
+        taken.clear()
+        fn(**good)
+        assert taken == [True], fn                                     # the ordinary call goes that way
+        names = [k for k, v in good.items() if isinstance(v, torch.Tensor)]
+        for over in mistakes + [{k: good[k].cpu()} for k in names]:
+            taken.clear()
+            with pytest.raises(PaArgumentError):
+                fn(**{**good, **over})
+            assert not any(taken), (fn, over.keys())
+    torch.cuda.synchronize()
+
+
+# ----------------------------------------------------------------------------- the operators in a row
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,query_len,group", [(16, 1, 4), (16, 2, 8), (64, 1, 1), (64, 3, 2)])
+def test_served_selections_are_those_of_the_scores(bs, query_len, group):
+    """The tables of a served step are the exact selection of the kernel's scores, and that of the oracle's wherever
+    the last page taken and the first one left are further apart than the scores may be off."""
+    sure = 0
+    for c, q, out, res, (kc, vc, ks, vs, bounds, lengths) in serve(4, bs, 6, group, query_len):
+        keep = 1 if query_len == 1 else 2
+        score = scores_of(q, bounds, lengths, c.tables, bs, ks, query_len)
+        want, terms = bo.scores(q, bounds, lengths, c.tables, SCALE, bs, ks)
+        assert_scores(score, want, terms)
+        got = res["block_tables"].cpu()
+        tables, tokens = bo.select(score, lengths, c.tables, bs, 6, 1, keep)
+        assert torch.equal(got, tables) and torch.equal(res["sequence_lengths"].cpu(), tokens)
+        tables, _ = bo.select(want, lengths, c.tables, bs, 6, 1, keep)
+        for s in range(3):
+            pages = -(-int(lengths[s]) // bs)
+            for h in range(c.hkv):
+                if pages > 6:
+                    rest, order = want[s, h, 1:pages - keep].sort(descending=True)
+                    slack = 2 * 260 * 2.0 ** -23 * float(terms[s, h, :pages].max())
+                    if float(rest[6 - 1 - keep - 1] - rest[6 - 1 - keep]) <= slack:
+                        continue
+                sure += 1
+                assert torch.equal(got[s, h], tables[s, h])
+    assert sure >= 12                                                  # of 24 selections: the comparison is not an empty one
+
+
+@pytest.mark.gpu
+def test_bounds_beyond_32_bits():
+    """Key bounds more than 4 GB into their tensor: appended, scored and selected by."""
+    hkv, bs, n = 8, 16, 200
+    nb = (1 << 32) // (hkv * 16 * D) + 40
+    kc = torch.empty(nb, hkv, 8, bs, 16, dtype=torch.uint8, device="cuda").view(FP8)
+    vc = torch.empty(nb, hkv, D, bs, dtype=torch.uint8, device="cuda").view(FP8)
+    ks, vs = torch.ones(nb, hkv, 1, 1, device="cuda"), torch.ones(nb, hkv, 1, 1, device="cuda")
+    bounds = torch.empty(nb, hkv, 16, D, dtype=torch.uint8, device="cuda").view(FP8)[:, :, :2]
+    assert bounds.stride(0) * (nb - 13) > 1 << 32
+    g = torch.Generator().manual_seed(1)
+    tables = torch.arange(nb - 13, nb).int()[None]
+    near = torch.arange(13).int()[None]
+    key, value = torch.randn(n, hkv, D, generator=g).bfloat16(), torch.randn(n, hkv, D, generator=g).bfloat16()
+    lengths, start = torch.tensor([n], dtype=torch.int32), torch.tensor([0, n], dtype=torch.int32)
+    pa.append_kv_cache(*cuda(key, value), kc, vc, ks, vs, *cuda(tables, lengths, start), key_bounds=bounds)
+    far = slice(nb - 13, nb)
+    ref = [torch.zeros(13, hkv, 8, bs, 16).to(FP8), torch.zeros(13, hkv, D, bs).to(FP8), torch.ones(13, hkv, 1, 1), torch.ones(13, hkv, 1, 1),
+           torch.zeros(13, hkv, 2, D).to(FP8)]
+    bo.append(key, value, *ref[:4], near, lengths, start, ref[4])
+    assert_same([ks[far].cpu(), vs[far].cpu(), bounds[far].cpu()], ref[2:])
+    q = torch.randn(1, hkv * 4, D, generator=g).bfloat16()
+    score = pa.score_blocks(q.cuda(), bounds, *cuda(lengths, tables), SCALE, 1, bs, key_scale=ks).cpu()
+    assert_scores(score, *bo.scores(q, ref[4], lengths, near, SCALE, bs, ref[2]))
+    got = pa.select_blocks(*cuda(score, lengths, tables), bs, 5)
+    assert torch.equal(got[0].cpu() - (nb - 13), bo.select(score, lengths, near, bs, 5)[0])
+
+
+# ----------------------------------------------------------------------------- KV-partition sharding
+@pytest.mark.gpu
+@pytest.mark.parametrize("world", [1, 2, 4])
+@pytest.mark.parametrize("bs,query_len", [(16, 1), (64, 2), (1024, 1)])
+def test_sharded_decode_with_block_scales(bs, query_len, world):
+    """Each rank's maxima are those of logit + log(value scale): ranks whose pages have scales far apart merge all the same."""
+    c = Cache([3000, 257, 1100, 60], 2, bs, seed=world)
+    for s, n in enumerate(c.lengths.tolist()):      # the pages of the context's second half: values a thousand times smaller
+        late = c.tables[s, -(-n // bs) // 2:-(-n // bs)].long()
+        c.vs[late] *= 2.0 ** -10
+    q = c.query(4, query_len)
+    kc, vc, ks, vs, tables, dq = cuda(c.key, c.value, c.ks, c.vs, c.tables, q)
+    plan = plan_kv_shards(c.lengths.tolist(), world, max(256, bs), query_len)
+    triples = [decode_kv_shard(dq, kc, vc, plan[r], local_block_table(tables, plan[r], bs), SCALE, ks, vs) for r in range(world)]
+    got = merge_triples_cuda(*(torch.stack([t[i] for t in triples]) for i in range(3)))
+    want = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, query_len)
+    assert_attention(got.view(q.shape).cpu(), want)
+    if world == 1:
+        dec = KvShardedDecoder(dq, kc, vc, plan[0], tables, SCALE, ks, vs)
+        assert_attention(dec.step().cpu(), want)
+        assert dec.params.tmp_dtype == _lib.PA_DT_F32
 
 
 # ----------------------------------------------------------------------------- host threads
