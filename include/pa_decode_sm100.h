@@ -365,8 +365,9 @@ int pa_cache_append_sm100(const PaCacheAppendParams* params, void* stream);
  * Page scores (no counterpart in the reference): for every page i of a sequence's table that holds a
  * token of its context
  *   scores[s, h, i] = key_scale[page, h] * max_r softmax_scale * qs_r * sum_d max(q_rd lo_d, q_rd hi_d)
- * over the query rows r of kv head h, where (lo, hi) = key_bounds[page, h]: no logit of the group
- * with a key of the page is larger.  Entries past the last such page become -inf; a query row that
+ * over the query rows r of kv head h, where (lo, hi) = key_bounds[page, h].  In exact arithmetic no logit of the
+ * group with a key of the page is larger; the sums are rounded to 32 bits (not upwards), so a score may fall short of
+ * that bound by 260 * 2^-23 of the sum of its terms' magnitudes.  Entries past the last such page become -inf; a query row that
  * holds a NaN makes the scores of its kv head NaN.  The sum is taken as q+ . hi + q- . lo (the positive and the
  * negative part of the row): an infinite element makes it infinite, or NaN where it meets a bound of zero or an
  * infinity of the other sign.

@@ -78,7 +78,7 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
 
     ``scores[s, h, i] = key_scale * max_r softmax_scale * query_scale_r * sum_d max(q_rd lo_d, q_rd hi_d)``
     over the query rows ``r`` of kv head ``h`` (all query tokens), ``lo`` and ``hi`` the page's key
-    bounds; ``-inf`` for entries past the sequence's last page, NaN where a query row holds one (an infinite
+    bounds (sums in 32 bits, rounded to nearest or truncated: a bound to choose pages by, not a proof); ``-inf`` for entries past the sequence's last page, NaN where a query row holds one (an infinite
     element gives infinity, or NaN where it meets a bound of zero).  ``query`` as in
     ``paged_attention_decode`` (bf16, or e4m3fn with ``query_scale``); ``key_bounds`` e4m3fn
     ``[num_blocks, num_kv_heads, 2, head_size]``; ``key_scale`` ``None``, per tensor or
