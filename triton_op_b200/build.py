@@ -42,6 +42,9 @@ def _nvcc() -> str:
     return exe
 
 
+CALLS_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+
+
 def _calls_command() -> list:
     import sysconfig
 
@@ -53,7 +56,7 @@ def _calls_command() -> list:
     for path in include:
         flags += ["-isystem", path]
     libs = ["-L" + os.path.join(root, "lib")] + ["-l" + n for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")]
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"] + flags + ["-o", CALLS_PATH, os.path.join(CSRC, CALLS_SOURCE)] + libs
+    return ["g++"] + CALLS_FLAGS + flags + ["-o", CALLS_PATH, os.path.join(CSRC, CALLS_SOURCE)] + libs
 
 
 def _object(source: str) -> str:
@@ -62,40 +65,84 @@ def _object(source: str) -> str:
     return os.path.join(LIB_DIR, os.path.splitext(source)[0] + ".o")
 
 
-def _stale(target: str, source: str) -> bool:
+def _how(source: str, trace: bool = False) -> str:
+    """What a product depends on besides its sources' times; kept beside it.  (No paths: a built tree may be moved.)"""
+    if source != CALLS_SOURCE:
+        return " ".join(_cuda_flags(trace))
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return ""
+    return " ".join(CALLS_FLAGS + [torch.__version__, str(torch._C._GLIBCXX_USE_CXX11_ABI), str(sysconfig.get_config_var("SOABI"))])
+
+
+def _cuda_flags(trace: bool) -> list:
+    return NVCC_FLAGS + (["-DPA_TRACE_BUILD"] if trace else [])
+
+
+def _built_so(source: str, trace: bool) -> bool:
+    """The product was built the way it would be built now."""
+    try:
+        with open(_object(source) + ".how") as f:
+            return f.read() == _how(source, trace)
+    except OSError:
+        return False
+
+
+def _note(source: str, trace: bool) -> None:
+    with open(_object(source) + ".how", "w") as f:
+        f.write(_how(source, trace))
+
+
+def _older(target: str, source: str) -> bool:
     if not os.path.exists(target):
         return True
     built = os.path.getmtime(target)
     return any(os.path.getmtime(os.path.join(CSRC, d)) > built for d in [source] + SOURCES[source])
 
 
-def needs_build() -> bool:
-    return any(_stale(CALLS_PATH if s == CALLS_SOURCE else LIB_PATH, s) for s in SOURCES)
+def needs_build(trace: bool = False) -> bool:
+    return any(_older(CALLS_PATH if s == CALLS_SOURCE else LIB_PATH, s) or not _built_so(s, trace) for s in SOURCES)
 
 
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
-    """Compile the library if it is missing or older than its sources; returns its path.
-    ``trace`` adds the instantiations that stamp SM clocks into ``PaDecodeParams.trace`` (tuning aid)."""
-    if not force and not needs_build():
+    """Compile what is missing, older than its sources or built in another way (other flags; for the host
+    calls, another torch or Python); returns the CUDA library's path.
+    ``trace`` adds the instantiations that stamp SM clocks into ``PaDecodeParams.trace`` (tuning aid).
+    The CUDA library needs neither torch nor its headers: it is there even where the host calls fail to compile,
+    which is raised at the end."""
+    if not force and not needs_build(trace):
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    flags = NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + (["-DPA_TRACE_BUILD"] if trace else [])
-    jobs = {s: subprocess.Popen(_calls_command() if s == CALLS_SOURCE else
-                                [_nvcc()] + flags + ["-c", "-o", _object(s), os.path.join(CSRC, s)],
-                                stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-            for s in SOURCES if force or _stale(_object(s), s)}
-    logs = {s: (job.communicate()[0], job.returncode) for s, job in jobs.items()}
-    for s, (text, code) in logs.items():
-        if code != 0:
-            if os.path.exists(_object(s)):
-                os.remove(_object(s))
-            raise RuntimeError(f"the compiler failed on {s}:\n{text}")
-        if verbose:
-            sys.stderr.write(text)
-    proc = subprocess.run([_nvcc()] + NVCC_FLAGS + ["-shared", "-o", LIB_PATH] + [_object(s) for s in SOURCES if s != CALLS_SOURCE],
-                          capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+    cuda = [s for s in SOURCES if s != CALLS_SOURCE]
+    todo = [s for s in SOURCES if force or _older(_object(s), s) or not _built_so(s, trace)]
+    jobs, logs = {}, {}
+    for s in todo:
+        if os.path.exists(_object(s) + ".how"):
+            os.remove(_object(s) + ".how")       # until it is built and linked
+        try:
+            command = (_calls_command() if s == CALLS_SOURCE else
+                       [_nvcc()] + _cuda_flags(trace) + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", _object(s), os.path.join(CSRC, s)])
+            jobs[s] = subprocess.Popen(command, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        except (OSError, ImportError) as e:      # no such compiler, no torch
+            logs[s] = (str(e), -1)
+    logs.update({s: (job.communicate()[0], job.returncode) for s, job in jobs.items()})
+    failed = [s for s in todo if logs[s][1] != 0]
+    for s in todo:
+        if s in failed and os.path.exists(_object(s)):
+            os.remove(_object(s))
+        elif verbose:
+            sys.stderr.write(logs[s][0])
+    if not any(s in cuda for s in failed):
+        proc = subprocess.run([_nvcc()] + NVCC_FLAGS + ["-shared", "-o", LIB_PATH] + [_object(s) for s in cuda], capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+        for s in todo:
+            if s not in failed:
+                _note(s, trace)
+    if failed:
+        raise RuntimeError("\n".join(f"the compiler failed on {s}:\n{logs[s][0]}" for s in failed))
     return LIB_PATH
 
 
