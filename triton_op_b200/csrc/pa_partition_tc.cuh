@@ -1636,7 +1636,7 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
       // lane r holds head dim r of every row: 2-byte stores, 64 contiguous bytes per warp and row, or (block
       // scales, where the workspaces are the call's own) 4-byte stores that round nothing: the error against 64
       // bits is then the bf16 result's alone, 0.0017 of the norm where partials in bf16 made it 0.0023, and a call
-      // takes 1 % longer at most, with 16 rows 5 % (48 sequences of 1 023 to 8 191 tokens: 105 -> 110 us)
+      // takes 1 % longer at most, with 16 rows 5 % (48 sequences of 1 023 to 8 191 tokens: 93 -> 97-99 us)
       const bool whole = BLK && p.tmp_f32 != 0;
       uint8_t* dst = p.tmp_out + ((int64_t)it.seq * p.tmp_stride_seq + (int64_t)it.head * p.tmp_stride_head +
                                   (int64_t)it.part * p.tmp_stride_part + (int64_t)(it.rb * QR) * p.tmp_stride_row + r) * (whole ? 4 : 2);

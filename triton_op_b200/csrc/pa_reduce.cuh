@@ -299,7 +299,8 @@ __device__ __forceinline__ void finish_row(const ReduceParams& p, const RowRef& 
 // after the other; with WPR = 16 the warps of a CTA take the 32-partition chunks of ONE row
 // round-robin and combine their running (max, sum, weighted output) through shared memory.
 // (Rows of up to 128 partitions have a kernel of their own below.)
-// F32: the partial outputs are fp32 (twice the registers for a row in flight, so fewer rows).
+// F32: the partial outputs are fp32.  A row in flight takes twice the registers, so fewer are (one warp a row: eight;
+// with sixteen a call of 48 sequences of 1 023 to 8 191 tokens and 16 rows took 102 us, with eight it takes 97-99).
 template <int WPR, bool F32>
 __global__ void __launch_bounds__(WPR == 1 ? 128 : 512) pa_reduce_kernel(const __grid_constant__ ReduceParams p) {
   static_assert(WPR == 1 || WPR == 16, "one warp per row (four rows per CTA) or sixteen");
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : 512) pa_reduce_kernel(const _
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   float W = 0.f;
   // rows in flight: a 16-warp row has one 32-partition chunk per warp, taken in one round trip
-  reduce_chunks<WPR == 16 ? (F32 ? 16 : 32) : 16, F32>(p, a, slice, WPR, lane, M, W, acc);
+  reduce_chunks<WPR == 16 ? (F32 ? 16 : 32) : (F32 ? 8 : 16), F32>(p, a, slice, WPR, lane, M, W, acc);
   if (WPR > 1) {
     // combine the warps' partial results: warp `slice` holds (M, W, acc) of its chunks
     __shared__ float s_m[kWarps], s_w[kWarps];
