@@ -382,7 +382,7 @@ typedef struct PaBlockScoreParams {
   const float* key_scale;      /* see kv_quant_mode: none, per tensor or per block */
   float* scores;               /* [S, Hkv, max_blocks_per_seq] */
   int32_t* status;             /* optional */
-  int32_t num_seqs, num_kv_heads;
+  int32_t num_seqs, num_kv_heads;   /* at least 17 800 sequences fit (an index of them lies in shared memory) */
   int32_t rows;                /* query rows per kv head, 1..64 */
   int32_t head_size, block_size, num_blocks, max_blocks_per_seq;
   int32_t q_dtype, q_quant_mode, kv_quant_mode;

@@ -152,8 +152,8 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Ten
     code of every head dim over the page's tokens, kept up to date for
     :func:`triton_op_b200.score_blocks`.  ``status`` (int32 scalar) receives ``PA_DEV_*`` bits for rows
     that have no place; they are skipped.  No page may get rows of two sequences in a call; what is
-    written (scales, codes and bounds of each page and kv head) may not share memory.  Runs on
-    the current stream; there is no CPU fallback.
+    written (scales, codes and bounds of each page and kv head) may not share memory.  At most 8 192
+    sequences.  Runs on the current stream; there is no CPU fallback.
     """
     done = _lib.calls().append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables, sequence_lengths,
                                query_start_loc, key_bounds, status)

@@ -13,7 +13,8 @@
 // counters are only added to: the same scores give the same table whatever the order of the threads.
 //
 // What bounds it: 4 bytes per page and kv head, a few MB at most; it is the latency of one CTA's chain
-// (lengths and scores, range, histogram, rank, ordered pass: six block barriers).  So keys stay in
+// (lengths and scores, range, histogram, rank, ordered pass: six block barriers), and in wide tables the warps that
+// hold the context: a warp owns neighbouring rows of the table's width, so those past a shorter context have none.  So keys stay in
 // registers, a warp's pages are rows of 32 (coalesced loads, ballots give a page's place among
 // the warp's), every warp combines the block's partial results for itself instead of waiting for
 // one that does, and the CTA is as large as the table is wide.

@@ -26,8 +26,9 @@
 // warps take the runs in turn.  A page of 64 has four warps, or one where each gets a few rows.  Keys are
 // stored as 16-byte chunks [d/16][token][16], values as 16 tokens of a head dim, 16 bytes too;
 // values of a run that is not whole are merged with the bytes that are there.
-// What bounds it: 512 bytes read and 256 written per (token, kv head).  A prompt is bound by the
-// instructions that quantise it: 16 000 tokens of eight kv heads take 22 us in pages of 16, 25 in pages of 64 and 33 in
+// What bounds it: 512 bytes read and 256 written per (token, kv head).  A prompt in pages of 16 fills nothing alone:
+// 59 % of the issue slots, 56 % of the ALU pipe, 71 % of the copy bandwidth, its warps waiting for their loads more than
+// for anything else.  16 000 tokens of eight kv heads take 22 us in pages of 16, 25 in pages of 64 and 33 in
 // pages of 1024 (15 at the copy bandwidth).  A row for each of 64 sequences takes 4.3, 5.1 and 9.1 us: launch
 // latency and one chain of loads, which is why whatever a page holds already is asked for at once.
 #pragma once
@@ -341,7 +342,7 @@ pa_cache_append_kernel(const __grid_constant__ CacheAppendParams p) {
     // Registers that keys use for the smallest (0 .. 7) and largest (8 .. 15) of a lane's head dims, and
     // values for the codes that share a run with new ones.  Those are asked for here, with the scale: after
     // the barrier below they would be read from sectors that another warp has just written half of, which took
-    // 67 us where this takes 49 (64 sequences of 448 rows into pages of 64, the first page begun inside a run).
+    // 67 us where this takes 49 (64 sequences of 448 rows into pages of 64, the first page begun inside a run; 73 and 49 for 1 to 900 rows)
     uint32_t ext[16];
     // (A page of 16 belongs to one warp, which reads its codes when it needs them: the registers are worth more.)
     constexpr bool kEarly = BS > 16;

@@ -82,7 +82,7 @@ def score_blocks(query: torch.Tensor, key_bounds: torch.Tensor, sequence_lengths
     element gives infinity, or NaN where it meets a bound of zero).  ``query`` as in
     ``paged_attention_decode`` (bf16, or e4m3fn with ``query_scale``); ``key_bounds`` e4m3fn
     ``[num_blocks, num_kv_heads, 2, head_size]``; ``key_scale`` ``None``, per tensor or
-    ``[num_blocks, num_kv_heads, 1, 1]``; ``scores``: an output tensor to use.
+    ``[num_blocks, num_kv_heads, 1, 1]``; ``scores``: an output tensor to use.  At most 17 800 sequences.
     """
     if query_scale is None and scores is None:
         done = _lib.calls().scores(query, key_bounds, sequence_lengths, block_tables, softmax_scale, query_sequence_length,
@@ -248,7 +248,7 @@ def sparse_attention_decode(output: torch.Tensor, query: torch.Tensor, key_cache
     """Decode attention of every kv head over its best ``top_k`` pages: :func:`score_blocks`,
     :func:`select_blocks` and ``paged_attention_decode``.  Arguments as there (e4m3fn caches; scales
     ``None``, per tensor or ``[num_blocks, num_kv_heads, 1, 1]``); ``keep_last`` defaults to 1, or 2 with
-    several query tokens.  A sequence of at most ``top_k`` pages gets its full attention.  Returns
+    several query tokens; at most 5 199 sequences (2 639 with more than eight query rows a kv head).  A sequence of at most ``top_k`` pages gets its full attention.  Returns
     ``paged_attention_decode``'s dictionary with the ``block_tables`` and ``sequence_lengths`` that were read.
     """
     if key_cache.dim() != 5:
