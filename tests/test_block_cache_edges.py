@@ -8,7 +8,7 @@ import torch
 
 import triton_op_b200 as pa
 from oracle import blocks_oracle as bo
-from test_block_cache import D, FP8, SCALE, Cache, assert_attention, assert_same, cuda, decode, serve
+from test_block_cache import D, FP8, SCALE, Cache, assert_attention, assert_same, cuda, decode, serve, transposed
 from triton_op_b200 import PaArgumentError, _lib
 from triton_op_b200.pa_decode import build_params
 from triton_op_b200.sharding import KvShardedDecoder, decode_kv_shard, local_block_table, merge_triples_cuda, plan_kv_shards
@@ -412,6 +412,93 @@ def test_served_selections_are_those_of_the_scores(bs, query_len, group):
                 sure += 1
                 assert torch.equal(got[s, h], tables[s, h])
     assert sure >= 12                                                  # of 24 selections: the comparison is not an empty one
+
+
+def strided_pool(c):
+    """The same pool as views of one allocation: a page's keys, values and scales side by side, heads apart."""
+    room = torch.zeros(c.nb, c.hkv, 2, D * c.bs + 32, dtype=torch.uint8, device="cuda")
+    key = room[:, :, 0, :D * c.bs].unflatten(2, (D // 16, c.bs, 16)).view(FP8)
+    value = room[:, :, 1, 16:D * c.bs + 16].unflatten(2, (D, c.bs)).view(FP8)
+    key.view(torch.uint8).copy_(c.key.view(torch.uint8))
+    value.view(torch.uint8).copy_(c.value.view(torch.uint8))
+    scales = torch.stack((c.ks, c.vs), 2).cuda()
+    return key, value, scales[:, :, 0], scales[:, :, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 64, 1024])
+@pytest.mark.parametrize("form", ["plain", "one pool", "transposed", "no scales", "one value", "fp8 query", "fp8 query rows", "sinks", "64 rows", "keeps"])
+def test_sparse_decode_in_every_form(form, bs):
+    """What paged_attention_decode takes, sparse_attention_decode takes: the exact selection of the kernel's scores, and
+    the attention over it."""
+    query_len, group = (4, 16) if form == "64 rows" else (1, 4)
+    c = Cache([9 * bs + 5, 40, 3 * bs, 0, 7 * bs + bs // 2 + 1], 2, bs, seed=bs + len(form))
+    q, bounds = c.query(group, query_len), c.bounds()
+    kc, vc, ks, vs = cuda(c.key, transposed(c.value) if form == "transposed" else c.value, c.ks, c.vs)
+    kw, ref, scale, top_k, first, last = {}, {}, {}, 5, 1, 1 if query_len == 1 else 2
+    oks, ovs = c.ks, c.vs
+    if form == "one pool":
+        kc, vc, ks, vs = strided_pool(c)
+    elif form == "no scales":
+        ks = vs = oks = ovs = None
+    elif form == "one value":
+        ks, vs, oks, ovs = 0.02, 0.03, torch.tensor(0.02), torch.tensor(0.03)
+    elif form.startswith("fp8"):
+        q = (q.float() * 40).to(FP8)
+        scale = dict(query_scale=torch.tensor(1 / 40) if form == "fp8 query" else torch.rand(5, 8, 1, generator=c.g) / 20 + 0.01)
+    elif form == "sinks":
+        ref["sink_tokens"] = torch.linspace(-2, 3, 8)
+        kw["sink_tokens"] = ref["sink_tokens"].cuda()
+    elif form == "keeps":
+        first, last = 0, 4
+    out = torch.full(q.shape, math.nan, dtype=torch.bfloat16, device="cuda")
+    dq, db, dl, dt = cuda(q, bounds, c.lengths, c.tables)
+    dscale = {k: v.cuda() for k, v in scale.items()}
+    status = torch.zeros((), dtype=torch.int32, device="cuda")
+    res = pa.sparse_attention_decode(out, dq, kc, vc, db, dl, dt, SCALE, query_len, top_k, dscale.get("query_scale"), ks, vs,
+                                     keep_first=first, keep_last=last, status=status, **kw)
+    assert int(status) == 0 and res["final_output"] is out
+    score = pa.score_blocks(dq, db, dl, dt, SCALE, query_len, bs, key_scale=ks, **dscale).cpu()
+    assert_scores(score, *bo.scores(q, bounds, c.lengths, c.tables, SCALE, bs, oks, **scale))
+    tables, tokens = bo.select(score, c.lengths, c.tables, bs, top_k, first, last)
+    assert torch.equal(res["block_tables"].cpu(), tables) and torch.equal(res["sequence_lengths"].cpu(), tokens)
+    assert_attention(out.cpu(), bo.attention(q, c.key, c.value, oks, ovs, tables, tokens, SCALE, query_len, **ref, **scale), form)
+    again = torch.empty_like(out)
+    for _ in range(5):
+        pa.sparse_attention_decode(again, dq, kc, vc, db, dl, dt, SCALE, query_len, top_k, dscale.get("query_scale"), ks, vs,
+                                   keep_first=first, keep_last=last, **kw)
+        assert torch.equal(again, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 64, 1024])
+def test_append_to_a_pool_of_views(bs):
+    counts, before = [5, 33, 1], [13, 20, 0]
+    c = Cache([18, 53, 1], 2, bs, seed=11)
+    start = torch.tensor([0, 5, 38, 39], dtype=torch.int32)
+    key, value = torch.randn(39, 2, D, generator=c.g).bfloat16(), torch.randn(39, 2, D, generator=c.g).bfloat16()
+    views = strided_pool(c)
+    bounds = c.bounds().cuda()
+    pa.append_kv_cache(*cuda(key, value), *views, *cuda(c.tables, c.lengths, start), key_bounds=bounds)
+    want = [c.key.clone(), c.value.clone(), c.ks.clone(), c.vs.clone(), c.bounds()]
+    bo.append(key, value, *want[:4], c.tables, c.lengths, start, want[4])
+    assert_same([t.cpu() for t in (*views, bounds)], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 1024])
+def test_decode_without_allocation_with_block_scales(bs):
+    """The library's own array holds bf16 partial outputs, whatever the parameter block says of its workspaces."""
+    c = Cache([700, 40, 0], 2, bs, seed=19)
+    q = c.query(4)
+    out = torch.full(q.shape, math.nan, dtype=torch.bfloat16, device="cuda")
+    dev = cuda(q, c.key, c.value, c.lengths, c.tables, c.ks, c.vs)
+    p, keep = build_params(out, *dev[:5], SCALE, 1, 700, None, None, *dev[5:], None, 256, None, None, None, None, None)
+    assert p.tmp_dtype == _lib.PA_DT_F32
+    p.exp_sums = p.max_logits = p.tmp_out = None
+    _lib.check(_lib.lib().pa_decode_noalloc_sm100(C.byref(p), torch.cuda.current_stream().cuda_stream), "pa_decode_noalloc_sm100")
+    assert_attention(out.cpu(), bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1))
+    del keep
 
 
 @pytest.mark.gpu
