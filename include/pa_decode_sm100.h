@@ -187,6 +187,10 @@ int pa_decode_sm100(const PaDecodeParams* params, void* stream);
  */
 int pa_decode_tables_sm100(const PaDecodeParams* params, int64_t bt_stride_head, void* stream);
 
+/* (With per-block scales or tmp_dtype PA_DT_F32 a NaN that a row attends to -- in its query, a key, a value or a scale --
+ * makes its output NaN, as an infinite query element does.  With the other forms a partition whose sum of weights is
+ * NaN weighs nothing.) */
+
 /* The partition kernel alone: fills exp_sums / max_logits / tmp_out, leaves `out` untouched. */
 int pa_partition_sm100(const PaDecodeParams* params, void* stream);
 

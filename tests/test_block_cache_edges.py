@@ -121,6 +121,80 @@ def test_timed_calls_keep_their_workspaces():
     assert torch.equal(plain["maximum_logits"][0], res[0]["maximum_logits"][0])
 
 
+def at_token(c, cache, seq, token, head):
+    """(page, slot) of a token, and a writable uint8 view of its page and kv head."""
+    page, slot = int(c.tables[seq, token // c.bs]), token % c.bs
+    return cache.view(torch.uint8)[page, head], slot
+
+
+def assert_attention_but(got, want, nan):
+    """The attention wherever `nan` [S, heads, D] is false, NaN wherever it is true."""
+    assert torch.equal(got.isnan(), nan), (int(got.isnan().sum()), int(nan.sum()), int((got.isnan() & nan).sum()))
+    out, mass, floor = want
+    err = (got.double() - out).abs()
+    assert bool((err <= bo.attention_tolerance(out, mass, floor))[~nan].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [200, 2000, 9000, 36000])
+@pytest.mark.parametrize("bs,group,query_len", [(16, 4, 1), (64, 8, 1), (1024, 4, 4)])
+def test_what_is_no_number_stays_none(bs, group, query_len, tokens):
+    """A NaN that a row attends to reaches that row, whichever partition it lies in, and no other row; so does an infinite
+    query element, whose logits have no softmax."""
+    c = Cache([tokens, 700, 300, 500, 40], 2, bs, seed=tokens + bs)
+    q = c.query(group, query_len)
+    want = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, query_len)
+    rows = group * query_len
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    q[0, 1, 17], nan[0, 1] = math.nan, True                             # a query row of head 0
+    q[1, rows, 3], nan[1, rows] = math.inf, True                        # one of head 1
+    page, slot = at_token(c, c.key, 0, tokens // 2, 1)                  # a key element: every row of the head
+    page[3, slot, 5], nan[0, rows:] = 0x7f, True
+    page, slot = at_token(c, c.value, 1, 650, 0)                        # a value element: its head dim
+    page[77, slot], nan[1, :rows, 77] = 0xff, True
+    c.ks[int(c.tables[2, 0]), 0], nan[2, :rows] = math.nan, True        # scales of pages in use
+    c.vs[int(c.tables[3, 0]), 1], nan[3, rows:] = math.nan, True
+    assert_attention_but(decode(c, q, query_len=query_len), want, nan)
+    if query_len == 1:                                                   # tables per head, and the pieces of a sharded call
+        heads = c.tables[:, None].expand(-1, 2, -1).contiguous()
+        assert_attention_but(decode(c, q, tables=heads), want, nan)
+        kc, vc, ks, vs, tables, dq = cuda(c.key, c.value, c.ks, c.vs, c.tables, q)
+        plan = plan_kv_shards(c.lengths.tolist(), 2, max(256, bs), 1)
+        triples = [decode_kv_shard(dq, kc, vc, plan[r], local_block_table(tables, plan[r], bs), SCALE, ks, vs) for r in range(2)]
+        got = merge_triples_cuda(*(torch.stack([t[i] for t in triples]) for i in range(3)))
+        assert_attention_but(got.view(q.shape).cpu(), want, nan)
+
+
+@pytest.mark.gpu
+def test_what_is_no_number_stays_none_among_many_rows():
+    """Rows of 33 to 128 partitions among many short ones, which eight warps share: a NaN in a later chunk of 32, and
+    rows that are NaN throughout."""
+    c = Cache([9000, 20000] + [300] * 40, 2, 16, seed=77)
+    q = c.query(8)
+    want = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1)
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    page, slot = at_token(c, c.key, 0, 8700, 1)
+    page[0, slot, 0], nan[0, 8:] = 0x7f, True
+    for row in (0, 5):
+        q[1, row, 100], nan[1, row] = math.nan, True
+    q[7, 3, 1], nan[7, 3] = -math.inf, True
+    assert_attention_but(decode(c, q), want, nan)
+
+
+@pytest.mark.gpu
+def test_what_is_no_number_stays_none_in_the_callers_workspaces():
+    c = Cache([900, 40], 2, 16, seed=6)
+    q = c.query(4)
+    want = bo.attention(q, c.key, c.value, c.ks, c.vs, c.tables, c.lengths, SCALE, 1)
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    q[0, 2, 0], nan[0, 2] = math.nan, True
+    for dtype in (torch.float32, torch.bfloat16):
+        shape = (2, 2, 4, 4)
+        got = decode(c, q, exp_sums=torch.empty(shape, device="cuda"), max_logits=torch.empty(shape, device="cuda"),
+                     tmp_output=torch.empty(*shape, D, dtype=dtype, device="cuda"))
+        assert_attention_but(got, want, nan)
+
+
 # ----------------------------------------------------------------------------- scores
 def scores_of(q, bounds, lengths, tables, bs, ks, query_len=1, **kw):
     return pa.score_blocks(*cuda(q, bounds, lengths, tables), SCALE, query_len, bs, key_scale=cuda(ks), **kw).cpu()

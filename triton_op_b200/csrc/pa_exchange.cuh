@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(128) pa_merge_wait_kernel(const __grid_constan
                wait_line(src + 2 + 2 * lane, step, b[j]);
           ok = __all_sync(kFullMask, ok);
           const float ms = __uint_as_float(h[j].x), ls = __uint_as_float(h[j].z);
-          if (ok && ls > 0.f && ms > -INFINITY) {
+          if (ok && ((ls > 0.f && ms > -INFINITY) || ls != ls)) {   // (a shard whose sum is NaN makes the row NaN)
             const float newM = fmaxf(M, ms);
             const float f = (M == -INFINITY) ? 0.f : expf(M - newM);
             const float w = ls * expf(ms - newM);

@@ -1054,7 +1054,10 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
             qs = __ldg(p.q_scale + (int64_t)it.seq * p.q_scale_stride_seq + it.head * p.eqG + row);
           // the row's positive factor that turns a raw product into a base-2 logit (> 0 always, so that
           // a masked -inf stays -inf and maxima commute with the factor)
-          sts32(aux + n * 4, __float_as_uint(fmaxf(inv_pre * qs * q_base_scale, 1e-30f)));
+          float factor = fmaxf(inv_pre * qs * q_base_scale, 1e-30f);
+          // (block scales: a row that holds a NaN or an infinity has no softmax, and its output says so)
+          if (BLK && ((!p.q_is_fp8 && be == 255) || qs != qs)) factor = __uint_as_float(0x7fc00000u);
+          sts32(aux + n * 4, __float_as_uint(factor));
           if (ALIBI)   // slope of the row's query head, in the base-2 logit domain
             sts32(aux + kQSlope + n * 4, __float_as_uint(row < p.eqG ? __ldg(p.alibi + it.head * p.G + row % p.G) * kLog2e : 0.f));
         }
@@ -1273,7 +1276,8 @@ pa_partition_fp8_tc_kernel(const __grid_constant__ KernelParams p, const __grid_
           } else {
             const int pg = BS == 16 ? (tok[tg] >> 4) : (BS == 64 ? (tok[tg] >> 6) : 0);
             ks_blk[tg] = __uint_as_float(lds32(item_aux + kQTokScales + pg * 4));
-            const float vs = fmaxf(__uint_as_float(lds32(item_aux + kQTokScales + (16 + pg) * 4)), 0x1p-100f);
+            float vs = __uint_as_float(lds32(item_aux + kQTokScales + (16 + pg) * 4));
+            vs = vs < 0x1p-100f ? 0x1p-100f : vs;   // (NaN stays)
             lv_blk[tg] = __log2f(vs);
             iv_blk[tg] = __fdividef(1.0f, vs);
           }

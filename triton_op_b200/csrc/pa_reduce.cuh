@@ -52,6 +52,7 @@ struct ReduceParams {
   const int32_t* push_counter;  // push_step == 0: the step is push_counter[1] + 1 (steps merged so far, + 1)
   int32_t push_world, push_rank, push_step;
   int32_t S, Hkv, eqG, G, partition_size, max_partitions, ctx_cap;
+  int32_t keep_nan;             // a partition whose sum is NaN makes the row NaN; 0: it weighs nothing
   int64_t out_stride_seq, out_stride_head;
   int64_t ws_stride_seq, ws_stride_head, ws_stride_part;
   int64_t tmp_stride_seq, tmp_stride_head, tmp_stride_part, tmp_stride_row;
@@ -225,7 +226,8 @@ __device__ __forceinline__ void reduce_chunks(const ReduceParams& p, const RowRe
       W *= f;
       M = newM;
     }
-    const float w = (l > 0.f && m > -INFINITY) ? l * expf(m - M) : 0.f;
+    float w = (l > 0.f && m > -INFINITY) ? l * expf(m - M) : 0.f;
+    if (p.keep_nan && l != l) w = l;
     for (int j0 = 0; j0 < cnt; j0 += FLIGHT) {
       if (j0 > 0) request(j0);
 #pragma unroll
@@ -243,7 +245,7 @@ __device__ __forceinline__ void reduce_chunks(const ReduceParams& p, const RowRe
 // Folds one more warp's (maximum, weight sum, weighted output) into a combination relative to the
 // common maximum mx (the order of these calls is the order of the additions).
 __device__ __forceinline__ void fold_partial(float ms, float ws, const float4& a, float mx, float& W, float (&acc)[4]) {
-  if (!(ms > -INFINITY)) return;    // that warp saw no partition with weight
+  if (!(ms > -INFINITY) && ws == ws) return;    // that warp saw no partition with weight
   const float f = expf(ms - mx);
   W = fmaf(ws, f, W);
   acc[0] = fmaf(a.x, f, acc[0]);
@@ -455,7 +457,7 @@ pa_merge_triples_kernel(uint8_t* out, int64_t out_stride_row, const float* __res
   for (int s = 0; s < num_shards; ++s) {
     const float ls = l[(int64_t)s * ml_stride + row];
     const float ms = m[(int64_t)s * ml_stride + row];
-    if (!(ls > 0.f) || !(ms > -INFINITY)) continue;
+    if (ls == ls && (!(ls > 0.f) || !(ms > -INFINITY))) continue;   // (a shard whose sum is NaN makes the row NaN)
     const float w = ls * expf(ms - M);
     const float4 v = *reinterpret_cast<const float4*>(o + (int64_t)s * o_stride + row * kD + 4 * lane);
     W += w;

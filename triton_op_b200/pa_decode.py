@@ -656,6 +656,8 @@ def paged_attention_decode(
     ``maximum_logits`` / ``exponential_sums`` then refer to logit + log(value scale) of the token, and
     ``temporary_output`` is fp32 (a ``tmp_output`` in the output dtype, which is taken with per-page
     scales, rounds each partition's output once more).  Value scales below 2**-100 count as 2**-100.
+    A NaN that a row attends to (its query, a key, a value, a scale) makes it NaN, and so does an infinite
+    query element; with the other forms a partition whose sum is NaN weighs nothing.
 
     Keyword-only additions: ``partition_size`` (reference constant 256); ``exp_sums`` /
     ``max_logits`` ``[num_seqs, num_kv_heads, P, eq_group]`` fp32 and ``tmp_output``
