@@ -79,6 +79,8 @@ typedef enum PaVLayout {
  * r = t*G + g holds new token t (0..L-1) of head g; row r attends key j iff
  * (L-1-t) + j < context_len (pa_decode_triton_gluon_fp8.py:915-920).
  */
+/* Zero the block before filling it in: a field of 0 asks for what the library did before it knew the field
+ * (tmp_dtype lies in what used to be the block's padding). */
 typedef struct PaDecodeParams {
   uint32_t struct_size;        /* = sizeof(PaDecodeParams) */
   uint32_t abi_version;        /* = PA_ABI_VERSION */
